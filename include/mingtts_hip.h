@@ -94,8 +94,9 @@ enum {
 };
 
 /* Element types.  Weights and bias are 16-bit; activations x may be any of the
- * three; y is always fp32 (an fp16/bf16 output alone would break 1e-3). */
-typedef enum mt_dtype { MT_F32 = 0, MT_F16 = 1, MT_BF16 = 2 } mt_dtype;
+ * first three; y is always fp32 (an fp16/bf16 output alone would break 1e-3).
+ * MT_F8 is the 8-bit format described at mt_kv; only the entry points below that name it take it. */
+typedef enum mt_dtype { MT_F32 = 0, MT_F16 = 1, MT_BF16 = 2, MT_F8 = 3 } mt_dtype;
 
 /* Kernel families, as reported by mt_linear_kernel: the lane-group GEMV (every 16-byte
  * weight chunk feeds all rows of x), the MFMA GEMM (tiles of x rows and weight rows), and
@@ -401,6 +402,110 @@ int mt_attention_decode(const float *q, uint32_t ldq, uint32_t B, uint32_t hq, u
                         const void *v_cache, mt_dtype cache_t, uint32_t cache_len,
                         uint64_t cache_stride, float *out, uint32_t ldo, float scale,
                         mt_stream_t stream);
+
+/*
+ * Caches and weights in 8 bits, and batches that share a prefix.  No counterpart in the reference
+ * (it keeps fp32 caches and bf16 weights, and runs one utterance at a time).
+ *
+ * The format MT_F8: OCP e4m3 codes (largest value 448, no infinities, codes 0x7F and 0xFF NaN) in
+ * blocks with one scale byte s each, which stands for 2^(s - 127).  A block is written with the
+ * least scale, 2^-126 or more, at which its largest finite |x| is at most 448, and x / scale
+ * rounded to nearest, ties to even; infinities and NaN become NaN.  Scale bytes are 1 .. 254 (written
+ * ones at most 247).  A stored value is off by at most 2^-4 of itself, or 2^-10 of the scale where that is
+ * more, and is exactly a bf16 number.  In a cache a block is the 64 values of one head at one position; in a
+ * matrix it is 128 consecutive values of a row (the last block of a row may be shorter).
+ *
+ * mt_kv -- the caches of one layer for a batch of sequences: k and v [hkv, cache_len, 64] of type
+ * cache_t (MT_F32, MT_F16 or MT_F8), 16-byte aligned, each sequence's `stride` elements behind the
+ * one before (a multiple of 16; not read for one sequence); with MT_F8 also k_scale and v_scale
+ * [hkv, cache_len] bytes, 4-byte aligned, scale_stride bytes a sequence (a multiple of 4), and
+ * cache_len a multiple of 4.  cache_len is at most 2^30.
+ *
+ * Rows: the calls below take B sequences of T rows each, row b T + t being sequence b's row t.  pos
+ * (device, B uint32; NULL: zeros) gives each sequence's first row's slot in its own caches, so row t
+ * stands at slot pos[b] + t; counts (device, B uint32; NULL: T each) how many of its T rows a
+ * sequence brings.  Rows past that are padding: nothing is read, written or computed for them.
+ * B T (hq + 2 hkv) must stay below 2^31.
+ */
+typedef struct mt_kv {
+    void *k;
+    void *v;
+    uint8_t *k_scale;
+    uint8_t *v_scale;
+    uint64_t stride;
+    uint64_t scale_stride;
+    uint32_t cache_len;
+    int32_t cache_t; /* mt_dtype */
+} mt_kv;
+
+/*
+ * mt_rope_append -- mt_rope_cache for such rows: the hq query heads and the hkv key heads of each
+ * qkv row ([q (hq*64) | k (hkv*64) | v (hkv*64)] at stride ldq) rotated by NeoX RoPE at position
+ * offset + pos[b] + t (offset: the positions before the own caches, e.g. a shared prefix), the
+ * query heads written to q (stride ldo; q may be qkv at the same stride, or NULL: not wanted),
+ * the rotated keys and the raw values appended at slot pos[b] + t, rounded to the caches' type.  A
+ * slot past the cache appends nothing (the query heads are still rotated).  The angle is taken in
+ * 64 bits, so far positions keep their accuracy; mt_rope_cache rounds it to fp32.  qkv and q 16-byte aligned
+ * with 16-byte row strides.
+ */
+int mt_rope_append(const float *qkv, uint32_t ldq, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, const uint32_t *pos,
+                   const uint32_t *counts, uint32_t offset, const mt_kv *kv, const float *inv_freq, float *q, uint32_t ldo,
+                   mt_stream_t stream);
+
+/*
+ * mt_kv_copy -- the rows' slots from src's caches to the same slots of dst's, converted between
+ * any two cache types: an fp16 cache quantised, an 8-bit one read back (exactly, into fp32; into fp16 as far
+ * as that holds the values), a sequence's prompt set aside as a shared prefix.  Slots past either cache are left
+ * out.  src and dst must not overlap.
+ */
+int mt_kv_copy(const mt_kv *src, const mt_kv *dst, uint32_t B, uint32_t T, uint32_t hkv, const uint32_t *pos,
+               const uint32_t *counts, mt_stream_t stream);
+
+/*
+ * mt_attention_shared -- grouped-query attention of the rows over prefix_len keys that every
+ * sequence sees first (slots 0 .. prefix_len - 1 of the one sequence in `prefix`; NULL with
+ * prefix_len 0) and then over their own keys up to their own slot (slot pos[b] + t, or the cache's last where
+ * that is past it): with own slots counted from prefix_len, keys [max(0, i + 1 - window), i] of row
+ * i (window 0 = unlimited).  q rows (stride ldq) hold hq heads of 64, already rotated; out
+ * rows stride ldo; scores scaled by `scale`, max-subtracted softmax; q and out are 16-byte
+ * aligned with 16-byte row strides and do not overlap.  Both caches are of one type.  Cache slots
+ * that a row does not attend do not reach its result, whatever they hold.
+ *
+ * len_max is the caller's bound on the own keys, max(pos[b] + counts[b]) (0: cache_len).  It only
+ * places the work (longer sequences give the same results, more slowly).  The keys are split over
+ * workgroups where rows are few and keys are many; their parts meet in `workspace`, 16-byte aligned device memory
+ * of at least mt_attention_shared_workspace(the same sizes) bytes (0: none needed, NULL is fine), which
+ * holds nothing between calls.  Calls that may overlap, captured graphs among them, need a workspace each.
+ */
+uint64_t mt_attention_shared_workspace(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t prefix_len,
+                                       uint32_t len_max, uint32_t window, mt_dtype cache_t);
+int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, const uint32_t *pos,
+                        const uint32_t *counts, const mt_kv *kv, const mt_kv *prefix, uint32_t prefix_len, uint32_t len_max,
+                        uint32_t window, float *out, uint32_t ldo, float scale, void *workspace, uint64_t workspace_bytes,
+                        mt_stream_t stream);
+
+/*
+ * mt_quantize_f8 -- `rows` rows of K values x (type xt, row stride ldx) as a matrix in 8 bits: codes
+ * [rows, ldq] and scales [rows, lds], lds >= 4 ceil(K / 512) and a multiple of 4 (the bytes past
+ * the row's blocks are set to 0).  With norm ([K] of type nt, as mt_linear_rmsnorm's) the rows are
+ * x * rsqrt(mean(x^2) + eps) * norm.  K a multiple of 16; x, norm and codes 16-byte aligned with 16-byte row
+ * strides, scales 4-byte aligned.  codes and scales must not overlap x.
+ *
+ * mt_linear_f8 -- mt_linear with weights in 8 bits: y = epilogue(x w^T), w and the gate partner w2
+ * codes [N, K], contiguous, with scales ws, w2s [N, 4 ceil(K / 512)].  x is a matrix in 8 bits too: codes
+ * and scales as mt_quantize_f8 writes them (xt MT_F8, ldx and ldxs their row strides in bytes), or
+ * up to 16 rows of fp32, fp16 or bf16 values, which the call quantises on the way in, after the RMSNorm
+ * with gain `norm` and p.eps if norm is given (more rows, or a norm over K > 32768: MT_ENOTSUP, quantise
+ * them first; a norm takes K <= 524288 there).  The same
+ * bytes as mt_quantize_f8 of x enter the product.  Products are exact and sums fp32.  bias and norm are of type bt (MT_F16 or
+ * MT_BF16); flags, bias, epilogue, y and overlap rules as mt_linear; K a multiple of 16; codes 16-byte
+ * aligned, scales 4-byte aligned.
+ */
+int mt_quantize_f8(const void *x, mt_dtype xt, uint32_t rows, uint32_t K, uint32_t ldx, const void *norm, mt_dtype nt, float eps,
+                   uint8_t *codes, uint32_t ldq, uint8_t *scales, uint32_t lds, mt_stream_t stream);
+int mt_linear_f8(const void *x, mt_dtype xt, const uint8_t *xs, uint32_t ldxs, const void *norm, const uint8_t *w,
+                 const uint8_t *ws, const uint8_t *w2, const uint8_t *w2s, const void *bias, mt_dtype bt, float *y,
+                 mt_gemv_params p, mt_stream_t stream);
 
 /*
  * The DiT flow step around its linears (MingEngine.encodeStep's flow loop,

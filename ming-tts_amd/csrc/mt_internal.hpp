@@ -179,6 +179,19 @@ int split_workspace(const FixedWs *fixed, hipStream_t stream, size_t part_bytes,
 
 // Compute units of the current device (cached per device), or <= 0 when it cannot be queried.
 int device_cus();
+// Operators on 8-bit storage and shared prefixes (f8.hpp).
+struct KvArgs;
+struct RowsArgs;
+struct SharedArgs;
+struct F8LinearArgs;
+int launch_rope_append(const float *qkv, uint32_t ldq, const RowsArgs &rows, uint32_t hq, uint32_t hkv, uint32_t offset,
+                       const KvArgs &kv, int ct, const float *inv_freq, float *q, uint32_t ldo, hipStream_t stream);
+int launch_kv_copy(const KvArgs &src, int st, const KvArgs &dst, int dt, const RowsArgs &rows, uint32_t hkv, hipStream_t stream);
+int launch_attention_shared(const SharedArgs &a, int ct, hipStream_t stream);
+int launch_quantize_f8(const void *x, int xt, uint32_t rows, uint32_t K, uint32_t ldx, const uint16_t *norm, int nt, float eps,
+                       uint8_t *codes, uint32_t ldq, uint8_t *scales, uint32_t lds, hipStream_t stream);
+int launch_linear_f8(const F8LinearArgs &a, int xt, int bt, hipStream_t stream);
+
 // Split-K workspace of `stream` on the current device: at least `part_bytes` of partial sums
 // and `counters` zeroed arrival counters (the kernels leave them zero again).  Grows by
 // synchronising the stream, so it is not for use under graph capture once it must grow.

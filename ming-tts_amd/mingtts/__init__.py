@@ -19,7 +19,7 @@ from typing import Optional, Sequence
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.normpath(os.path.join(_HERE, "..", "csrc", "libmingtts_hip.so"))
 
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, F8 = 0, 1, 2, 3
 OK, EHIP, ENOMEM, EINVAL, ERANGE, ENOTSUP = 0, -5, -12, -22, -34, -95
 KERNEL_GEMV, KERNEL_GEMM, KERNEL_GEMV_MFMA = 1, 2, 3
 (TUNE_GEMV_ROWS_MAX, TUNE_GEMV_LANES, TUNE_GEMM_SPLITK, TUNE_SEQ_GROUPS, TUNE_SEQ_LAUNCH, TUNE_GEMM_TILE,
@@ -32,7 +32,8 @@ EXPORTS = (
     "mt_seq_create_items", "mt_seq_run",
     "mt_seq_destroy", "mt_seq_groups", "mt_seq_kernel", "mt_seq_check", "mt_rope_cache", "mt_rope_cache_decode",
     "mt_attention", "mt_attention_decode", "mt_rope_attention", "mt_dit_attention", "mt_dit_attention_linear", "mt_flow_assemble",
-    "mt_flow_euler", "mt_flow_euler_assemble",
+    "mt_flow_euler", "mt_flow_euler_assemble", "mt_rope_append", "mt_kv_copy", "mt_attention_shared",
+    "mt_attention_shared_workspace", "mt_quantize_f8", "mt_linear_f8",
     "mt_upsample4", "mt_istft_frames", "mt_istft_emit", "mt_st_open", "mt_st_close", "mt_st_count", "mt_st_name", "mt_st_find", "mt_arena_create", "mt_arena_tensor",
     "mt_arena_padded", "mt_arena_bytes", "mt_arena_upload", "mt_arena_audit", "mt_arena_destroy",
     "mt_last_error", "mt_version",
@@ -93,6 +94,13 @@ SEQ_LINEAR, SEQ_ATTENTION, SEQ_DIT_ATTENTION = 0, 1, 2
 class SeqItem(ctypes.Structure):
     """mt_seq_item: a linear, a decode attention or a DiT attention item of a sequence."""
     _fields_ = [("kind", ctypes.c_int32), ("linear", LinearOp), ("attn", AttnOp), ("dit", DitAttnOp)]
+
+
+class KvStruct(ctypes.Structure):
+    """mt_kv: the caches of one layer for a batch of sequences."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("stride", ctypes.c_uint64), ("scale_stride", ctypes.c_uint64),
+                ("cache_len", ctypes.c_uint32), ("cache_t", ctypes.c_int32)]
 
 
 class StEntry(ctypes.Structure):
@@ -166,6 +174,19 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     L.mt_istft_frames.restype = i32
     L.mt_istft_emit.argtypes = [vp, vp, u32, u32, u32, u32, u32, u32, vp, vp]
     L.mt_istft_emit.restype = i32
+    kv = ctypes.POINTER(KvStruct)
+    L.mt_rope_append.argtypes = [vp, u32, u32, u32, u32, u32, vp, vp, u32, kv, vp, vp, u32, vp]
+    L.mt_rope_append.restype = i32
+    L.mt_kv_copy.argtypes = [kv, kv, u32, u32, u32, vp, vp, vp]
+    L.mt_kv_copy.restype = i32
+    L.mt_attention_shared_workspace.argtypes = [u32, u32, u32, u32, u32, u32, u32, i32]
+    L.mt_attention_shared_workspace.restype = u64
+    L.mt_attention_shared.argtypes = [vp, u32, u32, u32, u32, u32, vp, vp, kv, kv, u32, u32, u32, vp, u32, f32, vp, u64, vp]
+    L.mt_attention_shared.restype = i32
+    L.mt_quantize_f8.argtypes = [vp, i32, u32, u32, u32, vp, i32, f32, vp, u32, vp, u32, vp]
+    L.mt_quantize_f8.restype = i32
+    L.mt_linear_f8.argtypes = [vp, i32, vp, u32, vp, vp, vp, vp, vp, vp, i32, vp, GemvParams, vp]
+    L.mt_linear_f8.restype = i32
     cp = ctypes.c_char_p
     L.mt_st_open.argtypes = [cp, ctypes.POINTER(vp)]
     L.mt_st_open.restype = i32
@@ -421,6 +442,169 @@ def attention_decode(q, ldq, B, hq, hkv, lens, window, kc, vc, cache_len, cache_
     check(load().mt_attention_decode(_ptr(q), ldq, B, hq, hkv, _ptr(lens), window, _ptr(kc), _ptr(vc),
                                      dtype_code(kc), cache_len, cache_stride, _ptr(out), ldo, scale,
                                      _stream(stream)))
+
+
+# ----------------------------------- 8-bit storage and shared prefixes --
+
+def _storage_code(t) -> int:
+    """dtype_code, and F8 for codes (uint8 or float8_e4m3fn)."""
+    if t.element_size() == 1:
+        import torch
+        if t.dtype in (torch.uint8, torch.float8_e4m3fn):
+            return F8
+    return dtype_code(t)
+
+
+class KV:
+    """The caches of one layer (mt_kv): k and v torch tensors [B, hkv, cache_len, 64], or [hkv, cache_len, 64]
+    for one sequence (a shared prefix), fp32, fp16 or 8-bit codes (uint8 or float8_e4m3fn); 8-bit caches have
+    scale bytes k_scale and v_scale [B, hkv, cache_len].  A sequence's caches are contiguous; the batch may be strided,
+    the same way for k and v (and for both scales)."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        t = _storage_code(k)
+        for name, x, y, inner in (("k and v", k, v, 3), ("k_scale and v_scale", k_scale, v_scale, 2)):
+            if inner == 2 and t != F8:
+                continue
+            if x is None or y is None or x.shape != y.shape or x.dtype != y.dtype or x.stride() != y.stride():
+                raise ValueError(f"{name} must be two tensors of one shape, type and layout")
+            if x.dim() not in (inner, inner + 1) or not x[(0,) * (x.dim() - inner)].is_contiguous():
+                raise ValueError(f"{name}: [B, hkv, cache_len{', 64' if inner == 3 else ''}], contiguous but for B")
+        if k.shape[-1] != 64 or t == BF16:
+            raise ValueError("caches hold heads of 64 fp32, fp16 or 8-bit values")
+        if t == F8 and (k_scale.shape != k.shape[:-1] or k_scale.element_size() != 1):
+            raise ValueError("one scale byte a head and position")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.hkv, self.cache_len, self.type = k.shape[-3], k.shape[-2], t
+        self.batch = k.shape[0] if k.dim() == 4 else 1
+        batched = k.dim() == 4
+        self.struct = KvStruct(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), k.stride(0) if batched else 0,
+                               k_scale.stride(0) if batched and t == F8 else 0, self.cache_len, t)
+        self.ref = ctypes.byref(self.struct)
+
+    @staticmethod
+    def empty(batch, hkv, cache_len, dtype, device):
+        """Zeroed caches of torch type ``dtype`` (uint8: 8 bits) for ``batch`` sequences."""
+        import torch
+        k = torch.zeros(batch, hkv, cache_len, 64, dtype=dtype, device=device)
+        if _storage_code(k) != F8:
+            return KV(k, torch.zeros_like(k))
+        s = torch.ones(batch, hkv, cache_len, dtype=torch.uint8, device=device)
+        return KV(k, torch.zeros_like(k), s, torch.ones_like(s))
+
+
+def _check_kv(kv, B, hkv):
+    if kv.hkv != hkv or kv.batch < B:
+        raise ValueError(f"caches of {kv.batch} sequences and {kv.hkv} heads for {B} and {hkv}")
+
+
+def rope_append(qkv, B, T, hq, hkv, pos, kv, inv_freq, q=None, counts=None, offset=0, ldq=None, ldo=None, stream=None) -> None:
+    """mt_rope_append: B x T rows of qkv rotated at offset + pos[b] + t, their keys and values appended to ``kv`` at
+    slot pos[b] + t (pos None: 0), the rotated queries written to q.  counts (int32 [B]): a sequence's rows of T."""
+    _check_kv(kv, B, hkv)
+    check(load().mt_rope_append(_ptr(qkv), qkv.stride(0) if ldq is None else ldq, B, T, hq, hkv, _ptr(pos), _ptr(counts),
+                                offset, kv.ref, _ptr(inv_freq), _ptr(q),
+                                ldo if ldo is not None else 0 if q is None else q.stride(0), _stream(stream)))
+
+
+def kv_copy(src, dst, B, T, pos=None, counts=None, stream=None) -> None:
+    """mt_kv_copy: slots pos[b] .. pos[b] + counts[b] - 1 of ``src`` to the same slots of ``dst``, converted."""
+    _check_kv(src, B, dst.hkv)
+    _check_kv(dst, B, src.hkv)
+    check(load().mt_kv_copy(src.ref, dst.ref, B, T, src.hkv, _ptr(pos), _ptr(counts), _stream(stream)))
+
+
+def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=None, len_max=0, window=0, counts=None,
+                     scale=0.125, ldq=None, ldo=None, workspace=None, stream=None) -> None:
+    """mt_attention_shared: the rows' attention over ``prefix`` (one sequence's KV, its first prefix_len slots; all
+    by default) and then their own keys in ``kv`` up to their slot.  The workspace, where the split of the keys
+    needs one, comes from torch's allocator (so a captured graph keeps its own) unless given as a uint8 tensor."""
+    _check_kv(kv, B, hkv)
+    if prefix is None:
+        prefix_len = 0
+    else:
+        _check_kv(prefix, 1, hkv)
+        if prefix_len is None:
+            prefix_len = prefix.cache_len
+    L = load()
+    s = _stream(stream)
+    need = L.mt_attention_shared_workspace(B, T, hq, hkv, prefix_len, len_max if len_max else kv.cache_len, window, kv.type)
+    if need and workspace is None:
+        workspace = _scratch(need, q, stream)
+    check(L.mt_attention_shared(_ptr(q), q.stride(0) if ldq is None else ldq, B, T, hq, hkv, _ptr(pos), _ptr(counts), kv.ref,
+                                prefix.ref if prefix is not None else None, prefix_len, len_max, window, _ptr(out),
+                                out.stride(0) if ldo is None else ldo, scale, _ptr(workspace),
+                                workspace.numel() if workspace is not None else 0, s))
+
+
+def _scratch(nbytes, like, stream):
+    """Device memory for one call on ``stream``, from torch's allocator."""
+    import torch
+    t = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    if stream is not None:  # the allocator only orders its reuse on the current stream
+        t.record_stream(stream if not isinstance(stream, int) else torch.cuda.ExternalStream(stream))
+    return t
+
+
+class F8Matrix:
+    """A matrix in 8 bits: codes [rows, K] (uint8 or float8_e4m3fn, rows contiguous) and scale bytes
+    [rows, 4 ceil(K / 512)], one a block of 128 values."""
+
+    def __init__(self, codes, scales):
+        if codes.dim() != 2 or _storage_code(codes) != F8 or codes.stride(1) != 1 or codes.shape[1] % 16:
+            raise ValueError("codes: [rows, K] of 8 bits, K a multiple of 16")
+        n, k = codes.shape
+        if tuple(scales.shape) != (n, 4 * ((k + 511) // 512)) or scales.element_size() != 1 or scales.stride(1) != 1:
+            raise ValueError("scales: [rows, 4 ceil(K / 512)] bytes")
+        self.codes, self.scales, self.shape = codes, scales, codes.shape
+
+    @staticmethod
+    def quantize(x, norm=None, eps=1e-6, stream=None):
+        """mt_quantize_f8 of x [rows, K] into new tensors."""
+        import torch
+        n, k = x.shape
+        m = F8Matrix(_scratch(n * k, x, stream).view(n, k), _scratch(n * 4 * ((k + 511) // 512), x, stream).view(n, -1))
+        quantize_f8(x, m, norm=norm, eps=eps, stream=stream)
+        return m
+
+
+def quantize_f8(x, out, norm=None, eps=1e-6, stream=None) -> None:
+    """mt_quantize_f8: the rows of x [rows, K], RMS-normalised with gain ``norm`` if given, into an F8Matrix."""
+    if tuple(x.shape) != tuple(out.shape) or x.stride(1) != 1:
+        raise ValueError("x and the matrix must be of one shape, x's rows contiguous")
+    check(load().mt_quantize_f8(_ptr(x), dtype_code(x), x.shape[0], x.shape[1], x.stride(0), _ptr(norm),
+                                dtype_code(norm) if norm is not None else F16, eps, _ptr(out.codes), out.codes.stride(0),
+                                _ptr(out.scales), out.scales.stride(0), _stream(stream)))
+
+
+LINEAR_F8_ROWS, LINEAR_F8_NORM_K = 16, 32768  # most rows mt_linear_f8 quantises itself, most values a row it normalises
+
+
+def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6, ldy=None, stream=None) -> None:
+    """mt_linear_f8: y[:M] (op)= x[:M] @ w.T, w (and w2) F8Matrix [N, K]; x an F8Matrix or a float tensor, which is
+    quantised in blocks of 128 on the way (after the RMSNorm with gain ``norm``), more than 16 rows by a call of
+    mt_quantize_f8 first."""
+    N, K = w.shape
+    M = x.shape[0] if M is None else M
+    if x.shape[1] != K or x.shape[0] < M or (w2 is not None and tuple(w2.shape) != (N, K)):
+        raise ValueError("x, w and w2 must agree in K, w and w2 in shape")
+    for m in (w, w2):
+        if m is not None and not (m.codes.is_contiguous() and m.scales.is_contiguous()):
+            raise ValueError("weights must be contiguous")
+    if not isinstance(x, F8Matrix) and (M > LINEAR_F8_ROWS or (norm is not None and K > LINEAR_F8_NORM_K)):
+        x, norm = F8Matrix.quantize(x[:M], norm=norm, eps=eps, stream=stream), None
+    b = bias if bias is not None else norm
+    bt = dtype_code(b) if b is not None else F16
+    if bias is not None and norm is not None and dtype_code(norm) != bt:
+        raise ValueError("bias and norm must be of one type")
+    if isinstance(x, F8Matrix):
+        xp, xt, xs, ldx, ldxs = x.codes, F8, x.scales, x.codes.stride(0), x.scales.stride(0)
+    else:
+        xp, xt, xs, ldx, ldxs = x, dtype_code(x), None, x.stride(0), 0
+    p = GemvParams(M, N, K, ldx, y.stride(0) if ldy is None else ldy, flags, eps)
+    check(load().mt_linear_f8(_ptr(xp), xt, _ptr(xs), ldxs, _ptr(norm), _ptr(w.codes), _ptr(w.scales),
+                              _ptr(w2.codes) if w2 is not None else None, _ptr(w2.scales) if w2 is not None else None,
+                              _ptr(bias), bt, _ptr(y), p, _stream(stream)))
 
 
 def dit_attention(qkv, B, S, H, inv_freq, out, ld=None, ldo=None, scale=0.125, stream=None) -> None:
