@@ -124,8 +124,9 @@ int mt_kv_copy(const mt_kv *src, const mt_kv *dst, uint32_t B, uint32_t T, uint3
 
 uint64_t mt_attention_shared_workspace(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t prefix_len, uint32_t len_max,
                                        uint32_t window, mt_dtype cache_t) {
-    (void)B, (void)T, (void)hq, (void)hkv, (void)prefix_len, (void)len_max, (void)window, (void)cache_t;
-    return 0;
+    if (validate_rows("mt_attention_shared_workspace", B, T, hq, hkv) || hq == 0 || hq % hkv || B == 0 || T == 0) return 0;
+    const SharedPlan p = shared_plan(B, T, hq, hkv, prefix_len, len_max, window, cache_t);
+    return p.apart ? static_cast<uint64_t>(B) * T * hq * (p.sp + p.so) * (64 + 2) * 4 : 0;
 }
 
 int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, const uint32_t *pos,
@@ -154,8 +155,8 @@ int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, ui
         return set_error(MT_EINVAL, "%s: q / out must be 16-byte aligned with 16-byte row strides", who);
     const uint64_t all = static_cast<uint64_t>(B) * T, w = static_cast<uint64_t>(hq) * 64;
     if (meet(q, span(all, w, ldq, 4), out, span(all, w, ldo, 4))) return set_error(MT_EINVAL, "%s: out overlaps q", who);
-    const uint64_t need = mt_attention_shared_workspace(B, T, hq, hkv, prefix_len, len_max ? len_max : kv->cache_len, window,
-                                                        static_cast<mt_dtype>(kv->cache_t));
+    const uint32_t most = len_max ? len_max : kv->cache_len;
+    const uint64_t need = mt_attention_shared_workspace(B, T, hq, hkv, prefix_len, most, window, static_cast<mt_dtype>(kv->cache_t));
     if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return set_error(MT_EINVAL, "%s: needs %llu bytes of 16-byte aligned workspace, got %llu", who,
                          static_cast<unsigned long long>(need), static_cast<unsigned long long>(workspace ? workspace_bytes : 0));
@@ -169,7 +170,8 @@ int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, ui
     a.rows = RowsArgs{pos, counts, B, T};
     a.prefix_len = prefix_len;
     a.scale = scale;
-    return launch_attention_shared(a, kv->cache_t, reinterpret_cast<hipStream_t>(stream));
+    a.part = static_cast<float *>(workspace);
+    return launch_attention_shared(a, shared_plan(B, T, hq, hkv, prefix_len, most, window, kv->cache_t), kv->cache_t, reinterpret_cast<hipStream_t>(stream));
 }
 
 int mt_quantize_f8(const void *x, mt_dtype xt, uint32_t rows, uint32_t K, uint32_t ldx, const void *norm, mt_dtype nt, float eps,

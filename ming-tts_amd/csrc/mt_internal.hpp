@@ -187,7 +187,11 @@ struct F8LinearArgs;
 int launch_rope_append(const float *qkv, uint32_t ldq, const RowsArgs &rows, uint32_t hq, uint32_t hkv, uint32_t offset,
                        const KvArgs &kv, int ct, const float *inv_freq, float *q, uint32_t ldo, hipStream_t stream);
 int launch_kv_copy(const KvArgs &src, int st, const KvArgs &dst, int dt, const RowsArgs &rows, uint32_t hkv, hipStream_t stream);
-int launch_attention_shared(const SharedArgs &a, int ct, hipStream_t stream);
+// Where mt_attention_shared's work goes, from the sizes alone.
+struct SharedPlan;
+SharedPlan shared_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t prefix_len, uint32_t len_max, uint32_t window,
+                       int ct);
+int launch_attention_shared(const SharedArgs &a, const SharedPlan &p, int ct, hipStream_t stream);
 int launch_quantize_f8(const void *x, int xt, uint32_t rows, uint32_t K, uint32_t ldx, const uint16_t *norm, int nt, float eps,
                        uint8_t *codes, uint32_t ldq, uint8_t *scales, uint32_t lds, hipStream_t stream);
 int launch_linear_f8(const F8LinearArgs &a, int xt, int bt, hipStream_t stream);
