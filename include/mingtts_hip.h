@@ -196,10 +196,12 @@ enum {
                                     for 3..16 rows (default; 3..8 with a fused norm), 1 = never
                                     (lane-group GEMV up to 8 rows, GEMM above), 2 = up to 64 rows of
                                     x of the weights' type (32 otherwise) */
-    MT_TUNE_SEQ_LAYER = 9        /* 0: a sequence of Qwen2-0.5B decode layers (qkv 1152 x 896, o,
+    MT_TUNE_SEQ_LAYER = 9,       /* 0: a sequence of Qwen2-0.5B decode layers (qkv 1152 x 896, o,
                                     gate|up 2 x 4864 x 896, down at 1, 2 or 4 rows) runs on the
                                     kernel specialised for those shapes (default); 1: on the
                                     general sequence kernel */
+    MT_TUNE_F8_TILE = 10         /* tile (x rows x weight rows) of mt_linear_f8's GEMM: 0 = auto, 1 =
+                                    256 x 256, 2 = 128 x 128, 3 = 64 x 128 */
 };
 int mt_set_tuning(int key, int value);
 
@@ -498,7 +500,7 @@ int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, ui
  * with gain `norm` and p.eps if norm is given (more rows, or a norm over K > 32768: MT_ENOTSUP, quantise
  * them first; a norm takes K <= 524288 there).  The same
  * bytes as mt_quantize_f8 of x enter the product.  Products are exact and sums fp32.  bias and norm are of type bt (MT_F16 or
- * MT_BF16); flags, bias, epilogue, y and overlap rules as mt_linear; K a multiple of 16; codes 16-byte
+ * MT_BF16); flags, bias, epilogue, y and overlap rules as mt_linear; K a multiple of 16 up to 2^22 (and ldx of codes); codes 16-byte
  * aligned, scales 4-byte aligned.
  */
 int mt_quantize_f8(const void *x, mt_dtype xt, uint32_t rows, uint32_t K, uint32_t ldx, const void *norm, mt_dtype nt, float eps,

@@ -140,6 +140,7 @@ int mt_set_tuning(int key, int value) {
         case MT_TUNE_GEMM_STAGES: slot = &g_tuning.gemm_stages; def = 0; break;
         case MT_TUNE_GEMV_MFMA: slot = &g_tuning.gemv_mfma; def = 0; break;
         case MT_TUNE_SEQ_LAYER: slot = &g_tuning.seq_layer; def = 0; break;
+        case MT_TUNE_F8_TILE: slot = &g_tuning.f8_tile; def = 0; break;
         default: return set_error(MT_EINVAL, "mt_set_tuning: unknown key %d", key);
     }
     if (key == MT_TUNE_SEQ_LAUNCH && value > 1)
@@ -152,6 +153,8 @@ int mt_set_tuning(int key, int value) {
         return set_error(MT_EINVAL, "mt_set_tuning: the GEMM pipeline depth is 1..4, got %d", value);
     if (key == MT_TUNE_GEMM_TILE && value > 5)
         return set_error(MT_EINVAL, "mt_set_tuning: the GEMM tile choice is 0..5, got %d", value);
+    if (key == MT_TUNE_F8_TILE && value > 3)
+        return set_error(MT_EINVAL, "mt_set_tuning: the 8-bit GEMM's tile choice is 0..3, got %d", value);
     if (key == MT_TUNE_GEMV_ROWS_MAX && value > 8)
         return set_error(MT_EINVAL, "mt_set_tuning: the GEMV takes at most 8 rows per block, got %d", value);
     return slot->exchange(value < 0 ? def : value, std::memory_order_relaxed);

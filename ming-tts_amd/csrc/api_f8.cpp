@@ -212,6 +212,8 @@ int mt_linear_f8(const void *x, mt_dtype xt, const uint8_t *xs, uint32_t ldxs, c
     if (!x || !w || !ws || !y) return set_error(MT_EINVAL, "%s: null x, w, ws or y", who);
     if (p.K == 0 || p.K % 16) return set_error(MT_EINVAL, "%s: K must be a positive multiple of 16, got %u", who, p.K);
     if (p.ldx < p.K || p.ldy < p.N) return set_error(MT_EINVAL, "%s: ldx %u < K %u or ldy %u < N %u", who, p.ldx, p.K, p.ldy, p.N);
+    if (p.K > (1u << 22) || (xt == MT_F8 && p.ldx > (1u << 22)))
+        return set_error(MT_EINVAL, "%s: K %u or ldx %u past 2^22", who, p.K, p.ldx);
     const uint64_t es = elem_bytes(xt);
     if (!aligned(x, 16) || p.ldx * es % 16 || !aligned(w, 16) || (gated && !aligned(w2, 16)))
         return set_error(MT_EINVAL, "%s: x, w and w2 must be 16-byte aligned, x with a 16-byte row stride", who);

@@ -109,42 +109,6 @@ __device__ __forceinline__ void row_operand(const uint8_t *codes, uint32_t k, ui
     }
 }
 
-// One wave a tile of 16 features and 16 rows.
-template <int BT>
-__global__ __launch_bounds__(64) void linear_f8_kernel(F8LinearArgs a) {
-    const uint32_t lane = threadIdx.x, l16 = lane & 15, g = lane >> 4;
-    const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
-    const uint32_t n = min(n0 + l16, a.N - 1), m = min(m0 + l16, a.M - 1);
-    const bool gated = (a.flags & F_SILU_GATE) != 0;
-    f32x4v acc = {0.f, 0.f, 0.f, 0.f}, acc2 = acc;
-    for (uint32_t kb = 0; kb * 128 < a.K; kb++) {
-        const uint32_t k = kb * 128 + 32 * g;
-        bf16x8t wv[4], xv[4], gv[4];
-        row_operand(a.w + static_cast<size_t>(n) * a.K, k, a.K, a.ws[static_cast<size_t>(n) * a.lds + kb], wv);
-        row_operand(static_cast<const uint8_t *>(a.x) + static_cast<size_t>(m) * a.ldx, k, a.K, a.xs[static_cast<size_t>(m) * a.ldxs + kb], xv);
-        f32x4v t = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4; i++) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[i], xv[i], t, 0, 0, 0);
-        acc += t;
-        if (gated) {
-            row_operand(a.w2 + static_cast<size_t>(n) * a.K, k, a.K, a.w2s[static_cast<size_t>(n) * a.lds + kb], gv);
-            t = f32x4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 4; i++) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gv[i], xv[i], t, 0, 0, 0);
-            acc2 += t;
-        }
-    }
-    if (m0 + l16 >= a.M) return;
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const uint32_t nn = n0 + 4 * g + r;
-        if (nn >= a.N) continue;
-        float *y = a.y + static_cast<size_t>(m) * a.ldy + nn;
-        const float v = epilogue(acc[r], acc2[r], a.flags & F_BIAS ? dec1<BT>(a.bias[nn]) : 0.0f, a.flags);
-        *y = a.flags & F_ACCUM ? v + *y : v;
-    }
-}
-
 // Up to 16 rows of x: a workgroup of up to 16 waves takes 16 features, each wave every WAVES-th block of
 // 128 values of K.  A lane's 32 codes of a weight row are two loads; x comes quantised, or the wave
 // quantises its blocks itself, 16 lanes a block, and passes the codes through LDS into the operand's order (its
@@ -273,10 +237,7 @@ int launch_linear_f8(const F8LinearArgs &a, int xt, int bt, hipStream_t stream) 
         else few_rows<DT_F8>(a, bt, stream);
         return check_launch("linear (8-bit, few rows)");
     }
-    const dim3 grid((a.N + 15) / 16, (a.M + 15) / 16);
-    if (bt == DT_BF16) hipLaunchKernelGGL(linear_f8_kernel<DT_BF16>, grid, dim3(64), 0, stream, a);
-    else hipLaunchKernelGGL(linear_f8_kernel<DT_F16>, grid, dim3(64), 0, stream, a);
-    return check_launch("linear (8-bit)");
+    return launch_gemm_f8(a, bt, stream);
 }
 
 }  // namespace mt

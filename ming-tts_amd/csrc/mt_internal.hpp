@@ -32,6 +32,7 @@ struct Tuning {
     std::atomic<int> seq_groups{0};
     std::atomic<int> seq_launch{1};
     std::atomic<int> seq_layer{0};
+    std::atomic<int> f8_tile{0};
 };
 Tuning &tuning();
 
@@ -195,6 +196,7 @@ int launch_attention_shared(const SharedArgs &a, const SharedPlan &p, int ct, hi
 int launch_quantize_f8(const void *x, int xt, uint32_t rows, uint32_t K, uint32_t ldx, const uint16_t *norm, int nt, float eps,
                        uint8_t *codes, uint32_t ldq, uint8_t *scales, uint32_t lds, hipStream_t stream);
 int launch_linear_f8(const F8LinearArgs &a, int xt, int bt, hipStream_t stream);
+int launch_gemm_f8(const F8LinearArgs &a, int bt, hipStream_t stream);
 
 // Split-K workspace of `stream` on the current device: at least `part_bytes` of partial sums
 // and `counters` zeroed arrival counters (the kernels leave them zero again).  Grows by

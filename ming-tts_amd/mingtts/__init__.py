@@ -23,7 +23,7 @@ F32, F16, BF16, F8 = 0, 1, 2, 3
 OK, EHIP, ENOMEM, EINVAL, ERANGE, ENOTSUP = 0, -5, -12, -22, -34, -95
 KERNEL_GEMV, KERNEL_GEMM, KERNEL_GEMV_MFMA = 1, 2, 3
 (TUNE_GEMV_ROWS_MAX, TUNE_GEMV_LANES, TUNE_GEMM_SPLITK, TUNE_SEQ_GROUPS, TUNE_SEQ_LAUNCH, TUNE_GEMM_TILE,
- TUNE_GEMM_STAGES, TUNE_GEMV_MFMA, TUNE_SEQ_LAYER) = 1, 2, 3, 4, 5, 6, 7, 8, 9
+ TUNE_GEMM_STAGES, TUNE_GEMV_MFMA, TUNE_SEQ_LAYER, TUNE_F8_TILE) = 1, 2, 3, 4, 5, 6, 7, 8, 9, 10
 SEQ_GENERAL, SEQ_DECODE_LAYER, SEQ_DIT_BLOCK = 0, 1, 2
 
 # Every symbol include/mingtts_hip.h declares.

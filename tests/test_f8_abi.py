@@ -172,6 +172,12 @@ def test_linear_refuses(call, code, needle):
     assert needle in mt.last_error(), mt.last_error()
 
 
+def test_the_tile_choice_is_checked():
+    with pytest.raises(mt.MingTTSError, match="tile choice"):
+        mt.set_tuning(mt.TUNE_F8_TILE, 99)
+    assert mt.set_tuning(mt.TUNE_F8_TILE, -1) == 0
+
+
 def test_calls_without_work():
     kv = kv_struct()
     assert append(kv, B=0) == append(kv, T=0) == mt.OK

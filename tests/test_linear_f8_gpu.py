@@ -134,9 +134,17 @@ def test_few_rows(gpu, M, N, K, xt, quantized):
     run_linear(gpu, M, N, K, xt=xt, quantized=quantized, pad=4)
 
 
+@pytest.fixture(params=[0, 1, 2, 3])
+def tile(request):
+    """The GEMM's own choice, then each of its tiles by force."""
+    mt.set_tuning(mt.TUNE_F8_TILE, request.param)
+    yield request.param
+    mt.set_tuning(mt.TUNE_F8_TILE, -1)
+
+
 @pytest.mark.parametrize("M,N,K", [(17, 16, 16), (17, 64, 128), (31, 1152, 896), (64, 100, 176), (65, 129, 1040), (128, 896, 4864), (200, 333, 640),
                                    (257, 255, 512), (300, 1000, 2064), (512, 640, 896)])
-def test_many_rows(gpu, M, N, K):
+def test_many_rows(gpu, tile, M, N, K):
     say(f"many rows {M}x{N}x{K}")
     run_linear(gpu, M, N, K)
     run_linear(gpu, M, N, K, pad=4, xt="bf16", seed=1)
@@ -148,7 +156,9 @@ FLAGS = [F.gelu, F.silu, F.accumulate, F.siluGate, F.siluGate | F.accumulate, F.
 @pytest.mark.parametrize("bias", [None, "f16", "bf16"])
 @pytest.mark.parametrize("flags", FLAGS)
 @pytest.mark.parametrize("M,N,K", [(2, 100, 896), (70, 200, 272), (140, 131, 144)])
-def test_epilogues(gpu, M, N, K, flags, bias):
+def test_epilogues(gpu, tile, M, N, K, flags, bias):
+    if M <= 16 and tile:
+        pytest.skip("no GEMM")
     say(f"epilogue {M}x{N}x{K} {flags} {bias}")
     run_linear(gpu, M, N, K, flags=flags, bias=bias, pad=3)
 
