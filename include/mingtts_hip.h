@@ -200,8 +200,9 @@ enum {
                                     gate|up 2 x 4864 x 896, down at 1, 2 or 4 rows) runs on the
                                     kernel specialised for those shapes (default); 1: on the
                                     general sequence kernel */
-    MT_TUNE_F8_TILE = 10         /* tile (x rows x weight rows) of mt_linear_f8's GEMM: 0 = auto, 1 =
-                                    256 x 256, 2 = 128 x 128, 3 = 64 x 128 */
+    MT_TUNE_F8_TILE = 10         /* mt_linear_f8 with x in 8 bits: 0 = auto, else the GEMM on tiles (x rows x
+                                    weight rows) 1 = 256 x 256, 2 = 64 x 128, 3 = 64 x 64 with K split
+                                    over two groups of waves, 4 = 32 x 64 with four */
 };
 int mt_set_tuning(int key, int value);
 

@@ -153,8 +153,8 @@ int mt_set_tuning(int key, int value) {
         return set_error(MT_EINVAL, "mt_set_tuning: the GEMM pipeline depth is 1..4, got %d", value);
     if (key == MT_TUNE_GEMM_TILE && value > 5)
         return set_error(MT_EINVAL, "mt_set_tuning: the GEMM tile choice is 0..5, got %d", value);
-    if (key == MT_TUNE_F8_TILE && value > 3)
-        return set_error(MT_EINVAL, "mt_set_tuning: the 8-bit GEMM's tile choice is 0..3, got %d", value);
+    if (key == MT_TUNE_F8_TILE && value > 4)
+        return set_error(MT_EINVAL, "mt_set_tuning: the 8-bit GEMM's tile choice is 0..4, got %d", value);
     if (key == MT_TUNE_GEMV_ROWS_MAX && value > 8)
         return set_error(MT_EINVAL, "mt_set_tuning: the GEMV takes at most 8 rows per block, got %d", value);
     return slot->exchange(value < 0 ? def : value, std::memory_order_relaxed);

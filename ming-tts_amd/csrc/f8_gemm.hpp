@@ -11,11 +11,15 @@ typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
 
 // A tile of BM rows of x and BN rows of the weights (gated: BN / 2 features of w and of w2), on WM x WN
 // waves of MB x NB fragments of 32 x 32.
-template <int MB_, int NB_, int WM_, int WN_>
+// KG groups of such waves take every KG-th block of 128 k each; their sums meet at the end.  LDS holds P stages a
+// group, P - 1 of them on their way.
+template <int MB_, int NB_, int WM_, int WN_, int KG_, int P_>
 struct Tile {
-    static constexpr int MB = MB_, NB = NB_, WM = WM_, WN = WN_, WAVES = WM * WN;
+    static constexpr int MB = MB_, NB = NB_, WM = WM_, WN = WN_, KG = KG_, P = P_, WAVES = WM * WN;
     static constexpr int BM = 32 * MB * WM, BN = 32 * NB * WN;
-    static constexpr uint32_t STAGE = (BM + BN) * 128;  // bytes of a stage: 128 k
+    static constexpr uint32_t STAGE = (BM + BN) * 128;  // bytes of a stage
+    static constexpr int LOADS = (BM + BN) / 8 / WAVES;   // loads of 1 KiB a wave and stage
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole loads a wave");
 };
 
 __device__ __forceinline__ void lds16(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t off) {
@@ -27,29 +31,38 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const uint8_t *p, uint
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, static_cast<int>((rows - 1) * ld + K), 0x00020000);
 }
 
+// Workgroup ids are dealt to the eight XCDs in turn: a contiguous run of tiles for each.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
+    const uint32_t x = b & 7u, i = b >> 3, q = n >> 3, r = n & 7u;
+    return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + i;
+}
+
 template <class TL, bool GATED>
-__global__ __launch_bounds__(64 * TL::WAVES) void gemm_kernel(F8LinearArgs a, int bt, uint32_t tiles_m, uint32_t tiles_n) {
-    constexpr int MB = TL::MB, NB = TL::NB, BM = TL::BM, BN = TL::BN, W = TL::WAVES;
+__global__ __launch_bounds__(64 * TL::WAVES * TL::KG) void gemm_kernel(F8LinearArgs a, int bt, uint32_t tiles_m, uint32_t tiles_n) {
+    constexpr int MB = TL::MB, NB = TL::NB, BM = TL::BM, BN = TL::BN, W = TL::WAVES, KG = TL::KG;
     constexpr uint32_t FEAT = GATED ? BN / 2 : BN;  // features of a tile
     constexpr uint32_t OUT = 0xF0000000u;           // past every buffer: the load gives zeros
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % TL::WM, wn = wave / TL::WM;
-    const uint32_t tm = blockIdx.x % tiles_m, tn = blockIdx.x / tiles_m;
+    const uint32_t id = __builtin_amdgcn_readfirstlane(tid >> 6), kg = id / W, wave = id % W;
+    const uint32_t wm = wave % TL::WM, wn = wave / TL::WM;
+    const uint32_t tile = xcd_order(blockIdx.x, gridDim.x), tm = tile % tiles_m, tn = tile / tiles_m;
     const uint32_t m0 = tm * BM, n0 = tn * FEAT;
     const uint32_t mrows = min(static_cast<uint32_t>(BM), a.M - m0), nrows = min(FEAT, a.N - n0);
-    const uint32_t blocks = (a.K + 127) / 128;
+    const uint32_t blocks = (a.K + 127) / 128, steps = (blocks + KG - 1) / KG;
 
     const __amdgpu_buffer_rsrc_t xr = rows_of(static_cast<const uint8_t *>(a.x) + static_cast<size_t>(m0) * a.ldx, mrows, a.ldx, a.K);
     const __amdgpu_buffer_rsrc_t wr = rows_of(a.w + static_cast<size_t>(n0) * a.K, nrows, a.K, a.K);
     const __amdgpu_buffer_rsrc_t ur = rows_of((GATED ? a.w2 : a.w) + static_cast<size_t>(n0) * a.K, nrows, a.K, a.K);
 
     // A wave's load of 1 KiB: eight rows, lane l's 16-byte chunk l % 8 of row l / 8, which holds the row's
-    // chunk (l % 8) ^ (row % 8), so eight rows' same chunk lie in eight different bank groups.
-    const uint32_t lr = lane >> 3, lc = 16 * ((lane & 7) ^ lr);
+    // chunk (l % 8) ^ (row / 2 % 8): 16 rows' same chunk then lies in 16 different places of the
+    // 64 banks (two rows each 256 bytes).
+    const uint32_t lr = lane >> 3, lc = 16 * ((lane & 7) ^ (((8 * wave + lr) >> 1) & 7));
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
-    auto stage = [&](uint32_t kb) {
-        const uint32_t at = base + (kb & 1) * TL::STAGE, k = kb * 128 + lc;
+    // The group's step i, block KG i + kg (past the last one: zeros), into a buffer.
+    auto stage = [&](uint32_t i, uint32_t buffer) {
+        const uint32_t at = base + (buffer * KG + kg) * TL::STAGE, k = (i * KG + kg) * 128 + lc;
         const bool in = k < a.K;
 #pragma unroll
         for (int i = 0; i < BM / 8 / W; i++) {
@@ -81,6 +94,8 @@ __global__ __launch_bounds__(64 * TL::WAVES) void gemm_kernel(F8LinearArgs a, in
         brow[j] = second ? BN / 2 + f : f;
         bsc[j] = (second ? a.w2s : a.ws) + static_cast<size_t>(min(n0 + f, a.N - 1)) * a.lds;
     }
+    // A word holds four blocks' scales, of which the group's are every KG-th.
+    constexpr int SC = 4 / KG;  // steps a word
     uint32_t as[MB], bs[NB], an[MB], bn[NB];
     auto scales = [&](uint32_t kb) {
 #pragma unroll
@@ -97,51 +112,106 @@ __global__ __launch_bounds__(64 * TL::WAVES) void gemm_kernel(F8LinearArgs a, in
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
 
-    scales(0);
-    stage(0);
-    for (uint32_t kb = 0; kb < blocks; kb++) {
-        if ((kb & 3) == 0) {
+    // 32 k of a stage: half g of the lanes holds the 16 of chunk 2 q + g, eight for each of two steps.
+    struct Raw {
+        u32x4v a[MB], b[NB];
+    };
+    const uint32_t sw = (l32 >> 1) & 7;
+    auto read = [&](Raw &f, const uint8_t *at, int q) {
+        const uint32_t c = 16 * ((2 * q + g) ^ sw);
 #pragma unroll
-            for (int i = 0; i < MB; i++) as[i] = an[i];
+        for (int i = 0; i < MB; i++) f.a[i] = *reinterpret_cast<const u32x4v *>(at + arow[i] * 128 + c);
 #pragma unroll
-            for (int j = 0; j < NB; j++) bs[j] = bn[j];
-        }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (kb + 1 < blocks) stage(kb + 1);
-        if ((kb & 3) == 0 && kb + 4 < blocks) scales(kb + 4);
-        const uint8_t *at = lds + (kb & 1) * TL::STAGE, *bt_ = at + BM * 128;
+        for (int j = 0; j < NB; j++) f.b[j] = *reinterpret_cast<const u32x4v *>(at + BM * 128 + brow[j] * 128 + c);
+    };
+    auto value = [](const u32x4v &w, int s, float f) {
+        return __builtin_bit_cast(bf16x8v, u32x4v{f8_bf16x2<false>(w[2 * s], f), f8_bf16x2<true>(w[2 * s], f),
+                                                  f8_bf16x2<false>(w[2 * s + 1], f), f8_bf16x2<true>(w[2 * s + 1], f)});
+    };
+    auto compute = [&](const uint8_t *at, int c) {
         float fa[MB], fb[NB];
 #pragma unroll
-        for (int i = 0; i < MB; i++) fa[i] = f8_pow2((as[i] >> (8 * (kb & 3))) & 255u);
+        for (int i = 0; i < MB; i++) fa[i] = f8_pow2((as[i] >> (8 * (c * KG + kg))) & 255u);
 #pragma unroll
-        for (int j = 0; j < NB; j++) fb[j] = f8_pow2((bs[j] >> (8 * (kb & 3))) & 255u);
+        for (int j = 0; j < NB; j++) fb[j] = f8_pow2((bs[j] >> (8 * (c * KG + kg))) & 255u);
+        Raw f[2];
+        read(f[0], at, 0);
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            // 32 k: half g of the lanes holds the 16 of chunk 2 q + g, eight for each of two steps
-            u32x4v ar[MB], br[NB];
-#pragma unroll
-            for (int i = 0; i < MB; i++) ar[i] = *reinterpret_cast<const u32x4v *>(at + arow[i] * 128 + 16 * ((2 * q + g) ^ (arow[i] & 7)));
-#pragma unroll
-            for (int j = 0; j < NB; j++) br[j] = *reinterpret_cast<const u32x4v *>(bt_ + brow[j] * 128 + 16 * ((2 * q + g) ^ (brow[j] & 7)));
+            if (q < 3) read(f[(q + 1) & 1], at, q + 1);
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 bf16x8v av[MB], bv[NB];
 #pragma unroll
-                for (int i = 0; i < MB; i++)
-                    av[i] = __builtin_bit_cast(bf16x8v, u32x4v{f8_bf16x2<false>(ar[i][2 * s], fa[i]), f8_bf16x2<true>(ar[i][2 * s], fa[i]),
-                                                               f8_bf16x2<false>(ar[i][2 * s + 1], fa[i]), f8_bf16x2<true>(ar[i][2 * s + 1], fa[i])});
+                for (int i = 0; i < MB; i++) av[i] = value(f[q & 1].a[i], s, fa[i]);
 #pragma unroll
-                for (int j = 0; j < NB; j++)
-                    bv[j] = __builtin_bit_cast(bf16x8v, u32x4v{f8_bf16x2<false>(br[j][2 * s], fb[j]), f8_bf16x2<true>(br[j][2 * s], fb[j]),
-                                                               f8_bf16x2<false>(br[j][2 * s + 1], fb[j]), f8_bf16x2<true>(br[j][2 * s + 1], fb[j])});
+                for (int j = 0; j < NB; j++) bv[j] = value(f[q & 1].b[j], s, fb[j]);
 #pragma unroll
                 for (int i = 0; i < MB; i++)
 #pragma unroll
                     for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av[i], bv[j], acc[i][j], 0, 0, 0);
             }
         }
+    };
+
+    // Stage kb is waited for with P - 2 younger ones still on their way (the scales' loads among them only make
+    // that wait longer); behind the barrier every wave has left the buffer that stage kb + P - 1 takes.
+    constexpr int P = TL::P;
+    scales(0);
+#pragma unroll
+    for (int i = 0; i < P - 1; i++) stage(i, i);
+    uint32_t buffer = 0;
+    for (uint32_t i0 = 0; i0 < steps; i0 += SC) {
+#pragma unroll
+        for (int i = 0; i < MB; i++) as[i] = an[i];
+#pragma unroll
+        for (int j = 0; j < NB; j++) bs[j] = bn[j];
+#pragma unroll
+        for (int c = 0; c < SC; c++) {
+            if (i0 + c >= steps) break;
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((P - 2) * TL::LOADS) : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            stage(i0 + c + P - 1, buffer == 0 ? P - 1 : buffer - 1);
+            if (c == 0) scales(min((i0 + SC) * KG, (blocks - 1) & ~3u));
+            compute(lds + (buffer * KG + kg) * TL::STAGE, c);
+            buffer = buffer == P - 1 ? 0 : buffer + 1;
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing lands in LDS behind here
+
+    // The groups' sums in their order, all in group 0.
+    if constexpr (KG > 1) {
+        constexpr int REGS = MB * NB * 16;
+        static_assert((KG - 1) * W * REGS * 256 <= KG * P * TL::STAGE, "the sums overlay the stages");
+        float *sum = reinterpret_cast<float *>(lds);
+        __syncthreads();
+        if (kg > 0) {
+#pragma unroll
+            for (int i = 0; i < MB; i++)
+#pragma unroll
+                for (int j = 0; j < NB; j++)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4)
+                        *reinterpret_cast<float4 *>(sum + (((kg - 1) * W + wave) * REGS + (i * NB + j) * 16 + r) * 64 + 4 * lane) =
+                            make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]);
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int q = 0; q < KG - 1; q++)
+#pragma unroll
+            for (int i = 0; i < MB; i++)
+#pragma unroll
+                for (int j = 0; j < NB; j++)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(sum + ((q * W + wave) * REGS + (i * NB + j) * 16 + r) * 64 + 4 * lane);
+                        acc[i][j][r] += v.x;
+                        acc[i][j][r + 1] += v.y;
+                        acc[i][j][r + 2] += v.z;
+                        acc[i][j][r + 3] += v.w;
+                    }
     }
 
     // Lane l holds feature l % 32 of rows 8 (r / 4) + 4 g + r % 4 of each fragment.

@@ -1,5 +1,7 @@
 // Matrices in 8 bits (f8.hpp: a block is 128 consecutive values of a row): the quantiser
 // (mt_quantize_f8) and the linears over such weights (mt_linear_f8).
+#include <algorithm>
+
 #include "f8_linear.hpp"
 #include "mt_internal.hpp"
 
@@ -93,26 +95,36 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void *x, uint32_t K
     }
 }
 
-// A lane's 32 codes of a row (from k on, those past K as zeros) as bf16 values, four operands of eight.
-__device__ __forceinline__ void row_operand(const uint8_t *codes, uint32_t k, uint32_t K, uint32_t s, bf16x8t (&o)[4]) {
-    const float f = f8_pow2(s);
+// A lane's 32 codes of a row from k on (those past K as zeros) and the block's scale byte.
+struct RowCodes {
+    u32x4v c[2];
+    uint32_t s;
+};
+__device__ __forceinline__ RowCodes row_load(const uint8_t *codes, uint32_t k, uint32_t K, const uint8_t *scale) {
+    RowCodes r;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        u32x4v w = {0u, 0u, 0u, 0u};
-        if (k + 16 * i < K) w = *reinterpret_cast<const u32x4v *>(codes + k + 16 * i);
+        r.c[i] = u32x4v{0u, 0u, 0u, 0u};
+        if (k + 16 * i < K) r.c[i] = *reinterpret_cast<const u32x4v *>(codes + k + 16 * i);
+    }
+    r.s = *scale;
+    return r;
+}
+// Their bf16 values, four operands of eight.
+__device__ __forceinline__ void row_values(const RowCodes &r, bf16x8t (&o)[4]) {
+    const float f = f8_pow2(r.s);
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const u32x4v d = {f8_bf16x2<false>(w[2 * j], f), f8_bf16x2<true>(w[2 * j], f), f8_bf16x2<false>(w[2 * j + 1], f),
-                              f8_bf16x2<true>(w[2 * j + 1], f)};
-            o[2 * i + j] = __builtin_bit_cast(bf16x8t, d);
-        }
+    for (int i = 0; i < 4; i++) {
+        const uint32_t a = r.c[i / 2][2 * (i & 1)], b = r.c[i / 2][2 * (i & 1) + 1];
+        o[i] = __builtin_bit_cast(bf16x8t, u32x4v{f8_bf16x2<false>(a, f), f8_bf16x2<true>(a, f), f8_bf16x2<false>(b, f),
+                                                  f8_bf16x2<true>(b, f)});
     }
 }
 
-// Up to 16 rows of x: a workgroup of up to 16 waves takes 16 features, each wave every WAVES-th block of
-// 128 values of K.  A lane's 32 codes of a weight row are two loads; x comes quantised, or the wave
-// quantises its blocks itself, 16 lanes a block, and passes the codes through LDS into the operand's order (its
-// own, so the loop has no barrier).  The waves' sums meet in LDS in wave order.
+// Few rows of x: a workgroup of up to 16 waves takes 16 features and MT tiles of 16 rows, each wave every
+// WAVES-th block of 128 values of K.  A lane's 32 codes of a weight row are two loads; x comes quantised, or (MT
+// 1) the wave quantises its blocks itself, 16 lanes a block, and passes the codes through LDS into the operand's
+// order (its own, so the loop has no barrier).  The waves' sums meet in LDS in wave order.
 constexpr uint32_t FEW_LDX = 144;                      // bytes of a row of a wave's codes (128 and a skew)
 constexpr uint32_t FEW_WAVE = 16 * FEW_LDX + 16 * 4;   // bytes of a wave's codes and scales
 
@@ -122,7 +134,7 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(F8LinearArgs a, int bt) 
     constexpr uint32_t ES = XT == DT_F32 ? 4 : XT == DT_F8 ? 1 : 2;
     const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x / 64;
-    const uint32_t n0 = blockIdx.x * 16, n = min(n0 + l16, a.N - 1), m = min(l16, a.M - 1);
+    const uint32_t n0 = blockIdx.x * 16, n = min(n0 + l16, a.N - 1), m0 = blockIdx.y * 16, rows = min(a.M - m0, 16u);
     const uint32_t blocks = (a.K + 127) / 128;
     uint8_t *mine = lds + wave * FEW_WAVE;
     uint32_t *scale = reinterpret_cast<uint32_t *>(mine + 16 * FEW_LDX);
@@ -147,38 +159,59 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(F8LinearArgs a, int bt) 
     }
 
     f32x4v acc = {0.f, 0.f, 0.f, 0.f}, acc2 = acc;
-    for (uint32_t kb = wave; kb < blocks; kb += waves) {
+    // A block's loads are issued as soon as the registers of the block before are converted, so a wave with several
+    // blocks waits for memory once.
+    RowCodes w, u, xc;
+    float v[4][8];
+    auto load_w = [&](uint32_t kb) {
         const uint32_t k = kb * 128 + 32 * g;
-        bf16x8t wv[4], gv[4], xv[4];
-        row_operand(a.w + static_cast<size_t>(n) * a.K, k, a.K, a.ws[static_cast<size_t>(n) * a.lds + kb], wv);
-        if constexpr (GATED) row_operand(a.w2 + static_cast<size_t>(n) * a.K, k, a.K, a.w2s[static_cast<size_t>(n) * a.lds + kb], gv);
+        w = row_load(a.w + static_cast<size_t>(n) * a.K, k, a.K, a.ws + static_cast<size_t>(n) * a.lds + kb);
+        if constexpr (GATED) u = row_load(a.w2 + static_cast<size_t>(n) * a.K, k, a.K, a.w2s + static_cast<size_t>(n) * a.lds + kb);
+    };
+    auto load_x = [&](uint32_t kb) {
         if constexpr (XT == DT_F8) {
-            row_operand(static_cast<const uint8_t *>(a.x) + static_cast<size_t>(m) * a.ldx, k, a.K,
-                        a.xs[static_cast<size_t>(m) * a.ldxs + kb], xv);
+            const size_t m = m0 + min(l16, rows - 1);
+            xc = row_load(static_cast<const uint8_t *>(a.x) + m * a.ldx, kb * 128 + 32 * g, a.K, a.xs + m * a.ldxs + kb);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
+                if (4u * i >= rows) break;
+                load_x8<XT>(x + static_cast<size_t>(min(4 * i + g, rows - 1)) * a.ldx * ES, kb * 128 + 8 * l16, a.K, a.norm, bt, rs[i], v[i]);
+            }
+        }
+    };
+    load_w(wave);
+    load_x(wave);
+    for (uint32_t kb = wave; kb < blocks; kb += waves) {
+        const uint32_t next = kb + waves;
+        bf16x8t wv[4], uv[4];
+        row_values(w, wv);
+        if constexpr (GATED) row_values(u, uv);
+        if (next < blocks) load_w(next);
+        if constexpr (XT != DT_F8) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
                 const uint32_t r = 4 * i + g;
-                if (4u * i >= a.M) break;
-                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (r < a.M) load_x8<XT>(x + static_cast<size_t>(r) * a.ldx * ES, kb * 128 + 8 * l16, a.K, a.norm, bt, rs[i], v);
+                if (4u * i >= rows) break;
                 uint32_t s;
-                *reinterpret_cast<u32x2v *>(mine + r * FEW_LDX + 8 * l16) = block_encode(v, s);
+                *reinterpret_cast<u32x2v *>(mine + r * FEW_LDX + 8 * l16) = block_encode(v[i], s);
                 if (l16 == 0) scale[r] = s;
             }
             wave_sync();
-            row_operand(mine + m * FEW_LDX, 32 * g, 128, scale[m], xv);
+            const uint32_t m = min(l16, rows - 1);
+            xc.c[0] = *reinterpret_cast<const u32x4v *>(mine + m * FEW_LDX + 32 * g);
+            xc.c[1] = *reinterpret_cast<const u32x4v *>(mine + m * FEW_LDX + 32 * g + 16);
+            xc.s = scale[m];
             wave_sync();
         }
-        f32x4v t = {0.f, 0.f, 0.f, 0.f};
+        bf16x8t xv[4];
+        row_values(xc, xv);
+        if (next < blocks) load_x(next);
 #pragma unroll
-        for (int i = 0; i < 4; i++) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[i], xv[i], t, 0, 0, 0);
-        acc += t;
+        for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[i], xv[i], acc, 0, 0, 0);
         if constexpr (GATED) {
-            t = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; i++) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gv[i], xv[i], t, 0, 0, 0);
-            acc2 += t;
+            for (int i = 0; i < 4; i++) acc2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(uv[i], xv[i], acc2, 0, 0, 0);
         }
     }
 
@@ -189,8 +222,8 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(F8LinearArgs a, int bt) 
     *reinterpret_cast<f32x4v *>(part + wave * PW + l16 * 16 + 4 * g) = acc;
     if constexpr (GATED) *reinterpret_cast<f32x4v *>(part + wave * PW + 256 + l16 * 16 + 4 * g) = acc2;
     __syncthreads();
-    for (uint32_t i = tid; i < a.M * 16; i += blockDim.x) {
-        const uint32_t row = i / 16, nn = n0 + (i & 15);
+    for (uint32_t i = tid; i < rows * 16; i += blockDim.x) {
+        const uint32_t row = m0 + i / 16, nn = n0 + (i & 15);
         if (nn >= a.N) continue;
         float s = 0.0f, s2 = 0.0f;
         for (uint32_t w = 0; w < waves; w++) {
@@ -204,15 +237,22 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(F8LinearArgs a, int bt) 
     }
 }
 
+// Waves of a workgroup: the blocks of K over at most 16, evenly.
+uint32_t few_waves(uint32_t K) {
+    const uint32_t blocks = (K + 127) / 128, each = (blocks + 15) / 16;
+    return (blocks + each - 1) / each;
+}
+
 template <int XT>
-void few_rows(const F8LinearArgs &a, int bt, hipStream_t stream) {
-    const uint32_t blocks = (a.K + 127) / 128, each = (blocks + 15) / 16, waves = (blocks + each - 1) / each;
+int few_rows(const F8LinearArgs &a, int bt, hipStream_t stream) {
+    const uint32_t blocks = (a.K + 127) / 128, waves = few_waves(a.K);
     const bool gated = (a.flags & F_SILU_GATE) != 0;
-    uint32_t bytes = waves * FEW_WAVE + (a.norm ? a.M * blocks * 4 : 0);
-    static_assert(FEW_WAVE >= 2048, "the waves' sums overlay their codes");
-    const dim3 grid((a.N + 15) / 16), block(64 * waves);
+    const uint32_t codes = XT == DT_F8 ? 0 : waves * FEW_WAVE, sums = waves * 1024 * (gated ? 2 : 1);
+    const uint32_t bytes = std::max(codes + (a.norm ? a.M * blocks * 4 : 0), sums);
+    const dim3 grid((a.N + 15) / 16, (a.M + 15) / 16), block(64 * waves);
     if (gated) hipLaunchKernelGGL((few_rows_kernel<XT, true>), grid, block, bytes, stream, a, bt);
     else hipLaunchKernelGGL((few_rows_kernel<XT, false>), grid, block, bytes, stream, a, bt);
+    return check_launch("linear (8-bit, few rows)");
 }
 
 }  // namespace
@@ -230,13 +270,18 @@ int launch_quantize_f8(const void *x, int xt, uint32_t rows, uint32_t K, uint32_
 }
 
 int launch_linear_f8(const F8LinearArgs &a, int xt, int bt, hipStream_t stream) {
-    if (a.M <= 16) {
-        if (xt == DT_F32) few_rows<DT_F32>(a, bt, stream);
-        else if (xt == DT_F16) few_rows<DT_F16>(a, bt, stream);
-        else if (xt == DT_BF16) few_rows<DT_BF16>(a, bt, stream);
-        else few_rows<DT_F8>(a, bt, stream);
-        return check_launch("linear (8-bit, few rows)");
-    }
+    if (xt == DT_F32) return few_rows<DT_F32>(a, bt, stream);
+    if (xt == DT_F16) return few_rows<DT_F16>(a, bt, stream);
+    if (xt == DT_BF16) return few_rows<DT_BF16>(a, bt, stream);
+    // Rows that come quantised: this kernel while its waves are at most 16 a CU (a tile of 16 x 16 without LDS or
+    // barriers is the quicker one until the CUs queue).  Measured, us, it against the GEMM: 64 rows of 896 x 4864
+    // (2912 waves of 256 CUs) 7.6 against 11.0, 64 of 1152 x 896 (2016) 4.5 against 5.0, 96 of 896 x 4864 (4368) 12.7 against
+    // 11.0, 174 of 1152 x 896 (5544) 6.4 against 5.1, 64 of 2 x 4864 x 896 (8512) 10.2 against 6.5.
+    const int cus = device_cus();
+    const uint64_t tiles = static_cast<uint64_t>((a.N + 15) / 16) * ((a.M + 15) / 16);
+    if (tuning().f8_tile.load(std::memory_order_relaxed) == 0 && a.M <= 16 * 65535u &&
+        tiles * few_waves(a.K) <= 16ull * (cus > 0 ? cus : 256))
+        return few_rows<DT_F8>(a, bt, stream);
     return launch_gemm_f8(a, bt, stream);
 }
 

@@ -134,16 +134,16 @@ def test_few_rows(gpu, M, N, K, xt, quantized):
     run_linear(gpu, M, N, K, xt=xt, quantized=quantized, pad=4)
 
 
-@pytest.fixture(params=[0, 1, 2, 3])
+@pytest.fixture(params=[0, 1, 2, 3, 4])
 def tile(request):
-    """The GEMM's own choice, then each of its tiles by force."""
+    """The call's own choice, then each of the GEMM's tiles by force."""
     mt.set_tuning(mt.TUNE_F8_TILE, request.param)
     yield request.param
     mt.set_tuning(mt.TUNE_F8_TILE, -1)
 
 
 @pytest.mark.parametrize("M,N,K", [(17, 16, 16), (17, 64, 128), (31, 1152, 896), (64, 100, 176), (65, 129, 1040), (128, 896, 4864), (200, 333, 640),
-                                   (257, 255, 512), (300, 1000, 2064), (512, 640, 896)])
+                                   (257, 255, 512), (300, 1000, 2064), (512, 640, 896), (600, 16, 1024)])
 def test_many_rows(gpu, tile, M, N, K):
     say(f"many rows {M}x{N}x{K}")
     run_linear(gpu, M, N, K)
