@@ -58,23 +58,23 @@ __global__ __launch_bounds__(64 * TL::WAVES * TL::KG) void gemm_kernel(F8LinearA
     // A wave's load of 1 KiB: eight rows, lane l's 16-byte chunk l % 8 of row l / 8, which holds the row's
     // chunk (l % 8) ^ (row / 2 % 8): 16 rows' same chunk then lies in 16 different places of the
     // 64 banks (two rows each 256 bytes).
-    const uint32_t lr = lane >> 3, lc = 16 * ((lane & 7) ^ (((8 * wave + lr) >> 1) & 7));
+    const uint32_t lr = lane >> 3;
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
-    // The group's step i, block KG i + kg (past the last one: zeros), into a buffer.
-    auto stage = [&](uint32_t i, uint32_t buffer) {
-        const uint32_t at = base + (buffer * KG + kg) * TL::STAGE, k = (i * KG + kg) * 128 + lc;
-        const bool in = k < a.K;
+    auto chunk = [&](uint32_t r8) { return 16 * ((lane & 7) ^ (4 * (r8 & 1) + (lr >> 1))); };
+    // The group's step, its block KG step + kg (past the last one: zeros), into a buffer.
+    auto stage = [&](uint32_t step, uint32_t buffer) {
+        const uint32_t at = base + (buffer * KG + kg) * TL::STAGE, k0 = (step * KG + kg) * 128;
 #pragma unroll
         for (int i = 0; i < BM / 8 / W; i++) {
-            const uint32_t r8 = wave + W * i;
-            lds16(xr, at + r8 * 1024, in ? (8 * r8 + lr) * a.ldx + k : OUT);
+            const uint32_t r8 = wave + W * i, k = k0 + chunk(r8);
+            lds16(xr, at + r8 * 1024, k < a.K ? (8 * r8 + lr) * a.ldx + k : OUT);
         }
 #pragma unroll
         for (int i = 0; i < BN / 8 / W; i++) {
-            const uint32_t r8 = wave + W * i;
+            const uint32_t r8 = wave + W * i, k = k0 + chunk(r8);
             const bool second = GATED && r8 >= BN / 16;
             const uint32_t row = 8 * (second ? r8 - BN / 16 : r8) + lr;
-            const uint32_t off = in ? row * a.K + k : OUT;
+            const uint32_t off = k < a.K ? row * a.K + k : OUT;
             if (second) lds16(ur, at + BM * 128 + r8 * 1024, off);
             else lds16(wr, at + BM * 128 + r8 * 1024, off);
         }
