@@ -24,26 +24,26 @@ __device__ __forceinline__ float wave_max(float v) {
 // One head's keys and values: those of the shared prefix (slots 0 .. prefix - 1) and then a
 // sequence's own.
 struct HeadKv {
-    const char *k[2], *v[2];       // [0] prefix, [1] own: the head's first row
-    const uint8_t *ks[2], *vs[2];  // 8-bit caches: the head's first scale
+    const char *pk, *pv, *ok, *ov;          // prefix and own: the head's first row
+    const uint8_t *pks, *pvs, *oks, *ovs;  // 8-bit caches: the head's first scale
     uint32_t prefix;
 };
 
 template <int CT>
 __device__ __forceinline__ HeadKv head_kv(const SharedArgs &a, uint32_t b, uint32_t kvh) {
-    HeadKv h;
+    HeadKv h{};
     const size_t own = b * a.kv.stride * Cached<CT>::ES + static_cast<size_t>(kvh) * a.kv.len * Cached<CT>::ROW;
     const size_t pre = static_cast<size_t>(kvh) * a.prefix.len * Cached<CT>::ROW;
-    h.k[1] = static_cast<const char *>(a.kv.k) + own;
-    h.v[1] = static_cast<const char *>(a.kv.v) + own;
-    h.k[0] = static_cast<const char *>(a.prefix.k) + pre;
-    h.v[0] = static_cast<const char *>(a.prefix.v) + pre;
+    h.ok = static_cast<const char *>(a.kv.k) + own;
+    h.ov = static_cast<const char *>(a.kv.v) + own;
+    h.pk = static_cast<const char *>(a.prefix.k) + pre;
+    h.pv = static_cast<const char *>(a.prefix.v) + pre;
     if constexpr (CT == DT_F8) {
         const size_t so = b * a.kv.sstride + static_cast<size_t>(kvh) * a.kv.len, sp = static_cast<size_t>(kvh) * a.prefix.len;
-        h.ks[1] = a.kv.ks + so;
-        h.vs[1] = a.kv.vs + so;
-        h.ks[0] = a.prefix.ks + sp;
-        h.vs[0] = a.prefix.vs + sp;
+        h.oks = a.kv.ks + so;
+        h.ovs = a.kv.vs + so;
+        h.pks = a.prefix.ks + sp;
+        h.pvs = a.prefix.vs + sp;
     }
     h.prefix = a.prefix_len;
     return h;
@@ -61,17 +61,17 @@ __device__ __forceinline__ float cached(const char *base, const uint8_t *scales,
 // One query head over keys [lo, hi) (prefix first) by one wave, touching those keys only: each lane a
 // key's score, then each lane a dim's sum.  An online softmax in fp32, 64 keys at a time.
 template <int CT>
-__device__ void attend_wave(const float *q, const HeadKv &h, uint32_t lo, uint32_t hi, float scale, float *out) {
+__device__ __forceinline__ void attend_wave(const float *q, const HeadKv &h, uint32_t lo, uint32_t hi, float scale, float *out) {
     const uint32_t lane = threadIdx.x & 63;
     float m = -INFINITY, l = 0.0f, o = 0.0f;
     for (uint32_t k0 = lo; k0 < hi; k0 += 64) {
         const uint32_t key = k0 + lane;
         float s = -INFINITY;
         if (key < hi) {
-            const int own = key >= h.prefix;
+            const bool own = key >= h.prefix;
             const size_t slot = own ? key - h.prefix : key;
             float d = 0.0f;
-            for (uint32_t e = 0; e < 64; e++) d = fmaf(q[e], cached<CT>(h.k[own], h.ks[own], slot, e), d);
+            for (uint32_t e = 0; e < 64; e++) d = fmaf(q[e], cached<CT>(own ? h.ok : h.pk, own ? h.oks : h.pks, slot, e), d);
             s = d * scale;
         }
         const float mn = fmaxf(m, wave_max(s));
@@ -83,9 +83,9 @@ __device__ void attend_wave(const float *q, const HeadKv &h, uint32_t lo, uint32
         const uint32_t n = min(hi - k0, 64u);
         for (uint32_t j = 0; j < n; j++) {
             const uint32_t kj = k0 + j;
-            const int own = kj >= h.prefix;
+            const bool own = kj >= h.prefix;
             const size_t slot = own ? kj - h.prefix : kj;
-            o = fmaf(__shfl(p, static_cast<int>(j), 64), cached<CT>(h.v[own], h.vs[own], slot, lane), o);
+            o = fmaf(__shfl(p, static_cast<int>(j), 64), cached<CT>(own ? h.ov : h.pv, own ? h.ovs : h.pvs, slot, lane), o);
         }
     }
     out[lane] = o / l;
@@ -179,82 +179,218 @@ __device__ __forceinline__ float rows_max(float v) {
 constexpr int AS_WAVES = 8;
 constexpr uint32_t AS_LD = 68;  // floats of a row in the waves' hand-over (64 and a 16-byte skew)
 
-// A workgroup's rows (of all rows (sequence, t, head of the group) of one key head) and keys.
-struct Item {
-    uint32_t kvh, r0, r1;      // rows [r0, r1)
-    uint32_t b;                // the sequence whose own keys are read
-    uint32_t p0, p1, o0, o1;   // tiles of 32 prefix keys and of 32 own keys
-    uint32_t split;            // apart: the part's place
+// One wave's 16 rows and TK = 32 SUB keys at a time: the raw keys and values of a tile.  Lane (l16, g) holds dims
+// 16 g .. + 15 of keys 16 u + l16 (u < 2 SUB), and dims 4 l16 .. + 3 of the values of keys 32 i + 4 g + j and 32 i
+// + 16 + 4 g + j (i < SUB, j < 4), which are the weights' places in the scores' accumulators.
+template <int CT>
+struct Raw {
+    static constexpr int SUB = CT == DT_F32 ? 1 : 2;
+    static constexpr uint32_t TK = 32 * SUB;
+    u32x4v k[2 * SUB * Kind<CT>::KW];
+    uint32_t v[8 * SUB * Kind<CT>::KW];
+    uint32_t ks[2 * SUB], vs[2 * SUB];
 };
 
-template <int CT, int RT, bool APART>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t span_of(const void *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, static_cast<int>(bytes), 0x00020000);
+}
+
+// The keys of n slots from `base` on (those past n: zeros, which the buffer's bound gives).
+template <int CT>
+__device__ __forceinline__ void load_keys(Raw<CT> &r, const char *base, const uint8_t *sc, uint32_t n, uint32_t l16, uint32_t g) {
+    constexpr uint32_t ROW = Cached<CT>::ROW;
+    const __amdgpu_buffer_rsrc_t b = span_of(base, n * ROW);
+#pragma unroll
+    for (int u = 0; u < 2 * Raw<CT>::SUB; u++)
+#pragma unroll
+        for (int i = 0; i < Kind<CT>::KW; i++)
+            r.k[u * Kind<CT>::KW + i] = __builtin_amdgcn_raw_buffer_load_b128(b, l16 * ROW + 16 * Cached<CT>::ES * g + 16 * ROW * u + 16 * i, 0, 0);
+    if constexpr (CT == DT_F8) {
+        const __amdgpu_buffer_rsrc_t s = span_of(sc, n);
+#pragma unroll
+        for (int u = 0; u < 2 * Raw<CT>::SUB; u++) r.ks[u] = __builtin_amdgcn_raw_buffer_load_b8(s, l16 + 16 * u, 0, 0);
+    }
+}
+template <int CT>
+__device__ __forceinline__ void load_values(Raw<CT> &r, const char *base, const uint8_t *sc, uint32_t n, uint32_t l16, uint32_t g) {
+    constexpr uint32_t ROW = Cached<CT>::ROW;
+    const __amdgpu_buffer_rsrc_t b = span_of(base, n * ROW);
+#pragma unroll
+    for (int j = 0; j < 8 * Raw<CT>::SUB; j++) {
+        const uint32_t at = 4 * g * ROW + 4 * Cached<CT>::ES * l16 + (16 * (j >> 2) + (j & 3)) * ROW;
+        if constexpr (CT == DT_F8) {
+            r.v[j] = __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0);
+        } else if constexpr (CT == DT_F16) {
+            const u32x2v w = __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0);
+            r.v[2 * j] = w[0];
+            r.v[2 * j + 1] = w[1];
+        } else {
+            const u32x4v w = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; e++) r.v[4 * j + e] = w[e];
+        }
+    }
+    if constexpr (CT == DT_F8) {  // four keys' bytes a load: up to three past n, which the caches' whole words hold
+        const __amdgpu_buffer_rsrc_t s = span_of(sc, (n + 3) & ~3u);
+#pragma unroll
+        for (int u = 0; u < 2 * Raw<CT>::SUB; u++) r.vs[u] = __builtin_amdgcn_raw_buffer_load_b32(s, 4 * g + 16 * u, 0, 0);
+    }
+}
+
+// One of two values: a conditional of two variables would name one of the variables, and keep both in memory.
+template <class V>
+__device__ __forceinline__ V pick(bool second, V first, V other) {
+    return second ? other : first;
+}
+
+template <int CT, bool APART>
 __global__ __launch_bounds__(64 * AS_WAVES) void attention_shared_kernel(SharedArgs a) {
     typedef Kind<CT> KD;
-    constexpr uint32_t ROW = Cached<CT>::ROW;
-    extern __shared__ __attribute__((aligned(16))) float part[];  // [wave][16 RT][AS_LD], then [2][wave][16 RT]
-    __shared__ uint32_t redo[AS_WAVES];
+    constexpr int SUB = Raw<CT>::SUB;
+    constexpr uint32_t ROW = Cached<CT>::ROW, TK = Raw<CT>::TK;
+    __shared__ __attribute__((aligned(16))) float part[AS_WAVES * 16 * AS_LD];
+    __shared__ float ms[AS_WAVES * 16], sums[AS_WAVES * 16];
+    __shared__ uint32_t redo[AS_WAVES / 2];
     const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t wk = wave % a.keys, wr = wave / a.keys, groups = AS_WAVES / a.keys;
-    const uint32_t G = a.hq / a.hkv, T = a.rows.T, span = groups * 16 * RT;  // rows of a workgroup
+    const uint32_t wk = wave % a.keys, wr = wave / a.keys;
+    const uint32_t G = a.hq / a.hkv, T = a.rows.T, span = AS_WAVES / a.keys * 16;  // rows of a workgroup
     const uint32_t P = a.prefix_len;
 
-    Item it;
+    // The workgroup's rows [r0, r1) of all rows (sequence, t, head of the group) of one key head, whose own keys are
+    // sequence b's, and its part of the keys.
     const uint32_t seq_tiles = (T * G + span - 1) / span;
-    uint32_t x = blockIdx.x;
-    bool own = true, pre = true;
+    uint32_t x = blockIdx.x, parts = 1, mine = 0;
+    bool own = true, pre = P > 0;
     if constexpr (APART) {
         const uint32_t pre_items = a.sp * a.hkv * ((a.rows.B * T * G + span - 1) / span);
         own = x >= pre_items;
         pre = !own;
         if (own) x -= pre_items;
-    }
-    uint32_t parts = 1, mine = 0;
-    if constexpr (APART) {
         parts = own ? a.so : a.sp;
         mine = x % parts;
         x /= parts;
     }
-    it.kvh = x % a.hkv;
+    const uint32_t kvh = x % a.hkv;
     x /= a.hkv;
-    it.split = own ? a.sp + mine : mine;
+    uint32_t b = 0, r0, r1;
     if (own) {
-        it.b = x / seq_tiles;
-        const uint32_t n = a.rows.counts ? min(a.rows.counts[it.b], T) : T;
-        it.r0 = it.b * T * G + (x % seq_tiles) * span;
-        it.r1 = min(it.b * T * G + n * G, it.r0 + span);
-        if (it.r0 >= it.r1) return;
+        b = x / seq_tiles;
+        const uint32_t n = a.rows.counts ? min(a.rows.counts[b], T) : T;
+        r0 = b * T * G + (x % seq_tiles) * span;
+        r1 = min(b * T * G + n * G, r0 + span);
+        if (r0 >= r1) return;
     } else {
-        it.b = 0;
-        it.r0 = x * span;
-        it.r1 = min(a.rows.B * T * G, it.r0 + span);
+        r0 = x * span;
+        r1 = min(a.rows.B * T * G, r0 + span);
     }
 
-    // The wave's rows: their keys [lo, hi) of the prefix and the own keys together (none: not a row), and q.
-    uint32_t lo[RT], hi[RT];
-    u32x4v qf[RT][2][KD::NQ];
-    float c[RT];
-    const float c0 = a.scale * 1.4426950408889634f;
+    // The lane's row (all four g's the same one), its query's 16 dims and its keys [lo, hi) of the prefix and the own
+    // keys together (none: not a row).
+    const uint32_t rw = r0 + wr * 16, r = rw + l16, row = r / G;
+    uint32_t lo = 0, hi = 0;
+    float4 qv[4] = {};
+    {
+        uint32_t rb;
+        uint64_t slot;
+        if (r < r1 && a.rows.at(row, rb, slot)) {
+            const float4 *p = reinterpret_cast<const float4 *>(a.q + static_cast<size_t>(row) * a.ldq + (kvh * G + r % G) * 64 + 16 * g);
 #pragma unroll
-    for (int i = 0; i < RT; i++) {
-        const uint32_t r = it.r0 + (wr * RT + i) * 16 + l16, row = r / G;
-        uint32_t b = 0;
-        uint64_t slot = 0;
-        lo[i] = hi[i] = 0;
+            for (int e = 0; e < 4; e++) qv[e] = p[e];
+            row_keys(a, slot, lo, hi);
+        }
+    }
+    // What the wave's rows have in common: keys from lo_all to hi_all, of which those from inner_lo to inner_hi belong to
+    // every row.  A sequence's rows are in order; rows of many sequences differ by their windows.
+    uint32_t lo_all = 0, hi_all = 0, inner_lo = 0, inner_hi = ~0u;
+    if (own) {
+        if (rw < r1) {
+            const uint64_t at = a.rows.pos ? a.rows.pos[b] : 0u;
+            const uint32_t first = (rw - b * T * G) / G, last = (min(rw + 16, r1) - 1 - b * T * G) / G;
+            row_keys(a, at + first, lo_all, inner_hi);
+            row_keys(a, at + last, inner_lo, hi_all);
+        }
+    } else if (a.window == 0) {
+        hi_all = P;
+    } else {
+        uint32_t l = hi ? lo : ~0u, h = hi, il = lo;
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) {
+            l = min(l, static_cast<uint32_t>(__shfl_xor(static_cast<int>(l), d, 64)));
+            h = max(h, static_cast<uint32_t>(__shfl_xor(static_cast<int>(h), d, 64)));
+            il = max(il, static_cast<uint32_t>(__shfl_xor(static_cast<int>(il), d, 64)));
+        }
+        lo_all = __builtin_amdgcn_readfirstlane(l);
+        hi_all = __builtin_amdgcn_readfirstlane(h);
+        inner_lo = __builtin_amdgcn_readfirstlane(il);
+    }
+    // Their tiles of TK keys, first those of the prefix, then the own ones: this workgroup's part of them, every keys-th.
+    const uint32_t pend = pre ? min(hi_all, P) : 0, oend = own && hi_all > P ? hi_all - P : 0;
+    uint32_t p0 = min(lo_all, pend) / TK, p1 = (pend + TK - 1) / TK;
+    uint32_t o0 = oend && lo_all > P ? (lo_all - P) / TK : 0, o1 = (oend + TK - 1) / TK;
+    if constexpr (APART) {
+        // The prefix in equal parts; the own keys in runs of a.run tiles, the last part all that is left, so a workgroup's work
+        // does not grow with its sequence.
+        const uint32_t first = pick(own, p0, o0), last = pick(own, p1, o1), n = last - first;
+        const uint32_t t0 = own ? min(last, first + mine * a.run) : first + static_cast<uint32_t>(static_cast<uint64_t>(n) * mine / parts);
+        const uint32_t t1 = mine == parts - 1 ? last
+                            : own             ? min(last, t0 + a.run)
+                                              : first + static_cast<uint32_t>(static_cast<uint64_t>(n) * (mine + 1) / parts);
+        p0 = own ? 0 : t0;
+        p1 = own ? 0 : t1;
+        o0 = own ? t0 : 0;
+        o1 = own ? t1 : 0;
+    }
+    const uint32_t np = p1 - p0, nt = np + (o1 - o0);
+    if constexpr (APART) {
+        if (nt == 0) {  // all waves alike (they share their rows): no key for any row
+            if (tid < 16 && hi > 0) {
+                const uint32_t S = a.sp + a.so;
+                const size_t at = (static_cast<size_t>(row) * a.hq + kvh * G + r % G) * S + (own ? a.sp + mine : mine);
+                reinterpret_cast<float2 *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * S * 64)[at] = make_float2(INFINITY, 0.0f);
+            }
+            return;
+        }
+    }
+
+    const HeadKv h = head_kv<CT>(a, b, kvh);
+    Raw<CT> raw;
+    auto tile = [&](uint32_t t, bool &seg, uint32_t &s0, uint32_t &end) {
+        seg = t >= np;
+        s0 = TK * pick(seg, p0 + t, o0 + t - np);
+        end = pick(seg, pend, oend);
+    };
+    auto keys = [&](uint32_t t) {
+        bool seg;
+        uint32_t s0, end;
+        tile(t, seg, s0, end);
+        load_keys<CT>(raw, pick(seg, h.pk, h.ok) + static_cast<size_t>(s0) * ROW, CT == DT_F8 ? pick(seg, h.pks, h.oks) + s0 : nullptr,
+                      min(end - s0, TK), l16, g);
+    };
+    auto values = [&](uint32_t t) {
+        bool seg;
+        uint32_t s0, end;
+        tile(t, seg, s0, end);
+        load_values<CT>(raw, pick(seg, h.pv, h.ov) + static_cast<size_t>(s0) * ROW, CT == DT_F8 ? pick(seg, h.pvs, h.ovs) + s0 : nullptr,
+                        min(end - s0, TK), l16, g);
+    };
+    uint32_t t = wk;
+    if (t < nt) {
+        keys(t);
+        values(t);
+    }
+
+    // The query as the operand's pieces, scaled so that the scores are base-2 exponents (fp16 pieces: times c).
+    u32x4v qf[2][KD::NQ];
+    const float c0 = a.scale * 1.4426950408889634f;
+    float c = 1.0f;
+    {
         float v[16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) v[e] = 0.0f;
-        if (r < it.r1 && a.rows.at(row, b, slot)) {
-            row_keys(a, slot, lo[i], hi[i]);
-            const float4 *p = reinterpret_cast<const float4 *>(a.q + static_cast<size_t>(row) * a.ldq + (it.kvh * G + r % G) * 64 + 16 * g);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float4 w = p[e];
-                v[4 * e] = w.x; v[4 * e + 1] = w.y; v[4 * e + 2] = w.z; v[4 * e + 3] = w.w;
-            }
+        for (int e = 0; e < 4; e++) {
+            v[4 * e] = qv[e].x; v[4 * e + 1] = qv[e].y; v[4 * e + 2] = qv[e].z; v[4 * e + 3] = qv[e].w;
         }
         float f = c0;
-        c[i] = 1.0f;
         if constexpr (CT == DT_F16) {  // the row's largest |q| to 2^13 .. 2^14
             float mx = 0.0f;
 #pragma unroll
@@ -262,259 +398,154 @@ __global__ __launch_bounds__(64 * AS_WAVES) void attention_shared_kernel(SharedA
             mx = rows_max(mx);
             const int ex = min(267 - static_cast<int>(__float_as_uint(mx) >> 23), 253);
             f = __uint_as_float(static_cast<uint32_t>(ex) << 23);
-            c[i] = fabsf(c0) * __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+            c = fabsf(c0) * __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
             if (c0 < 0.0f) f = -f;
         }
 #pragma unroll
         for (int e = 0; e < 16; e++) v[e] *= f;
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++) split8<CT>(v + 8 * kk, qf[i][kk]);
+        for (int kk = 0; kk < 2; kk++) split8<CT>(v + 8 * kk, qf[kk]);
     }
-    // What the rows have in common: keys from the smallest lo to the largest hi; those between inner_lo and inner_hi
-    // belong to every row.
-    uint32_t lo_all = ~0u, hi_all = 0, inner_lo[RT], inner_hi[RT];
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-        uint32_t l = hi[i] ? lo[i] : ~0u, h = hi[i], il = lo[i], ih = hi[i] ? hi[i] : ~0u;
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) {
-            l = min(l, static_cast<uint32_t>(__shfl_xor(static_cast<int>(l), d, 64)));
-            h = max(h, static_cast<uint32_t>(__shfl_xor(static_cast<int>(h), d, 64)));
-            il = max(il, static_cast<uint32_t>(__shfl_xor(static_cast<int>(il), d, 64)));
-            ih = min(ih, static_cast<uint32_t>(__shfl_xor(static_cast<int>(ih), d, 64)));
-        }
-        lo_all = min(lo_all, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(l)));
-        hi_all = max(hi_all, static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(h)));
-        inner_lo[i] = __builtin_amdgcn_readfirstlane(il);
-        inner_hi[i] = __builtin_amdgcn_readfirstlane(ih);
-    }
-    // The wave's tiles: the rows' tiles, this workgroup's part of them, every `keys`-th of those.
-    const bool any = hi_all > 0;
-    const uint32_t pend = pre && any ? min(hi_all, P) : 0;
-    const uint32_t oend = own && any && hi_all > P ? hi_all - P : 0;  // own keys end here
-    it.p0 = pend ? min(lo_all, pend) / 32 : 0;
-    it.p1 = (pend + 31) / 32;
-    it.o0 = oend && lo_all > P ? (lo_all - P) / 32 : 0;
-    it.o1 = (oend + 31) / 32;
-    if constexpr (APART) {
-        const uint32_t first = own ? it.o0 : it.p0, n = own ? it.o1 - it.o0 : it.p1 - it.p0;
-        const uint32_t s0 = first + static_cast<uint32_t>(static_cast<uint64_t>(n) * mine / parts);
-        const uint32_t s1 = first + static_cast<uint32_t>(static_cast<uint64_t>(n) * (mine + 1) / parts);
-        if (own) it.o0 = s0, it.o1 = s1;
-        else it.p0 = s0, it.p1 = s1;
-    }
-    const uint32_t np = it.p1 - it.p0, nt = np + (it.o1 - it.o0);
 
-    const HeadKv h = head_kv<CT>(a, it.b, it.kvh);
-    u32x4v kr[2 * KD::KW];
-    uint32_t vr[8 * KD::KW];
-    uint32_t ksc[2], vsc[2];
-    // Tile t's keys: of slot s0, those past `end` re-read the last one.
-    auto place = [&](uint32_t t, uint32_t &seg, uint32_t &s0, uint32_t &end) {
-        seg = t >= np ? 1 : 0;
-        s0 = 32 * (seg ? it.o0 + t - np : it.p0 + t);
-        end = seg ? oend : pend;
-    };
-    auto loadk = [&](uint32_t t) {
-        uint32_t seg, s0, end;
-        place(t, seg, s0, end);
-        const char *base = seg ? h.k[1] : h.k[0];
-        const uint8_t *sc = seg ? h.ks[1] : h.ks[0];
+    f32x4v o[4];
+    float sub = INFINITY, ls = 0.0f;  // minus the running maximum (+infinity: no key yet), the lane's share of the weights' sum
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const uint32_t slot = min(s0 + 16 * u + l16, end - 1);
-            const u32x4v *p = reinterpret_cast<const u32x4v *>(base + static_cast<size_t>(slot) * ROW + 16 * Cached<CT>::ES * g);
-#pragma unroll
-            for (int i = 0; i < KD::KW; i++) kr[u * KD::KW + i] = p[i];
-            if constexpr (CT == DT_F8) ksc[u] = sc[slot];
-        }
-    };
-    auto loadv = [&](uint32_t t) {
-        uint32_t seg, s0, end;
-        place(t, seg, s0, end);
-        const char *base = (seg ? h.v[1] : h.v[0]) + 4 * Cached<CT>::ES * l16;
-        const uint8_t *sc = seg ? h.vs[1] : h.vs[0];
-        auto ld = [&](int j, uint32_t slot) {
-            const char *p = base + static_cast<size_t>(slot) * ROW;
-            if constexpr (CT == DT_F8) {
-                vr[j] = *reinterpret_cast<const uint32_t *>(p);
-            } else if constexpr (CT == DT_F16) {
-                const u32x2v w = *reinterpret_cast<const u32x2v *>(p);
-                vr[2 * j] = w[0];
-                vr[2 * j + 1] = w[1];
-            } else {
-                const u32x4v w = *reinterpret_cast<const u32x4v *>(p);
-#pragma unroll
-                for (int e = 0; e < 4; e++) vr[4 * j + e] = w[e];
-            }
-        };
-        if (s0 + 32 <= end) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) ld(j, s0 + 16 * (j >> 2) + 4 * g + (j & 3));
-            if constexpr (CT == DT_F8) {
-#pragma unroll
-                for (int u = 0; u < 2; u++) vsc[u] = *reinterpret_cast<const uint32_t *>(sc + s0 + 16 * u + 4 * g);
-            }
-        } else {
-            if constexpr (CT == DT_F8) vsc[0] = vsc[1] = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t slot = min(s0 + 16 * (j >> 2) + 4 * g + (j & 3), end - 1);
-                ld(j, slot);
-                if constexpr (CT == DT_F8) vsc[j >> 2] |= static_cast<uint32_t>(sc[slot]) << (8 * (j & 3));
-            }
-        }
-    };
-
-    f32x4v o[RT][4];
-    float sub[RT], ls[RT];
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-        sub[i] = INFINITY;
-        ls[i] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < 4; d++) o[i][d] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    }
-    uint32_t t = wk;
-    if (t < nt) {
-        loadk(t);
-        loadv(t);
-    }
+    for (int d = 0; d < 4; d++) o[d] = f32x4v{0.f, 0.f, 0.f, 0.f};
     for (; t < nt; t += a.keys) {
         const uint32_t next = t + a.keys;
-        uint32_t seg, s0, end;
-        place(t, seg, s0, end);
+        bool seg;
+        uint32_t s0, end;
+        tile(t, seg, s0, end);
         const uint32_t k0 = s0 + (seg ? P : 0), stop = end + (seg ? P : 0);
-        f32x4v s[RT][2];
+        f32x4v s[2 * SUB];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-#pragma unroll
-            for (int i = 0; i < RT; i++) s[i][u] = f32x4v{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < 2 * SUB; u++) {
+            s[u] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
                 u32x4v kf[KD::NC];
                 if constexpr (CT == DT_F8) {
-                    const float f = f8_pow2(ksc[u]);
-                    const uint32_t w0 = kr[u][2 * kk], w1 = kr[u][2 * kk + 1];
+                    const float f = f8_pow2(raw.ks[u]);
+                    const uint32_t w0 = raw.k[u][2 * kk], w1 = raw.k[u][2 * kk + 1];
                     kf[0] = u32x4v{f8_bf16x2<false>(w0, f), f8_bf16x2<true>(w0, f), f8_bf16x2<false>(w1, f), f8_bf16x2<true>(w1, f)};
                 } else if constexpr (CT == DT_F16) {
-                    kf[0] = kr[2 * u + kk];
+                    kf[0] = raw.k[2 * u + kk];
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const u32x4v w = kr[4 * u + 2 * kk + (e >> 1)];
+                        const u32x4v w = raw.k[4 * u + 2 * kk + (e >> 1)];
                         uint32_t p[3];
                         split2<CT>(__uint_as_float(w[2 * (e & 1)]), __uint_as_float(w[2 * (e & 1) + 1]), p);
 #pragma unroll
                         for (int i = 0; i < 3; i++) kf[i][e] = p[i];
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < RT; i++) s[i][u] = dot<CT>(kf, qf[i][kk], s[i][u]);
+                s[u] = dot<CT>(kf, qf[kk], s[u]);
             }
         }
-        if (next < nt) loadk(next);
+        if (next < nt) keys(next);
 
-        u32x4v pf[RT][KD::NQ];
-        float al[RT];
+        if (k0 < inner_lo || k0 + TK > min(inner_hi, stop)) {
+            // keys of the segment up to its end that lie in [lo, hi)
+            const uint32_t top = min(hi, stop);
 #pragma unroll
-        for (int i = 0; i < RT; i++) {
-            if (!(k0 >= inner_lo[i] && k0 + 32 <= min(inner_hi[i], stop))) {
-                // keys of the segment up to its end that lie in [lo, hi)
-                const uint32_t top = min(hi[i], stop);
+            for (int u = 0; u < 2 * SUB; u++) {
+                const uint32_t first = k0 + 16 * u + 4 * g;
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const uint32_t key = k0 + 16 * u + 4 * g + r;
-                        s[i][u][r] = key >= lo[i] && key < top ? s[i][u][r] : -INFINITY;
-                    }
+                for (int e = 0; e < 4; e++) s[u][e] = first + e >= lo && first + e < top ? s[u][e] : -INFINITY;
+                if constexpr (CT == DT_F8) {  // a scale byte past the segment may stand for anything
+                    const uint32_t n = stop > first ? min(stop - first, 4u) : 0;
+                    raw.vs[u] &= n == 4 ? ~0u : (1u << (8 * n)) - 1;
+                }
             }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[i][u][r]);
-            mx = rows_max(mx);
-            const float sn = fminf(sub[i], -(mx * c[i]));
-            al[i] = sn == sub[i] ? 1.0f : __builtin_amdgcn_exp2f(sn - sub[i]);
-            sub[i] = sn;
-            const float su = sn == INFINITY ? 0.0f : sn;
-            float x8[8], sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x8[j] = __builtin_amdgcn_exp2f(fmaf(s[i][j >> 2][j & 3], c[i], su));
-                sum += x8[j];
-            }
-            ls[i] = fmaf(ls[i], al[i], sum);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if constexpr (CT == DT_F8) x8[j] *= f8_pow2((vsc[j >> 2] >> (8 * (j & 3))) & 255u);
-                else x8[j] *= KD::PS;
-            }
-            split8<CT>(x8, pf[i]);
         }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2 * SUB; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[u][e]);
+        mx = rows_max(mx);
+        const float sn = fminf(sub, -(mx * c));
+        const float al = sn == sub ? 1.0f : __builtin_amdgcn_exp2f(sn - sub);  // brings older sums to the new maximum
+        sub = sn;
+        const float su = sn == INFINITY ? 0.0f : sn;
+        u32x4v pf[SUB][KD::NQ];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SUB; i++) {
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                p[j] = __builtin_amdgcn_exp2f(fmaf(s[2 * i + (j >> 2)][j & 3], c, su));
+                sum += p[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if constexpr (CT == DT_F8) p[j] *= f8_pow2((raw.vs[2 * i + (j >> 2)] >> (8 * (j & 3))) & 255u);
+                else p[j] *= KD::PS;
+            }
+            split8<CT>(p, pf[i]);
+        }
+        ls = fmaf(ls, al, sum);
 
         // p . v: a tile's sum starts from zero and joins the running one in one rounding.
 #pragma unroll
         for (int d = 0; d < 4; d++) {
-            u32x4v vf[KD::NC];
+            f32x4v ot = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if constexpr (CT == DT_F8) {
-                    const uint32_t w = __builtin_amdgcn_perm(vr[2 * e + 1], vr[2 * e], d < 2 ? 0x05010400u : 0x07030602u);
-                    vf[0][e] = d & 1 ? f8_bf16x2<true>(w, 1.0f) : f8_bf16x2<false>(w, 1.0f);
-                } else if constexpr (CT == DT_F16) {
-                    vf[0][e] = __builtin_amdgcn_perm(vr[2 * (2 * e + 1) + (d >> 1)], vr[2 * (2 * e) + (d >> 1)],
-                                                     d & 1 ? 0x07060302u : 0x05040100u);
-                } else {
-                    uint32_t p[3];
-                    split2<CT>(__uint_as_float(vr[4 * (2 * e) + d]), __uint_as_float(vr[4 * (2 * e + 1) + d]), p);
+            for (int i = 0; i < SUB; i++) {
+                u32x4v vf[KD::NC];
 #pragma unroll
-                    for (int i = 0; i < 3; i++) vf[i][e] = p[i];
+                for (int e = 0; e < 4; e++) {
+                    const int j = 8 * i + 2 * e;
+                    if constexpr (CT == DT_F8) {
+                        const uint32_t w = __builtin_amdgcn_perm(raw.v[j + 1], raw.v[j], d < 2 ? 0x05010400u : 0x07030602u);
+                        vf[0][e] = d & 1 ? f8_bf16x2<true>(w, 1.0f) : f8_bf16x2<false>(w, 1.0f);
+                    } else if constexpr (CT == DT_F16) {
+                        vf[0][e] = __builtin_amdgcn_perm(raw.v[2 * (j + 1) + (d >> 1)], raw.v[2 * j + (d >> 1)],
+                                                         d & 1 ? 0x07060302u : 0x05040100u);
+                    } else {
+                        uint32_t w[3];
+                        split2<CT>(__uint_as_float(raw.v[4 * j + d]), __uint_as_float(raw.v[4 * (j + 1) + d]), w);
+#pragma unroll
+                        for (int q = 0; q < 3; q++) vf[q][e] = w[q];
+                    }
                 }
+                ot = dot<CT>(vf, pf[i], ot);
             }
 #pragma unroll
-            for (int i = 0; i < RT; i++) {
-                const f32x4v ot = dot<CT>(vf, pf[i], f32x4v{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                for (int r = 0; r < 4; r++) o[i][d][r] = fmaf(o[i][d][r], al[i], ot[r]);
-            }
+            for (int e = 0; e < 4; e++) o[d][e] = fmaf(o[d][e], al, ot[e]);
         }
-        if (next < nt) loadv(next);
+        if (next < nt) values(next);
     }
 
     // The waves' parts of each row meet in wave order: a thread joins four dims of a row.
-    float *ms = part + AS_WAVES * 16 * RT * AS_LD, *sums = ms + AS_WAVES * 16 * RT;
+    {
+        float *p = part + (wave * 16 + l16) * AS_LD + 16 * g;
 #pragma unroll
-    for (int i = 0; i < RT; i++) {
-        float *p = part + ((wave * RT + i) * 16 + l16) * AS_LD + 16 * g;
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            *reinterpret_cast<float4 *>(p + 4 * r) = make_float4(o[i][0][r], o[i][1][r], o[i][2][r], o[i][3][r]);
-        const float l = ls[i] + __shfl_xor(ls[i], 16, 64), all = l + __shfl_xor(l, 32, 64);
+        for (int e = 0; e < 4; e++) *reinterpret_cast<float4 *>(p + 4 * e) = make_float4(o[0][e], o[1][e], o[2][e], o[3][e]);
+        const float l = ls + __shfl_xor(ls, 16, 64), all = l + __shfl_xor(l, 32, 64);
         if (g == 0) {
-            ms[(wave * RT + i) * 16 + l16] = sub[i];
-            sums[(wave * RT + i) * 16 + l16] = all;
+            ms[wave * 16 + l16] = sub;
+            sums[wave * 16 + l16] = all;
         }
     }
-    if (tid < AS_WAVES) redo[tid] = 0;
+    if (tid < AS_WAVES / 2) redo[tid] = 0;
     __syncthreads();
     for (uint32_t j = tid; j < span * 16; j += 64 * AS_WAVES) {
-        const uint32_t rr = j / 16, d4 = 4 * (j & 15), r = it.r0 + rr;  // row rr of the workgroup
-        if (r >= it.r1) continue;
-        const uint32_t row = r / G, head = it.kvh * G + r % G;
-        uint32_t b;
+        const uint32_t rr = j / 16, d4 = 4 * (j & 15), rj = r0 + rr;  // row rr of the workgroup
+        if (rj >= r1) continue;
+        const uint32_t rowj = rj / G, head = kvh * G + rj % G;
+        uint32_t rb;
         uint64_t slot;
-        if (!a.rows.at(row, b, slot)) continue;
-        // the row's place in its waves' parts: waves grp * keys + w, tile and row inside
-        const uint32_t grp = rr / (16 * RT), in = rr - grp * 16 * RT;
+        if (!a.rows.at(rowj, rb, slot)) continue;
+        const uint32_t w0 = rr / 16 * a.keys, in = rr & 15;  // the row's waves, its place in each
         float m = INFINITY;
-        for (uint32_t w = 0; w < a.keys; w++) m = fminf(m, ms[(grp * a.keys + w) * 16 * RT + in]);
+        for (uint32_t w = 0; w < a.keys; w++) m = fminf(m, ms[(w0 + w) * 16 + in]);
         float l = 0.0f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (uint32_t w = 0; w < a.keys; w++) {
-            const uint32_t at = (grp * a.keys + w) * 16 * RT + in;
+            const uint32_t at = (w0 + w) * 16 + in;
             const float mw = ms[at], f = mw == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mw);
             const float4 v = *reinterpret_cast<const float4 *>(part + at * AS_LD + d4);
             l = fmaf(sums[at], f, l);
@@ -525,15 +556,15 @@ __global__ __launch_bounds__(64 * AS_WAVES) void attention_shared_kernel(SharedA
         }
         if constexpr (APART) {
             const uint32_t S = a.sp + a.so;
-            const size_t at = (static_cast<size_t>(row) * a.hq + head) * S + it.split;
+            const size_t at = (static_cast<size_t>(rowj) * a.hq + head) * S + (own ? a.sp + mine : mine);
             float2 *ml = reinterpret_cast<float2 *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * S * 64);
-            if (m != INFINITY) *reinterpret_cast<float4 *>(a.part + at * 64 + d4) = acc;
+            *reinterpret_cast<float4 *>(a.part + at * 64 + d4) = acc;
             if (d4 == 0) ml[at] = make_float2(m, l);
         } else {
             const float f = 1.0f / (l * KD::PS);
             acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
             if (fabsf(acc.x) < INFINITY && fabsf(acc.y) < INFINITY && fabsf(acc.z) < INFINITY && fabsf(acc.w) < INFINITY)
-                *reinterpret_cast<float4 *>(a.out + static_cast<size_t>(row) * a.ldo + head * 64 + d4) = acc;
+                *reinterpret_cast<float4 *>(a.out + static_cast<size_t>(rowj) * a.ldo + head * 64 + d4) = acc;
             else
                 atomicOr(&redo[rr / 32], 1u << (rr % 32));
         }
@@ -543,14 +574,14 @@ __global__ __launch_bounds__(64 * AS_WAVES) void attention_shared_kernel(SharedA
         __syncthreads();
         for (uint32_t rr = wave; rr < span; rr += AS_WAVES) {
             if (!((redo[rr / 32] >> (rr % 32)) & 1)) continue;
-            const uint32_t r = it.r0 + rr, row = r / G, head = it.kvh * G + r % G;
-            uint32_t b;
+            const uint32_t rj = r0 + rr, rowj = rj / G, head = kvh * G + rj % G;
+            uint32_t rb;
             uint64_t slot;
             uint32_t l, e;
-            a.rows.at(row, b, slot);
+            a.rows.at(rowj, rb, slot);
             row_keys(a, slot, l, e);
-            attend_wave<CT>(a.q + static_cast<size_t>(row) * a.ldq + head * 64, h, l, e, a.scale,
-                            a.out + static_cast<size_t>(row) * a.ldo + head * 64);
+            attend_wave<CT>(a.q + static_cast<size_t>(rowj) * a.ldq + head * 64, h, l, e, a.scale,
+                            a.out + static_cast<size_t>(rowj) * a.ldo + head * 64);
         }
     }
 }
@@ -571,18 +602,27 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SharedArgs a) {
     const float *o = a.part + at * 64;
     float m = INFINITY, l = 0.0f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t s = p; s < S; s += 16) {
-        const float2 e = ml[s];
-        if (e.x == INFINITY) continue;
-        const float4 x = *reinterpret_cast<const float4 *>(o + static_cast<size_t>(s) * 64 + d4);
-        const float mn = fminf(m, e.x);
-        const float f = m == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mn - m), k = __builtin_amdgcn_exp2f(mn - e.x);
-        m = mn;
-        l = fmaf(l, f, e.y * k);
-        v.x = fmaf(v.x, f, x.x * k);
-        v.y = fmaf(v.y, f, x.y * k);
-        v.z = fmaf(v.z, f, x.z * k);
-        v.w = fmaf(v.w, f, x.w * k);
+    for (uint32_t s0 = p; s0 < S; s0 += 64) {  // four parts' loads at once
+        float2 e[4];
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t s = min(s0 + 16 * i, S - 1);
+            e[i] = ml[s];
+            x[i] = *reinterpret_cast<const float4 *>(o + static_cast<size_t>(s) * 64 + d4);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (s0 + 16 * i >= S || e[i].x == INFINITY) continue;  // a part without keys of the row: its sums are zeros
+            const float mn = fminf(m, e[i].x);
+            const float f = m == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mn - m), k = __builtin_amdgcn_exp2f(mn - e[i].x);
+            m = mn;
+            l = fmaf(l, f, e[i].y * k);
+            v.x = fmaf(v.x, f, x[i].x * k);
+            v.y = fmaf(v.y, f, x[i].y * k);
+            v.z = fmaf(v.z, f, x[i].z * k);
+            v.w = fmaf(v.w, f, x[i].w * k);
+        }
     }
     acc[p][tid & 15] = v;
     if (d4 == 0) {
@@ -611,18 +651,16 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SharedArgs a) {
     attend_wave<CT>(a.q + static_cast<size_t>(row) * a.ldq + head * 64, head_kv<CT>(a, b, head / (a.hq / a.hkv)), lo, hi, a.scale, out);
 }
 
-template <int CT, int RT>
+template <int CT>
 int launch_kind(const SharedArgs &a, bool apart, hipStream_t stream) {
-    const uint32_t G = a.hq / a.hkv, span = AS_WAVES / a.keys * 16 * RT, B = a.rows.B, T = a.rows.T;
-    const uint32_t lds = AS_WAVES * 16 * RT * (AS_LD + 2) * 4;
+    const uint32_t G = a.hq / a.hkv, span = AS_WAVES / a.keys * 16, B = a.rows.B, T = a.rows.T;
     const uint64_t own = static_cast<uint64_t>(B) * a.hkv * ((T * G + span - 1) / span);
     if (!apart) {
-        hipLaunchKernelGGL((attention_shared_kernel<CT, RT, false>), dim3(static_cast<uint32_t>(own)), dim3(64 * AS_WAVES), lds, stream, a);
+        hipLaunchKernelGGL((attention_shared_kernel<CT, false>), dim3(static_cast<uint32_t>(own)), dim3(64 * AS_WAVES), 0, stream, a);
         return check_launch("attention shared");
     }
     const uint64_t pre = static_cast<uint64_t>(a.sp) * a.hkv * ((static_cast<uint64_t>(B) * T * G + span - 1) / span);
-    hipLaunchKernelGGL((attention_shared_kernel<CT, RT, true>), dim3(static_cast<uint32_t>(pre + own * a.so)), dim3(64 * AS_WAVES), lds,
-                       stream, a);
+    hipLaunchKernelGGL((attention_shared_kernel<CT, true>), dim3(static_cast<uint32_t>(pre + own * a.so)), dim3(64 * AS_WAVES), 0, stream, a);
     int rc = check_launch("attention shared (parts)");
     if (rc) return rc;
     hipLaunchKernelGGL(attention_join_kernel<CT>, dim3(B * T * a.hq), dim3(256), 0, stream, a);
@@ -631,24 +669,36 @@ int launch_kind(const SharedArgs &a, bool apart, hipStream_t stream) {
 
 }  // namespace
 
+// Where the work goes.  A CU holds one workgroup at a time (164 registers a lane), which takes about 2 us for each
+// 512 keys of its rows, and the second kernel of the split form costs about as much as 1200 keys.
+//   - keys: the waves of a workgroup share 16 rows and split the keys, unless that makes more workgroups than
+//     CUs and other rows can take the waves instead.  Measured, us for keys 8 / 4 / 2 / 1: 8 sequences of 130 rows over 1000
+//     + 256 keys (912 row tiles) 29.3 / 28.9 / 26.0 / 45.5, 1 of 300 rows (264) 11.7 / 9.7 / 12.2 / 17.1, 4 of 40 rows
+//     over 500 + 300 (144) 9.3 / 13.2 / 19.4 / 32.0.
+//   - apart: all keys of the prefix (once for all rows) and of the sequences spread over the CUs evenly, if the
+//     longest workgroup then costs less than the longest in one pass.  Measured, one pass against apart: 64 sequences
+//     of up to 4096 keys 21.0 against 17.8 us, 128 of them 23.0 against 27.8, 16 sequences over 8192 + 512 keys
+//     36.5 against 10.1, 128 over 2048 + 512 15.7 against 16.6, 256 over 4096 + 1024 47.2 against 38.8.
 SharedPlan shared_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t prefix_len, uint32_t len_max, uint32_t window,
                        int ct) {
-    const uint32_t G = hq / hkv;
-    SharedPlan p{1, AS_WAVES, false, 0, 0};
-    (void)ct;
-    // keys an own row attends at most
-    uint64_t own = len_max, pre = prefix_len;
-    if (window) own = own < window ? own : window, pre = pre < window ? pre : window;
-    const uint64_t rows = static_cast<uint64_t>(T) * G, tiles = (rows + 15) / 16;
-    // waves that other rows can use
-    while (p.keys > 1 && tiles * p.keys > AS_WAVES * 2) p.keys /= 2;
-    const uint64_t span = AS_WAVES / p.keys * 16, groups = static_cast<uint64_t>(B) * hkv * ((rows + span - 1) / span);
-    const uint64_t steps = (own + pre + 31) / 32 / p.keys;  // tiles a wave
-    if (p.keys == AS_WAVES && groups < 256 && steps > 4) {
+    const uint64_t tk = ct == DT_F32 ? Raw<DT_F32>::TK : Raw<DT_F8>::TK, cus = 256;
+    SharedPlan p{AS_WAVES, false, 0, 0, 0};
+    // keys a row attends at most
+    const uint64_t own = std::max<uint64_t>(1, window ? std::min<uint64_t>(len_max, static_cast<uint64_t>(window) + T - 1) : len_max);
+    const uint64_t pre = window ? std::min(prefix_len, window) : prefix_len;
+    const uint64_t rows = static_cast<uint64_t>(T) * (hq / hkv), heads = static_cast<uint64_t>(B) * hkv;
+    auto groups = [&](uint64_t keys) { return heads * ((rows + AS_WAVES / keys * 16 - 1) / (AS_WAVES / keys * 16)); };
+    while (p.keys > 1 && groups(p.keys) > cus && groups(p.keys / 2) < groups(p.keys)) p.keys /= 2;
+    if (p.keys != AS_WAVES) return p;
+    const uint64_t own_groups = groups(AS_WAVES), pre_groups = pre ? hkv * ((B * rows + 15) / 16) : 0;
+    const uint64_t share = (pre_groups * pre + own_groups * own) / cus, part = std::max<uint64_t>(share, 256);  // keys a workgroup
+    const uint64_t sp = pre ? std::max<uint64_t>(1, pre / part) : 0, so = std::max<uint64_t>(1, own / part);
+    const uint64_t longest = std::max({share, pre ? pre / sp : 0, own / so});
+    if (longest + 1200 < (own_groups + cus - 1) / cus * (pre + own)) {
         p.apart = true;
-        p.so = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((own + 255) / 256, 512 / groups)));
-        const uint64_t pg = static_cast<uint64_t>(hkv) * ((B * rows + span - 1) / span);
-        p.sp = pre ? static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((pre + 255) / 256, 512 / pg))) : 0;
+        p.sp = static_cast<uint32_t>(sp);
+        p.so = static_cast<uint32_t>(so);
+        p.run = static_cast<uint32_t>((own + so * tk - 1) / (so * tk));
     }
     return p;
 }
@@ -658,9 +708,10 @@ int launch_attention_shared(const SharedArgs &a, const SharedPlan &p, int ct, hi
     b.keys = p.keys;
     b.sp = p.sp;
     b.so = p.so;
-    if (ct == DT_F32) return launch_kind<DT_F32, 1>(b, p.apart, stream);
-    if (ct == DT_F16) return launch_kind<DT_F16, 1>(b, p.apart, stream);
-    return launch_kind<DT_F8, 1>(b, p.apart, stream);
+    b.run = p.run;
+    if (ct == DT_F32) return launch_kind<DT_F32>(b, p.apart, stream);
+    if (ct == DT_F16) return launch_kind<DT_F16>(b, p.apart, stream);
+    return launch_kind<DT_F8>(b, p.apart, stream);
 }
 
 }  // namespace mt

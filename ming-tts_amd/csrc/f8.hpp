@@ -93,10 +93,10 @@ struct RowsArgs {
 
 // How mt_attention_shared places its work (shared_plan).
 struct SharedPlan {
-    uint32_t tiles;     // tiles of 16 rows a wave holds (1 or 2)
     uint32_t keys;      // waves of a workgroup that share rows and split their keys (the rest: other rows)
     bool apart;         // prefix and own keys in workgroups of their own, joined by a second kernel
     uint32_t sp, so;    // parts of the prefix's and of the own keys then
+    uint32_t run;       // tiles of own keys a part
 };
 
 // The operands of mt_attention_shared.
@@ -109,7 +109,7 @@ struct SharedArgs {
     uint32_t prefix_len;
     float scale;
     float *part;    // apart: [B T, hq, sp + so] sums of 64 and behind them as many pairs (minus the maximum, the weights' sum)
-    uint32_t sp, so;
+    uint32_t sp, so, run;
     uint32_t keys;  // waves that split the keys
 };
 
