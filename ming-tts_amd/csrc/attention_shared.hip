@@ -176,7 +176,8 @@ __device__ __forceinline__ float rows_max(float v) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-constexpr int AS_WAVES = 8;
+constexpr int AS_WAVES = 8;       // of a workgroup
+constexpr int AS_PART_WAVES = 4;  // of one that has a part of the keys (apart)
 constexpr uint32_t AS_LD = 68;  // floats of a row in the waves' hand-over (64 and a 16-byte skew)
 
 // One wave's 16 rows and TK = 32 SUB keys at a time: the raw keys and values of a tile.  Lane (l16, g) holds dims
@@ -244,17 +245,18 @@ __device__ __forceinline__ V pick(bool second, V first, V other) {
 }
 
 template <int CT, bool APART>
-__global__ __launch_bounds__(64 * AS_WAVES) void attention_shared_kernel(SharedArgs a) {
+__global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void attention_shared_kernel(SharedArgs a) {
+    constexpr int WAVES = APART ? AS_PART_WAVES : AS_WAVES;
     typedef Kind<CT> KD;
     constexpr int SUB = Raw<CT>::SUB;
     constexpr uint32_t ROW = Cached<CT>::ROW, TK = Raw<CT>::TK;
-    __shared__ __attribute__((aligned(16))) float part[AS_WAVES * 16 * AS_LD];
-    __shared__ float ms[AS_WAVES * 16], sums[AS_WAVES * 16];
-    __shared__ uint32_t redo[AS_WAVES / 2];
+    __shared__ __attribute__((aligned(16))) float part[WAVES * 16 * AS_LD];
+    __shared__ float ms[WAVES * 16], sums[WAVES * 16];
+    __shared__ uint32_t redo[WAVES / 2];
     const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t wk = wave % a.keys, wr = wave / a.keys;
-    const uint32_t G = a.hq / a.hkv, T = a.rows.T, span = AS_WAVES / a.keys * 16;  // rows of a workgroup
+    const uint32_t G = a.hq / a.hkv, T = a.rows.T, span = WAVES / a.keys * 16;  // rows of a workgroup
     const uint32_t P = a.prefix_len;
 
     // The workgroup's rows [r0, r1) of all rows (sequence, t, head of the group) of one key head, whose own keys are
@@ -530,9 +532,9 @@ __global__ __launch_bounds__(64 * AS_WAVES) void attention_shared_kernel(SharedA
             sums[wave * 16 + l16] = all;
         }
     }
-    if (tid < AS_WAVES / 2) redo[tid] = 0;
+    if (tid < WAVES / 2) redo[tid] = 0;
     __syncthreads();
-    for (uint32_t j = tid; j < span * 16; j += 64 * AS_WAVES) {
+    for (uint32_t j = tid; j < span * 16; j += 64 * WAVES) {
         const uint32_t rr = j / 16, d4 = 4 * (j & 15), rj = r0 + rr;  // row rr of the workgroup
         if (rj >= r1) continue;
         const uint32_t rowj = rj / G, head = kvh * G + rj % G;
@@ -572,7 +574,7 @@ __global__ __launch_bounds__(64 * AS_WAVES) void attention_shared_kernel(SharedA
     if constexpr (!APART) {
         // Rows with an output that is not finite once more, each from its own keys alone.
         __syncthreads();
-        for (uint32_t rr = wave; rr < span; rr += AS_WAVES) {
+        for (uint32_t rr = wave; rr < span; rr += WAVES) {
             if (!((redo[rr / 32] >> (rr % 32)) & 1)) continue;
             const uint32_t rj = r0 + rr, rowj = rj / G, head = kvh * G + rj % G;
             uint32_t rb;
@@ -586,84 +588,83 @@ __global__ __launch_bounds__(64 * AS_WAVES) void attention_shared_kernel(SharedA
     }
 }
 
-// The parts of a row and head, of which there are sp + so, joined: thread (p, d4) takes every 16th part's four dims.
+// The parts of a row and head, of which there are sp + so, joined: lane d is dim d, a wave takes every waves-th part, and the
+// waves' sums meet in wave order.
+constexpr uint32_t AJ_WAVES = 16;  // at most
+
 template <int CT>
-__global__ __launch_bounds__(256) void attention_join_kernel(SharedArgs a) {
-    __shared__ float4 acc[16][16];
-    __shared__ float sums[16], ms[16];
-    const uint32_t tid = threadIdx.x, p = tid / 16, d4 = 4 * (tid & 15);
+__global__ __launch_bounds__(64 * AJ_WAVES) void attention_join_kernel(SharedArgs a) {
+    __shared__ float acc[AJ_WAVES][64], sums[AJ_WAVES], ms[AJ_WAVES];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / 64;
     const uint32_t row = blockIdx.x / a.hq, head = blockIdx.x - row * a.hq, S = a.sp + a.so;
     uint32_t b;
     uint64_t slot;
-    uint32_t lo, hi;
     if (!a.rows.at(row, b, slot)) return;
     const size_t at = static_cast<size_t>(blockIdx.x) * S;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part + static_cast<size_t>(a.rows.B) * a.rows.T * a.hq * S * 64) + at;
-    const float *o = a.part + at * 64;
-    float m = INFINITY, l = 0.0f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t s0 = p; s0 < S; s0 += 64) {  // four parts' loads at once
+    const float *o = a.part + at * 64 + lane;
+    float m = INFINITY, l = 0.0f, v = 0.0f;
+    for (uint32_t s0 = wave; s0 < S; s0 += 4 * waves) {  // four parts' loads at once
         float2 e[4];
-        float4 x[4];
+        float x[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t s = min(s0 + 16 * i, S - 1);
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t s = min(s0 + i * waves, S - 1);
             e[i] = ml[s];
-            x[i] = *reinterpret_cast<const float4 *>(o + static_cast<size_t>(s) * 64 + d4);
+            x[i] = o[static_cast<size_t>(s) * 64];
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (s0 + 16 * i >= S || e[i].x == INFINITY) continue;  // a part without keys of the row: its sums are zeros
+        for (uint32_t i = 0; i < 4; i++) {
+            if (s0 + i * waves >= S || e[i].x == INFINITY) continue;  // (a part without a key of the row has no sums)
             const float mn = fminf(m, e[i].x);
             const float f = m == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mn - m), k = __builtin_amdgcn_exp2f(mn - e[i].x);
             m = mn;
             l = fmaf(l, f, e[i].y * k);
-            v.x = fmaf(v.x, f, x[i].x * k);
-            v.y = fmaf(v.y, f, x[i].y * k);
-            v.z = fmaf(v.z, f, x[i].z * k);
-            v.w = fmaf(v.w, f, x[i].w * k);
+            v = fmaf(v, f, x[i] * k);
         }
     }
-    acc[p][tid & 15] = v;
-    if (d4 == 0) {
-        sums[p] = l;
-        ms[p] = m;
+    if (waves > 1) {
+        acc[wave][lane] = v;
+        if (lane == 0) {
+            sums[wave] = l;
+            ms[wave] = m;
+        }
+        __syncthreads();
+        if (wave > 0) return;
+        m = INFINITY;
+        for (uint32_t i = 0; i < waves; i++) m = fminf(m, ms[i]);
+        l = v = 0.0f;
+        for (uint32_t i = 0; i < waves; i++) {
+            const float f = ms[i] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - ms[i]);
+            l = fmaf(sums[i], f, l);
+            v = fmaf(acc[i][lane], f, v);
+        }
     }
-    __syncthreads();
-    if (tid >= 64) return;  // one wave joins the 16: lane d is dim d
-    float mm = INFINITY;
-#pragma unroll
-    for (int i = 0; i < 16; i++) mm = fminf(mm, ms[i]);
-    float total = 0.0f, x = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const float f = ms[i] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mm - ms[i]);
-        total = fmaf(sums[i], f, total);
-        x = fmaf(reinterpret_cast<const float *>(acc[i])[tid], f, x);
-    }
-    x *= 1.0f / (total * Kind<CT>::PS);
+    v *= 1.0f / (l * Kind<CT>::PS);
     float *out = a.out + static_cast<size_t>(row) * a.ldo + head * 64;
-    if (__all(fabsf(x) < INFINITY)) {
-        out[tid] = x;
+    if (__all(fabsf(v) < INFINITY)) {
+        out[lane] = v;
         return;
     }
+    uint32_t lo, hi;
     row_keys(a, slot, lo, hi);
     attend_wave<CT>(a.q + static_cast<size_t>(row) * a.ldq + head * 64, head_kv<CT>(a, b, head / (a.hq / a.hkv)), lo, hi, a.scale, out);
 }
 
 template <int CT>
 int launch_kind(const SharedArgs &a, bool apart, hipStream_t stream) {
-    const uint32_t G = a.hq / a.hkv, span = AS_WAVES / a.keys * 16, B = a.rows.B, T = a.rows.T;
+    const uint32_t G = a.hq / a.hkv, span = (apart ? AS_PART_WAVES : AS_WAVES) / a.keys * 16, B = a.rows.B, T = a.rows.T;
     const uint64_t own = static_cast<uint64_t>(B) * a.hkv * ((T * G + span - 1) / span);
     if (!apart) {
         hipLaunchKernelGGL((attention_shared_kernel<CT, false>), dim3(static_cast<uint32_t>(own)), dim3(64 * AS_WAVES), 0, stream, a);
         return check_launch("attention shared");
     }
     const uint64_t pre = static_cast<uint64_t>(a.sp) * a.hkv * ((static_cast<uint64_t>(B) * T * G + span - 1) / span);
-    hipLaunchKernelGGL((attention_shared_kernel<CT, true>), dim3(static_cast<uint32_t>(pre + own * a.so)), dim3(64 * AS_WAVES), 0, stream, a);
+    hipLaunchKernelGGL((attention_shared_kernel<CT, true>), dim3(static_cast<uint32_t>(pre + own * a.so)), dim3(64 * AS_PART_WAVES), 0, stream, a);
     int rc = check_launch("attention shared (parts)");
     if (rc) return rc;
-    hipLaunchKernelGGL(attention_join_kernel<CT>, dim3(B * T * a.hq), dim3(256), 0, stream, a);
+    const uint32_t waves = std::min(AJ_WAVES, (a.sp + a.so + 1) / 2);
+    hipLaunchKernelGGL(attention_join_kernel<CT>, dim3(B * T * a.hq), dim3(64 * waves), 0, stream, a);
     return check_launch("attention shared (join)");
 }
 
@@ -691,10 +692,12 @@ SharedPlan shared_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
     while (p.keys > 1 && groups(p.keys) > cus && groups(p.keys / 2) < groups(p.keys)) p.keys /= 2;
     if (p.keys != AS_WAVES) return p;
     const uint64_t own_groups = groups(AS_WAVES), pre_groups = pre ? hkv * ((B * rows + 15) / 16) : 0;
-    const uint64_t share = (pre_groups * pre + own_groups * own) / cus, part = std::max<uint64_t>(share, 256);  // keys a workgroup
-    const uint64_t sp = pre ? std::max<uint64_t>(1, pre / part) : 0, so = std::max<uint64_t>(1, own / part);
+    const uint64_t share = (pre_groups * pre + own_groups * own) / (2 * cus), part = std::max<uint64_t>(share, 256);  // keys a workgroup, two a CU
+    // At most 128 parts each, or the second kernel becomes the longer one.
+    const uint64_t sp = pre ? std::min<uint64_t>(std::max<uint64_t>(1, pre / part), 128) : 0;
+    const uint64_t so = std::min<uint64_t>(std::max<uint64_t>(1, own / part), 128);
     const uint64_t longest = std::max({share, pre ? pre / sp : 0, own / so});
-    if (longest + 1200 < (own_groups + cus - 1) / cus * (pre + own)) {
+    if (2 * longest + 1200 < (own_groups + cus - 1) / cus * (pre + own)) {
         p.apart = true;
         p.sp = static_cast<uint32_t>(sp);
         p.so = static_cast<uint32_t>(so);
@@ -705,7 +708,7 @@ SharedPlan shared_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
 
 int launch_attention_shared(const SharedArgs &a, const SharedPlan &p, int ct, hipStream_t stream) {
     SharedArgs b = a;
-    b.keys = p.keys;
+    b.keys = p.apart ? AS_PART_WAVES : p.keys;
     b.sp = p.sp;
     b.so = p.so;
     b.run = p.run;
