@@ -67,24 +67,22 @@ __device__ __forceinline__ u32x2v block_encode(const float *v, uint32_t &s) {
     return u32x2v{f8_encode4(v[0], v[1], v[2], v[3], inv), f8_encode4(v[4], v[5], v[6], v[7], inv)};
 }
 
-// One row a workgroup: 16 lanes a block of 128, eight values each.
+// Rows normalised first: one row a workgroup, 16 lanes a block of 128, eight values each.
 template <int XT>
-__global__ __launch_bounds__(256) void quantize_kernel(const void *x, uint32_t K, uint32_t ldx, const uint16_t *norm, int nt,
-                                                       float eps, uint8_t *codes, uint32_t ldq, uint8_t *scales, uint32_t lds) {
+__global__ __launch_bounds__(256) void quantize_norm_kernel(const void *x, uint32_t K, uint32_t ldx, const uint16_t *norm, int nt,
+                                                            float eps, uint8_t *codes, uint32_t ldq, uint8_t *scales, uint32_t lds) {
     constexpr uint32_t ES = XT == DT_F32 ? 4 : 2;
     extern __shared__ float sq[];
     const uint32_t row = blockIdx.x, l16 = threadIdx.x & 15, grp = threadIdx.x / 16, blocks = (K + 127) / 128;
     const char *xr = static_cast<const char *>(x) + static_cast<size_t>(row) * ldx * ES;
-    float v[8], rs = 1.0f;
-    if (norm) {
-        for (uint32_t kb = grp; kb < blocks; kb += 16) {
-            load_x8<XT>(xr, kb * 128 + 8 * l16, K, nullptr, 0, 1.0f, v);
-            const float t = block_square(v);
-            if (l16 == 0) sq[kb] = t;
-        }
-        __syncthreads();
-        rs = row_factor(sq, blocks, l16, K, eps);
+    float v[8];
+    for (uint32_t kb = grp; kb < blocks; kb += 16) {
+        load_x8<XT>(xr, kb * 128 + 8 * l16, K, nullptr, 0, 1.0f, v);
+        const float t = block_square(v);
+        if (l16 == 0) sq[kb] = t;
     }
+    __syncthreads();
+    const float rs = row_factor(sq, blocks, l16, K, eps);
     for (uint32_t kb = grp; kb < lds; kb += 16) {  // the row's padding bytes included
         const uint32_t k = kb * 128 + 8 * l16;
         load_x8<XT>(xr, k, K, norm, nt, rs, v);
@@ -93,6 +91,44 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void *x, uint32_t K
         if (k < K) *reinterpret_cast<u32x2v *>(codes + static_cast<size_t>(row) * ldq + k) = w;
         if (l16 == 0) scales[static_cast<size_t>(row) * lds + kb] = static_cast<uint8_t>(kb < blocks ? s : 0);
     }
+}
+
+// Rows as they are: 16 lanes a block of 128, as many blocks in flight as the rows have.  Lane l holds values 4 l .. + 3 and
+// 64 + 4 l .. + 3, so a load instruction's lanes stand side by side.  Bound: the bytes.
+template <int XT>
+__global__ __launch_bounds__(256) void quantize_kernel(const void *x, uint64_t all, uint32_t K, uint32_t ldx, uint8_t *codes,
+                                                       uint32_t ldq, uint8_t *scales, uint32_t lds) {
+    constexpr uint32_t ES = XT == DT_F32 ? 4 : 2;
+    // The group's block of all rows' blocks (the padding bytes' too): the workgroup's first by a division, lds is 4 or more.
+    const uint64_t first = static_cast<uint64_t>(blockIdx.x) * 16;
+    const uint32_t l16 = threadIdx.x & 15;
+    if (first + threadIdx.x / 16 >= all) return;
+    size_t row = first / lds;
+    uint32_t kb = static_cast<uint32_t>(first - row * lds) + threadIdx.x / 16;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (kb >= lds) kb -= lds, row++;
+    const uint32_t k = kb * 128 + 4 * l16;
+    const char *xr = static_cast<const char *>(x) + row * ldx * ES + static_cast<size_t>(k) * ES;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (k + 64 * h >= K) continue;
+        if constexpr (XT == DT_F32) {
+            const float4 w = *reinterpret_cast<const float4 *>(xr + 64 * h * ES);
+            v[4 * h] = w.x; v[4 * h + 1] = w.y; v[4 * h + 2] = w.z; v[4 * h + 3] = w.w;
+        } else {
+            const u32x2v w = *reinterpret_cast<const u32x2v *>(xr + 64 * h * ES);
+            v[4 * h] = dec_lo<XT>(w[0]); v[4 * h + 1] = dec_hi<XT>(w[0]);
+            v[4 * h + 2] = dec_lo<XT>(w[1]); v[4 * h + 3] = dec_hi<XT>(w[1]);
+        }
+    }
+    uint32_t s;
+    const u32x2v w = block_encode(v, s);
+    uint8_t *c = codes + row * ldq + k;
+    if (k < K) *reinterpret_cast<uint32_t *>(c) = w[0];
+    if (k + 64 < K) *reinterpret_cast<uint32_t *>(c + 64) = w[1];
+    if (l16 == 0) scales[row * lds + kb] = static_cast<uint8_t>(kb * 128 < K ? s : 0);
 }
 
 // A lane's 32 codes of a row from k on (those past K as zeros) and the block's scale byte.
@@ -180,14 +216,10 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(F8LinearArgs a, int bt) 
             }
         }
     };
+    load_x(wave);  // first: loads return in order, and x has the longer way to go
     load_w(wave);
-    load_x(wave);
     for (uint32_t kb = wave; kb < blocks; kb += waves) {
         const uint32_t next = kb + waves;
-        bf16x8t wv[4], uv[4];
-        row_values(w, wv);
-        if constexpr (GATED) row_values(u, uv);
-        if (next < blocks) load_w(next);
         if constexpr (XT != DT_F8) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -204,9 +236,12 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(F8LinearArgs a, int bt) 
             xc.s = scale[m];
             wave_sync();
         }
-        bf16x8t xv[4];
+        bf16x8t xv[4], wv[4], uv[4];
         row_values(xc, xv);
         if (next < blocks) load_x(next);
+        row_values(w, wv);
+        if constexpr (GATED) row_values(u, uv);
+        if (next < blocks) load_w(next);
 #pragma unroll
         for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[i], xv[i], acc, 0, 0, 0);
         if constexpr (GATED) {
@@ -259,9 +294,19 @@ int few_rows(const F8LinearArgs &a, int bt, hipStream_t stream) {
 
 int launch_quantize_f8(const void *x, int xt, uint32_t rows, uint32_t K, uint32_t ldx, const uint16_t *norm, int nt, float eps,
                        uint8_t *codes, uint32_t ldq, uint8_t *scales, uint32_t lds, hipStream_t stream) {
-    const uint32_t shared = norm ? (K + 127) / 128 * 4 : 0;
+    if (norm) {
+        const uint32_t shared = (K + 127) / 128 * 4;
 #define QUANTIZE(XT) \
-    hipLaunchKernelGGL(quantize_kernel<XT>, dim3(rows), dim3(256), shared, stream, x, K, ldx, norm, nt, eps, codes, ldq, scales, lds)
+    hipLaunchKernelGGL(quantize_norm_kernel<XT>, dim3(rows), dim3(256), shared, stream, x, K, ldx, norm, nt, eps, codes, ldq, scales, lds)
+        if (xt == DT_F32) QUANTIZE(DT_F32);
+        else if (xt == DT_F16) QUANTIZE(DT_F16);
+        else QUANTIZE(DT_BF16);
+#undef QUANTIZE
+        return check_launch("quantize (norm)");
+    }
+    const uint64_t all = static_cast<uint64_t>(rows) * lds;
+    const dim3 grid(static_cast<uint32_t>((all + 15) / 16));
+#define QUANTIZE(XT) hipLaunchKernelGGL(quantize_kernel<XT>, grid, dim3(256), 0, stream, x, all, K, ldx, codes, ldq, scales, lds)
     if (xt == DT_F32) QUANTIZE(DT_F32);
     else if (xt == DT_F16) QUANTIZE(DT_F16);
     else QUANTIZE(DT_BF16);
