@@ -137,6 +137,9 @@ int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, ui
     int rc = validate_rows(who, B, T, hq, hkv);
     if (rc) return rc;
     if (hq == 0 || hq % hkv) return set_error(MT_EINVAL, "%s: hq %u must be a positive multiple of hkv %u", who, hq, hkv);
+    const uint64_t G = hq / hkv;
+    if (G > 4096 || static_cast<uint64_t>(B) * T * G > 0xFFFFFFFFull / G)
+        return set_error(MT_EINVAL, "%s: %u x %u rows of %u query heads a key head are too many", who, B, T, hq / hkv);
     if (B == 0 || T == 0) return MT_OK;
     SharedArgs a{};
     rc = validate_kv(who, "kv", kv, B, hkv, a.kv);

@@ -245,7 +245,7 @@ __device__ __forceinline__ V pick(bool second, V first, V other) {
 }
 
 template <int CT, bool APART>
-__global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void attention_shared_kernel(SharedArgs a) {
+__global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void attention_shared_kernel(SharedArgs a) {
     constexpr int WAVES = APART ? AS_PART_WAVES : AS_WAVES;
     typedef Kind<CT> KD;
     constexpr int SUB = Raw<CT>::SUB;
@@ -256,7 +256,8 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void atten
     const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t wk = wave % a.keys, wr = wave / a.keys;
-    const uint32_t G = a.hq / a.hkv, T = a.rows.T, span = WAVES / a.keys * 16;  // rows of a workgroup
+    const uint32_t G = a.group, T = a.rows.T, span = WAVES / a.keys * 16;  // rows of a workgroup
+    auto by_group = [&](uint32_t v) { return __umulhi(v, a.group_magic); };  // v / G (SharedArgs)
     const uint32_t P = a.prefix_len;
 
     // The workgroup's rows [r0, r1) of all rows (sequence, t, head of the group) of one key head, whose own keys are
@@ -289,14 +290,17 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void atten
 
     // The lane's row (all four g's the same one), its query's 16 dims and its keys [lo, hi) of the prefix and the own
     // keys together (none: not a row).
-    const uint32_t rw = r0 + wr * 16, r = rw + l16, row = r / G;
+    const uint32_t rw = r0 + wr * 16, r = rw + l16, row = G == 1 ? r : by_group(r), head = kvh * G + r - row * G;
     uint32_t lo = 0, hi = 0;
     float4 qv[4] = {};
     {
-        uint32_t rb;
-        uint64_t slot;
-        if (r < r1 && a.rows.at(row, rb, slot)) {
-            const float4 *p = reinterpret_cast<const float4 *>(a.q + static_cast<size_t>(row) * a.ldq + (kvh * G + r % G) * 64 + 16 * g);
+        uint32_t rb = b;
+        uint64_t slot = 0;
+        bool have = r < r1;
+        if (own) slot = (a.rows.pos ? a.rows.pos[b] : 0u) + static_cast<uint64_t>(row - b * T);
+        else have = have && a.rows.at(row, rb, slot);
+        if (have) {
+            const float4 *p = reinterpret_cast<const float4 *>(a.q + static_cast<size_t>(row) * a.ldq + head * 64 + 16 * g);
 #pragma unroll
             for (int e = 0; e < 4; e++) qv[e] = p[e];
             row_keys(a, slot, lo, hi);
@@ -308,7 +312,8 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void atten
     if (own) {
         if (rw < r1) {
             const uint64_t at = a.rows.pos ? a.rows.pos[b] : 0u;
-            const uint32_t first = (rw - b * T * G) / G, last = (min(rw + 16, r1) - 1 - b * T * G) / G;
+            const uint32_t top = min(rw + 16, r1) - 1;
+            const uint32_t first = (G == 1 ? rw : by_group(rw)) - b * T, last = (G == 1 ? top : by_group(top)) - b * T;
             row_keys(a, at + first, lo_all, inner_hi);
             row_keys(a, at + last, inner_lo, hi_all);
         }
@@ -334,10 +339,10 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void atten
         // The prefix in equal parts; the own keys in runs of a.run tiles, the last part all that is left, so a workgroup's work
         // does not grow with its sequence.
         const uint32_t first = pick(own, p0, o0), last = pick(own, p1, o1), n = last - first;
-        const uint32_t t0 = own ? min(last, first + mine * a.run) : first + static_cast<uint32_t>(static_cast<uint64_t>(n) * mine / parts);
+        const uint32_t t0 = own ? min(last, first + mine * a.run) : first + n * mine / parts;  // below 2^25 tiles, 128 parts
         const uint32_t t1 = mine == parts - 1 ? last
                             : own             ? min(last, t0 + a.run)
-                                              : first + static_cast<uint32_t>(static_cast<uint64_t>(n) * (mine + 1) / parts);
+                                              : first + n * (mine + 1) / parts;
         p0 = own ? 0 : t0;
         p1 = own ? 0 : t1;
         o0 = own ? t0 : 0;
@@ -348,7 +353,7 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void atten
         if (nt == 0) {  // all waves alike (they share their rows): no key for any row
             if (tid < 16 && hi > 0) {
                 const uint32_t S = a.sp + a.so;
-                const size_t at = (static_cast<size_t>(row) * a.hq + kvh * G + r % G) * S + (own ? a.sp + mine : mine);
+                const size_t at = (static_cast<size_t>(row) * a.hq + head) * S + (own ? a.sp + mine : mine);
                 reinterpret_cast<float2 *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * S * 64)[at] = make_float2(INFINITY, 0.0f);
             }
             return;
@@ -537,10 +542,12 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void atten
     for (uint32_t j = tid; j < span * 16; j += 64 * WAVES) {
         const uint32_t rr = j / 16, d4 = 4 * (j & 15), rj = r0 + rr;  // row rr of the workgroup
         if (rj >= r1) continue;
-        const uint32_t rowj = rj / G, head = kvh * G + rj % G;
-        uint32_t rb;
-        uint64_t slot;
-        if (!a.rows.at(rowj, rb, slot)) continue;
+        const uint32_t rowj = G == 1 ? rj : by_group(rj), headj = kvh * G + rj - rowj * G;
+        if (!own) {
+            uint32_t rb;
+            uint64_t slot;
+            if (!a.rows.at(rowj, rb, slot)) continue;
+        }
         const uint32_t w0 = rr / 16 * a.keys, in = rr & 15;  // the row's waves, its place in each
         float m = INFINITY;
         for (uint32_t w = 0; w < a.keys; w++) m = fminf(m, ms[(w0 + w) * 16 + in]);
@@ -558,7 +565,7 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void atten
         }
         if constexpr (APART) {
             const uint32_t S = a.sp + a.so;
-            const size_t at = (static_cast<size_t>(rowj) * a.hq + head) * S + (own ? a.sp + mine : mine);
+            const size_t at = (static_cast<size_t>(rowj) * a.hq + headj) * S + (own ? a.sp + mine : mine);
             float2 *ml = reinterpret_cast<float2 *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * S * 64);
             *reinterpret_cast<float4 *>(a.part + at * 64 + d4) = acc;
             if (d4 == 0) ml[at] = make_float2(m, l);
@@ -566,7 +573,7 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void atten
             const float f = 1.0f / (l * KD::PS);
             acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
             if (fabsf(acc.x) < INFINITY && fabsf(acc.y) < INFINITY && fabsf(acc.z) < INFINITY && fabsf(acc.w) < INFINITY)
-                *reinterpret_cast<float4 *>(a.out + static_cast<size_t>(rowj) * a.ldo + head * 64 + d4) = acc;
+                *reinterpret_cast<float4 *>(a.out + static_cast<size_t>(rowj) * a.ldo + headj * 64 + d4) = acc;
             else
                 atomicOr(&redo[rr / 32], 1u << (rr % 32));
         }
@@ -576,14 +583,14 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES)) void atten
         __syncthreads();
         for (uint32_t rr = wave; rr < span; rr += WAVES) {
             if (!((redo[rr / 32] >> (rr % 32)) & 1)) continue;
-            const uint32_t rj = r0 + rr, rowj = rj / G, head = kvh * G + rj % G;
+            const uint32_t rj = r0 + rr, rowj = G == 1 ? rj : by_group(rj), headj = kvh * G + rj - rowj * G;
             uint32_t rb;
             uint64_t slot;
             uint32_t l, e;
             a.rows.at(rowj, rb, slot);
             row_keys(a, slot, l, e);
-            attend_wave<CT>(a.q + static_cast<size_t>(rowj) * a.ldq + head * 64, h, l, e, a.scale,
-                            a.out + static_cast<size_t>(rowj) * a.ldo + head * 64);
+            attend_wave<CT>(a.q + static_cast<size_t>(rowj) * a.ldq + headj * 64, h, l, e, a.scale,
+                            a.out + static_cast<size_t>(rowj) * a.ldo + headj * 64);
         }
     }
 }
@@ -648,7 +655,7 @@ __global__ __launch_bounds__(64 * AJ_WAVES) void attention_join_kernel(SharedArg
     }
     uint32_t lo, hi;
     row_keys(a, slot, lo, hi);
-    attend_wave<CT>(a.q + static_cast<size_t>(row) * a.ldq + head * 64, head_kv<CT>(a, b, head / (a.hq / a.hkv)), lo, hi, a.scale, out);
+    attend_wave<CT>(a.q + static_cast<size_t>(row) * a.ldq + head * 64, head_kv<CT>(a, b, head / a.group), lo, hi, a.scale, out);
 }
 
 template <int CT>
@@ -712,6 +719,8 @@ int launch_attention_shared(const SharedArgs &a, const SharedPlan &p, int ct, hi
     b.sp = p.sp;
     b.so = p.so;
     b.run = p.run;
+    b.group = a.hq / a.hkv;
+    b.group_magic = static_cast<uint32_t>((1ull << 32) / b.group + 1);
     if (ct == DT_F32) return launch_kind<DT_F32>(b, p.apart, stream);
     if (ct == DT_F16) return launch_kind<DT_F16>(b, p.apart, stream);
     return launch_kind<DT_F8>(b, p.apart, stream);

@@ -111,6 +111,8 @@ struct SharedArgs {
     float *part;    // apart: [B T, hq, sp + so] sums of 64 and behind them as many pairs (minus the maximum, the weights' sum)
     uint32_t sp, so, run;
     uint32_t keys;  // waves that split the keys
+    uint32_t group, group_magic;  // hq / hkv, and 2^32 / group + 1: v / group is the high word of their product while
+                                  // v group stays below 2^32 (rows times hq times group: validated)
 };
 
 }  // namespace mt

@@ -38,7 +38,7 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
 }
 
 template <class TL, bool GATED>
-__global__ __launch_bounds__(64 * TL::WAVES * TL::KG) void gemm_kernel(F8LinearArgs a, int bt, uint32_t tiles_m, uint32_t tiles_n) {
+__global__ __launch_bounds__(64 * TL::WAVES * TL::KG, 2) void gemm_kernel(F8LinearArgs a, int bt, uint32_t tiles_m, uint32_t tiles_n) {
     constexpr int MB = TL::MB, NB = TL::NB, BM = TL::BM, BN = TL::BN, W = TL::WAVES, KG = TL::KG;
     constexpr uint32_t FEAT = GATED ? BN / 2 : BN;  // features of a tile
     constexpr uint32_t OUT = 0xF0000000u;           // past every buffer: the load gives zeros
