@@ -327,10 +327,12 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void at
             h = max(h, static_cast<uint32_t>(__shfl_xor(static_cast<int>(h), d, 64)));
             il = max(il, static_cast<uint32_t>(__shfl_xor(static_cast<int>(il), d, 64)));
         }
-        lo_all = __builtin_amdgcn_readfirstlane(l);
-        hi_all = __builtin_amdgcn_readfirstlane(h);
-        inner_lo = __builtin_amdgcn_readfirstlane(il);
+        lo_all = l;
+        hi_all = h;
+        inner_lo = il;
     }
+    auto scalar = [](uint32_t &v) { v = __builtin_amdgcn_readfirstlane(v); };
+    scalar(lo_all), scalar(hi_all), scalar(inner_lo), scalar(inner_hi);
     // Their tiles of TK keys, first those of the prefix, then the own ones: this workgroup's part of them, every keys-th.
     const uint32_t pend = pre ? min(hi_all, P) : 0, oend = own && hi_all > P ? hi_all - P : 0;
     uint32_t p0 = min(lo_all, pend) / TK, p1 = (pend + TK - 1) / TK;
@@ -348,6 +350,7 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void at
         o0 = own ? t0 : 0;
         o1 = own ? t1 : 0;
     }
+    scalar(p0), scalar(p1), scalar(o0), scalar(o1);
     const uint32_t np = p1 - p0, nt = np + (o1 - o0);
     if constexpr (APART) {
         if (nt == 0) {  // all waves alike (they share their rows): no key for any row
@@ -367,25 +370,30 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void at
         s0 = TK * pick(seg, p0 + t, o0 + t - np);
         end = pick(seg, pend, oend);
     };
+    // Loads of a tile past the last one are issued too, of no bytes: with as many loads in flight on every path, the waits for
+    // the values leave the next keys on their way.  (A branch around them made each a wait for all: 26.3 us against 25.0
+    // for the eight prompts, 23.5 against 21.4 for 128 sequences of up to 4096 keys; a copy of the step without loads for
+    // the last tile: 25.4 and 23.2.)
     auto keys = [&](uint32_t t) {
         bool seg;
         uint32_t s0, end;
         tile(t, seg, s0, end);
         load_keys<CT>(raw, pick(seg, h.pk, h.ok) + static_cast<size_t>(s0) * ROW, CT == DT_F8 ? pick(seg, h.pks, h.oks) + s0 : nullptr,
-                      min(end - s0, TK), l16, g);
+                      t < nt ? min(end - s0, TK) : 0, l16, g);
     };
     auto values = [&](uint32_t t) {
         bool seg;
         uint32_t s0, end;
         tile(t, seg, s0, end);
         load_values<CT>(raw, pick(seg, h.pv, h.ov) + static_cast<size_t>(s0) * ROW, CT == DT_F8 ? pick(seg, h.pvs, h.ovs) + s0 : nullptr,
-                        min(end - s0, TK), l16, g);
+                        t < nt ? min(end - s0, TK) : 0, l16, g);
     };
     uint32_t t = wk;
-    if (t < nt) {
-        keys(t);
-        values(t);
-    }
+    __builtin_amdgcn_sched_barrier(0);  // in this order, as in the loop, or its first wait is for all of them
+    keys(t);
+    __builtin_amdgcn_sched_barrier(0);
+    values(t);
+    __builtin_amdgcn_sched_barrier(0);
 
     // The query as the operand's pieces, scaled so that the scores are base-2 exponents (fp16 pieces: times c).
     u32x4v qf[2][KD::NQ];
@@ -450,7 +458,7 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void at
                 s[u] = dot<CT>(kf, qf[kk], s[u]);
             }
         }
-        if (next < nt) keys(next);
+        keys(next);
 
         if (k0 < inner_lo || k0 + TK > min(inner_hi, stop)) {
             // keys of the segment up to its end that lie in [lo, hi)
@@ -523,7 +531,7 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void at
 #pragma unroll
             for (int e = 0; e < 4; e++) o[d][e] = fmaf(o[d][e], al, ot[e]);
         }
-        if (next < nt) values(next);
+        values(next);
     }
 
     // The waves' parts of each row meet in wave order: a thread joins four dims of a row.
