@@ -4,9 +4,10 @@
 //
 // Reference kernel replaced: ropeCache (Shaders.swift:451-486), for rows of many sequences.
 //
-//   - Angles: position times frequency is exact in 64 bits; its turns are taken off there and the
-//     rest, at most half a turn, goes to the fp32 sine and cosine, so a far position costs no bits
-//     (an fp32 product is off by 2^-24 of the angle: 0.008 radians at position 131072).
+//   - Angles: position times frequency is exact in 64 bits, and its turns are taken off there, so a far position
+//     costs no bits (an fp32 product is off by 2^-24 of the angle: 0.008 radians at position 131072).  Sine,
+//     cosine and rotation stay in 64 bits up to the one rounding into q or the cache: an 8-bit code that an
+//     fp32 rotation's error tips over is off by a whole step of 2^-3 (about one in a million values).
 //   - Eight lanes a head: lane r holds dims 4 r .. + 3 and 32 + 4 r .. + 3, both halves of its four
 //     pairs.  The block's largest value is three DPP steps, the codes two words a lane.
 //   - Bound: launch latency for a decode step's rows, the bytes of qkv for prompts.
@@ -22,12 +23,21 @@ constexpr uint32_t KV_OCTETS = KV_THREADS / 8;
 constexpr uint32_t KV_ROWS = 4;  // most rows of a workgroup
 
 // cos and sin of the angle pos * freq.
-__device__ __forceinline__ float2 turn(uint64_t pos, float freq) {
+__device__ __forceinline__ double2 turn(uint64_t pos, float freq) {
     double t = static_cast<double>(pos) * static_cast<double>(freq) * 0.15915494309189535;
     t -= rint(t);
-    float s, c;
-    sincospif(static_cast<float>(2.0 * t), &s, &c);
-    return make_float2(c, s);
+    double s, c;
+    sincospi(2.0 * t, &s, &c);
+    return make_double2(c, s);
+}
+
+// d as fp32, towards zero and with the last bit set where that loses anything: a rounding of the result to fewer bits is the
+// rounding of d.
+__device__ __forceinline__ float to_odd(double d) {
+    const float f = static_cast<float>(d);
+    uint32_t u = __float_as_uint(f);
+    if (static_cast<double>(f) != d) u = (u - (fabs(static_cast<double>(f)) > fabs(d) ? 1u : 0u)) | 1u;
+    return __uint_as_float(u);
 }
 
 // Eight values x (dims d0 .. + 3 and d1 .. + 3 of a 64-wide row) into a cache row of type CT; every
@@ -62,7 +72,7 @@ __global__ __launch_bounds__(KV_THREADS) void rope_append_kernel(const float *qk
                                                                  uint32_t hkv, uint32_t offset, KvArgs kv,
                                                                  const float *inv_freq, float *q, uint32_t ldo,
                                                                  uint32_t per_group) {
-    __shared__ float2 cs[KV_ROWS][32];
+    __shared__ double2 cs[KV_ROWS][32];
     const uint32_t tid = threadIdx.x, r = tid & 7, all = rows.B * rows.T;
     const uint32_t row0 = blockIdx.x * per_group, n = min(per_group, all - row0);
     if (tid < n * 32) {
@@ -86,8 +96,12 @@ __global__ __launch_bounds__(KV_THREADS) void rope_append_kernel(const float *qk
         if (h < hq + hkv) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float2 t = cs[m][4 * r + e];
-                rope_rotate(x[e], x[4 + e], t.x, t.y, x[e], x[4 + e]);
+                const double2 t = cs[m][4 * r + e];
+                const double a = x[e], b2 = x[4 + e];
+                const double lo2 = fma(-b2, t.y, a * t.x), hi2 = fma(a, t.y, b2 * t.x);
+                // (a NaN among the odd ones stays one; infinities are exact)
+                x[e] = CT == DT_F8 && !is_q ? to_odd(lo2) : static_cast<float>(lo2);
+                x[4 + e] = CT == DT_F8 && !is_q ? to_odd(hi2) : static_cast<float>(hi2);
             }
         }
         if (is_q) {

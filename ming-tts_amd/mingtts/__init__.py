@@ -12,6 +12,7 @@ torch device tensors (plumbing for memory and streams only).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 from typing import Optional, Sequence
@@ -502,7 +503,7 @@ def rope_append(qkv, B, T, hq, hkv, pos, kv, inv_freq, q=None, counts=None, offs
     """mt_rope_append: B x T rows of qkv rotated at offset + pos[b] + t, their keys and values appended to ``kv`` at
     slot pos[b] + t (pos None: 0), the rotated queries written to q.  counts (int32 [B]): a sequence's rows of T."""
     _check_kv(kv, B, hkv)
-    check(load().mt_rope_append(_ptr(qkv), qkv.stride(0) if ldq is None else ldq, B, T, hq, hkv, _ptr(pos), _ptr(counts),
+    check((_lib or load()).mt_rope_append(_ptr(qkv), qkv.stride(0) if ldq is None else ldq, B, T, hq, hkv, _ptr(pos), _ptr(counts),
                                 offset, kv.ref, _ptr(inv_freq), _ptr(q),
                                 ldo if ldo is not None else 0 if q is None else q.stride(0), _stream(stream)))
 
@@ -511,7 +512,13 @@ def kv_copy(src, dst, B, T, pos=None, counts=None, stream=None) -> None:
     """mt_kv_copy: slots pos[b] .. pos[b] + counts[b] - 1 of ``src`` to the same slots of ``dst``, converted."""
     _check_kv(src, B, dst.hkv)
     _check_kv(dst, B, src.hkv)
-    check(load().mt_kv_copy(src.ref, dst.ref, B, T, src.hkv, _ptr(pos), _ptr(counts), _stream(stream)))
+    check((_lib or load()).mt_kv_copy(src.ref, dst.ref, B, T, src.hkv, _ptr(pos), _ptr(counts), _stream(stream)))
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_need(*sizes) -> int:
+    """mt_attention_shared_workspace: the sizes alone decide."""
+    return load().mt_attention_shared_workspace(*sizes)
 
 
 def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=None, len_max=0, window=0, counts=None,
@@ -526,12 +533,11 @@ def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=Non
         _check_kv(prefix, 1, hkv)
         if prefix_len is None:
             prefix_len = prefix.cache_len
-    L = load()
     s = _stream(stream)
-    need = L.mt_attention_shared_workspace(B, T, hq, hkv, prefix_len, len_max if len_max else kv.cache_len, window, kv.type)
+    need = _shared_need(B, T, hq, hkv, prefix_len, len_max or kv.cache_len, window, kv.type)
     if need and workspace is None:
         workspace = _scratch(need, q, stream)
-    check(L.mt_attention_shared(_ptr(q), q.stride(0) if ldq is None else ldq, B, T, hq, hkv, _ptr(pos), _ptr(counts), kv.ref,
+    check(_lib.mt_attention_shared(_ptr(q), q.stride(0) if ldq is None else ldq, B, T, hq, hkv, _ptr(pos), _ptr(counts), kv.ref,
                                 prefix.ref if prefix is not None else None, prefix_len, len_max, window, _ptr(out),
                                 out.stride(0) if ldo is None else ldo, scale, _ptr(workspace),
                                 workspace.numel() if workspace is not None else 0, s))
@@ -556,7 +562,9 @@ class F8Matrix:
         n, k = codes.shape
         if tuple(scales.shape) != (n, 4 * ((k + 511) // 512)) or scales.element_size() != 1 or scales.stride(1) != 1:
             raise ValueError("scales: [rows, 4 ceil(K / 512)] bytes")
-        self.codes, self.scales, self.shape = codes, scales, codes.shape
+        self.codes, self.scales, self.shape = codes, scales, (n, k)
+        self.whole = codes.is_contiguous() and scales.is_contiguous()  # as weights have to be
+        self.args = (_ptr(codes), codes.stride(0), _ptr(scales), scales.stride(0))
 
     @staticmethod
     def quantize(x, norm=None, eps=1e-6, stream=None):
@@ -586,11 +594,11 @@ def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6,
     mt_quantize_f8 first."""
     N, K = w.shape
     M = x.shape[0] if M is None else M
-    if x.shape[1] != K or x.shape[0] < M or (w2 is not None and tuple(w2.shape) != (N, K)):
+    rows, k = x.shape
+    if k != K or rows < M or (w2 is not None and w2.shape != w.shape):
         raise ValueError("x, w and w2 must agree in K, w and w2 in shape")
-    for m in (w, w2):
-        if m is not None and not (m.codes.is_contiguous() and m.scales.is_contiguous()):
-            raise ValueError("weights must be contiguous")
+    if not w.whole or (w2 is not None and not w2.whole):
+        raise ValueError("weights must be contiguous")
     if not isinstance(x, F8Matrix) and (M > LINEAR_F8_ROWS or (norm is not None and K > LINEAR_F8_NORM_K)):
         x, norm = F8Matrix.quantize(x[:M], norm=norm, eps=eps, stream=stream), None
     b = bias if bias is not None else norm
@@ -598,13 +606,14 @@ def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6,
     if bias is not None and norm is not None and dtype_code(norm) != bt:
         raise ValueError("bias and norm must be of one type")
     if isinstance(x, F8Matrix):
-        xp, xt, xs, ldx, ldxs = x.codes, F8, x.scales, x.codes.stride(0), x.scales.stride(0)
+        xp, ldx, xs, ldxs = x.args
+        xt = F8
     else:
-        xp, xt, xs, ldx, ldxs = x, dtype_code(x), None, x.stride(0), 0
+        xp, xt, xs, ldx, ldxs = x.data_ptr(), dtype_code(x), None, x.stride(0), 0
+    wp, _, ws, _ = w.args
+    up, _, us, _ = w2.args if w2 is not None else (None, 0, None, 0)
     p = GemvParams(M, N, K, ldx, y.stride(0) if ldy is None else ldy, flags, eps)
-    check(load().mt_linear_f8(_ptr(xp), xt, _ptr(xs), ldxs, _ptr(norm), _ptr(w.codes), _ptr(w.scales),
-                              _ptr(w2.codes) if w2 is not None else None, _ptr(w2.scales) if w2 is not None else None,
-                              _ptr(bias), bt, _ptr(y), p, _stream(stream)))
+    check((_lib or load()).mt_linear_f8(xp, xt, xs, ldxs, _ptr(norm), wp, ws, up, us, _ptr(bias), bt, _ptr(y), p, _stream(stream)))
 
 
 def dit_attention(qkv, B, S, H, inv_freq, out, ld=None, ldo=None, scale=0.125, stream=None) -> None:
