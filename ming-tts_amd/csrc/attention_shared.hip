@@ -151,21 +151,21 @@ __device__ __forceinline__ void split8(const float *x, u32x4v *p) {
     }
 }
 
-// acc + c . q over the pieces' products that are not below 2^-24, the small ones first.
+// The products of pieces that are not below 2^-24, the small ones first: of piece C of k (or v) and piece Q of q (or the
+// weights).
 template <int CT>
-__device__ __forceinline__ f32x4v dot(const u32x4v *c, const u32x4v *q, f32x4v acc) {
-    constexpr bool H = Kind<CT>::HALF;
-    if constexpr (CT == DT_F32) {
-        acc = mma<H>(c[2], q[0], acc);
-        acc = mma<H>(c[0], q[2], acc);
-        acc = mma<H>(c[1], q[1], acc);
-        acc = mma<H>(c[1], q[0], acc);
-        acc = mma<H>(c[0], q[1], acc);
-    } else {
+struct Products {
+    static constexpr int N = CT == DT_F32 ? 6 : Kind<CT>::NQ;
+    static constexpr int C[6] = {CT == DT_F32 ? 2 : 0, 0, CT == DT_F32 ? 1 : 0, 1, 0, 0};
+    static constexpr int Q[6] = {CT == DT_F32 ? 0 : Kind<CT>::NQ - 1, CT == DT_F32 ? 2 : Kind<CT>::NQ - 2, CT == DT_F32 ? 1 : 0, 0, 1, 0};
+};
+// acc[i] + c[i] . q for N sums at once: an MFMA waits for the one before it on the same sum, so the sums take turns.
+template <int CT, int N>
+__device__ __forceinline__ void dots(const u32x4v (*c)[Kind<CT>::NC], const u32x4v *q, f32x4v *acc) {
 #pragma unroll
-        for (int i = Kind<CT>::NQ - 1; i > 0; i--) acc = mma<H>(c[0], q[i], acc);
-    }
-    return mma<H>(c[0], q[0], acc);
+    for (int p = 0; p < Products<CT>::N; p++)
+#pragma unroll
+        for (int i = 0; i < N; i++) acc[i] = mma<Kind<CT>::HALF>(c[i][Products<CT>::C[p]], q[Products<CT>::Q[p]], acc[i]);
 }
 
 // The maximum over the four lanes 16 apart.
@@ -434,17 +434,18 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void at
         const uint32_t k0 = s0 + (seg ? P : 0), stop = end + (seg ? P : 0);
         f32x4v s[2 * SUB];
 #pragma unroll
-        for (int u = 0; u < 2 * SUB; u++) {
-            s[u] = f32x4v{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < 2 * SUB; u++) s[u] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
-                u32x4v kf[KD::NC];
+        for (int kk = 0; kk < 2; kk++) {
+            u32x4v kf[2 * SUB][KD::NC];
+#pragma unroll
+            for (int u = 0; u < 2 * SUB; u++) {
                 if constexpr (CT == DT_F8) {
                     const float f = f8_pow2(raw.ks[u]);
                     const uint32_t w0 = raw.k[u][2 * kk], w1 = raw.k[u][2 * kk + 1];
-                    kf[0] = u32x4v{f8_bf16x2<false>(w0, f), f8_bf16x2<true>(w0, f), f8_bf16x2<false>(w1, f), f8_bf16x2<true>(w1, f)};
+                    kf[u][0] = u32x4v{f8_bf16x2<false>(w0, f), f8_bf16x2<true>(w0, f), f8_bf16x2<false>(w1, f), f8_bf16x2<true>(w1, f)};
                 } else if constexpr (CT == DT_F16) {
-                    kf[0] = raw.k[2 * u + kk];
+                    kf[u][0] = raw.k[2 * u + kk];
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
@@ -452,11 +453,11 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void at
                         uint32_t p[3];
                         split2<CT>(__uint_as_float(w[2 * (e & 1)]), __uint_as_float(w[2 * (e & 1) + 1]), p);
 #pragma unroll
-                        for (int i = 0; i < 3; i++) kf[i][e] = p[i];
+                        for (int i = 0; i < 3; i++) kf[u][i][e] = p[i];
                     }
                 }
-                s[u] = dot<CT>(kf, qf[kk], s[u]);
             }
+            dots<CT, 2 * SUB>(kf, qf[kk], s);
         }
         keys(next);
 
@@ -504,33 +505,36 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void at
         ls = fmaf(ls, al, sum);
 
         // p . v: a tile's sum starts from zero and joins the running one in one rounding.
+        f32x4v ot[4];
 #pragma unroll
-        for (int d = 0; d < 4; d++) {
-            f32x4v ot = {0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < 4; d++) ot[d] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < SUB; i++) {
-                u32x4v vf[KD::NC];
+        for (int i = 0; i < SUB; i++) {
+            u32x4v vf[4][KD::NC];
+#pragma unroll
+            for (int d = 0; d < 4; d++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int j = 8 * i + 2 * e;
                     if constexpr (CT == DT_F8) {
                         const uint32_t w = __builtin_amdgcn_perm(raw.v[j + 1], raw.v[j], d < 2 ? 0x05010400u : 0x07030602u);
-                        vf[0][e] = d & 1 ? f8_bf16x2<true>(w, 1.0f) : f8_bf16x2<false>(w, 1.0f);
+                        vf[d][0][e] = d & 1 ? f8_bf16x2<true>(w, 1.0f) : f8_bf16x2<false>(w, 1.0f);
                     } else if constexpr (CT == DT_F16) {
-                        vf[0][e] = __builtin_amdgcn_perm(raw.v[2 * (j + 1) + (d >> 1)], raw.v[2 * j + (d >> 1)],
-                                                         d & 1 ? 0x07060302u : 0x05040100u);
+                        vf[d][0][e] = __builtin_amdgcn_perm(raw.v[2 * (j + 1) + (d >> 1)], raw.v[2 * j + (d >> 1)],
+                                                            d & 1 ? 0x07060302u : 0x05040100u);
                     } else {
                         uint32_t w[3];
                         split2<CT>(__uint_as_float(raw.v[4 * j + d]), __uint_as_float(raw.v[4 * (j + 1) + d]), w);
 #pragma unroll
-                        for (int q = 0; q < 3; q++) vf[q][e] = w[q];
+                        for (int q = 0; q < 3; q++) vf[d][q][e] = w[q];
                     }
                 }
-                ot = dot<CT>(vf, pf[i], ot);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[d][e] = fmaf(o[d][e], al, ot[e]);
+            dots<CT, 4>(vf, pf[i], ot);
         }
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[d][e] = fmaf(o[d][e], al, ot[d][e]);
         values(next);
     }
 
