@@ -176,8 +176,7 @@ __device__ __forceinline__ float rows_max(float v) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-constexpr int AS_WAVES = 8;       // of a workgroup
-constexpr int AS_PART_WAVES = 4;  // of one that has a part of the keys (apart)
+constexpr uint32_t AS_WAVES = 8, AS_FEW = 4;  // waves of a workgroup: all on one row tile's keys, or one of several
 constexpr uint32_t AS_LD = 68;  // floats of a row in the waves' hand-over (64 and a 16-byte skew)
 
 // One wave's 16 rows and TK = 32 SUB keys at a time: the raw keys and values of a tile.  Lane (l16, g) holds dims
@@ -244,9 +243,8 @@ __device__ __forceinline__ V pick(bool second, V first, V other) {
     return second ? other : first;
 }
 
-template <int CT, bool APART>
-__global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void attention_shared_kernel(SharedArgs a) {
-    constexpr int WAVES = APART ? AS_PART_WAVES : AS_WAVES;
+template <int CT, bool APART, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void attention_shared_kernel(SharedArgs a) {
     typedef Kind<CT> KD;
     constexpr int SUB = Raw<CT>::SUB;
     constexpr uint32_t ROW = Cached<CT>::ROW, TK = Raw<CT>::TK;
@@ -280,7 +278,7 @@ __global__ __launch_bounds__(64 * (APART ? AS_PART_WAVES : AS_WAVES), 2) void at
     if (own) {
         b = x / seq_tiles;
         const uint32_t n = a.rows.counts ? min(a.rows.counts[b], T) : T;
-        r0 = b * T * G + (x % seq_tiles) * span;
+        r0 = b * T * G + (seq_tiles - 1 - x % seq_tiles) * span;  // the longest rows first
         r1 = min(b * T * G + n * G, r0 + span);
         if (r0 >= r1) return;
     } else {
@@ -671,15 +669,17 @@ __global__ __launch_bounds__(64 * AJ_WAVES) void attention_join_kernel(SharedArg
 }
 
 template <int CT>
-int launch_kind(const SharedArgs &a, bool apart, hipStream_t stream) {
-    const uint32_t G = a.hq / a.hkv, span = (apart ? AS_PART_WAVES : AS_WAVES) / a.keys * 16, B = a.rows.B, T = a.rows.T;
-    const uint64_t own = static_cast<uint64_t>(B) * a.hkv * ((T * G + span - 1) / span);
-    if (!apart) {
-        hipLaunchKernelGGL((attention_shared_kernel<CT, false>), dim3(static_cast<uint32_t>(own)), dim3(64 * AS_WAVES), 0, stream, a);
+int launch_kind(const SharedArgs &a, const SharedPlan &p, hipStream_t stream) {
+    const uint32_t span = p.waves / a.keys * 16, B = a.rows.B, T = a.rows.T;
+    const uint64_t own = static_cast<uint64_t>(B) * a.hkv * ((T * a.group + span - 1) / span);
+    const dim3 grid(static_cast<uint32_t>(own)), block(64 * p.waves);
+    if (!p.apart) {
+        if (p.waves == AS_WAVES) hipLaunchKernelGGL((attention_shared_kernel<CT, false, AS_WAVES>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((attention_shared_kernel<CT, false, AS_FEW>), grid, block, 0, stream, a);
         return check_launch("attention shared");
     }
-    const uint64_t pre = static_cast<uint64_t>(a.sp) * a.hkv * ((static_cast<uint64_t>(B) * T * G + span - 1) / span);
-    hipLaunchKernelGGL((attention_shared_kernel<CT, true>), dim3(static_cast<uint32_t>(pre + own * a.so)), dim3(64 * AS_PART_WAVES), 0, stream, a);
+    const uint64_t pre = static_cast<uint64_t>(a.sp) * a.hkv * ((static_cast<uint64_t>(B) * T * a.group + span - 1) / span);
+    hipLaunchKernelGGL((attention_shared_kernel<CT, true, AS_FEW>), dim3(static_cast<uint32_t>(pre + own * a.so)), block, 0, stream, a);
     int rc = check_launch("attention shared (parts)");
     if (rc) return rc;
     const uint32_t waves = std::min(AJ_WAVES, (a.sp + a.so + 1) / 2);
@@ -689,28 +689,34 @@ int launch_kind(const SharedArgs &a, bool apart, hipStream_t stream) {
 
 }  // namespace
 
-// Where the work goes.  A CU holds one workgroup at a time (164 registers a lane), which takes about 2 us for each
-// 512 keys of its rows, and the second kernel of the split form costs about as much as 1200 keys.
-//   - keys: the waves of a workgroup share 16 rows and split the keys, unless that makes more workgroups than
-//     CUs and other rows can take the waves instead.  Measured, us for keys 8 / 4 / 2 / 1: 8 sequences of 130 rows over 1000
-//     + 256 keys (912 row tiles) 29.3 / 28.9 / 26.0 / 45.5, 1 of 300 rows (264) 11.7 / 9.7 / 12.2 / 17.1, 4 of 40 rows
-//     over 500 + 300 (144) 9.3 / 13.2 / 19.4 / 32.0.
+// Where the work goes.  A CU holds one workgroup of eight waves or three of four (168 registers a lane); eight waves
+// take about 2 us for each 512 keys of their rows, and the second kernel of the split form costs about as much as
+// 1200 keys.
+//   - One row tile (16 rows) a workgroup of eight waves that split its keys, while that fills at most every CU once: 4
+//     sequences of 40 rows over 500 + 300 keys (144 workgroups) 8.8 us, with two tiles a workgroup 13.2, four 19.4.
+//   - More row tiles: four waves a tile, and two or four tiles a workgroup only where that would leave a wave less
+//     than four steps.  Eight prompts of 130 rows over 1000 + 256 keys (912 tiles) 21.1 us, two tiles a workgroup 24.4,
+//     eight waves 25.3; 1 of 2048 rows 37.7, 50.1; but 8 of 512 rows (1 to 8 steps) 28.3, four tiles a workgroup 25.1.
+//     The longest rows go first (2048 rows 37.7 -> 35.4).
 //   - apart: all keys of the prefix (once for all rows) and of the sequences spread over the CUs evenly, if the
 //     longest workgroup then costs less than the longest in one pass.  Measured, one pass against apart: 64 sequences
-//     of up to 4096 keys 21.0 against 17.8 us, 128 of them 23.0 against 27.8, 16 sequences over 8192 + 512 keys
-//     36.5 against 10.1, 128 over 2048 + 512 15.7 against 16.6, 256 over 4096 + 1024 47.2 against 38.8.
+//     of up to 4096 keys 21.0 against 16.2 us, 128 of them 20.8 against 26, 16 sequences over 8192 + 512 keys
+//     36.5 against 11.5, 128 over 2048 + 512 14.9 against 14.7, 256 over 4096 + 1024 47 against 29.3.
 SharedPlan shared_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t prefix_len, uint32_t len_max, uint32_t window,
                        int ct) {
     const uint64_t tk = ct == DT_F32 ? Raw<DT_F32>::TK : Raw<DT_F8>::TK, cus = 256;
-    SharedPlan p{AS_WAVES, false, 0, 0, 0};
+    SharedPlan p{AS_WAVES, AS_WAVES, false, 0, 0, 0};
     // keys a row attends at most
     const uint64_t own = std::max<uint64_t>(1, window ? std::min<uint64_t>(len_max, static_cast<uint64_t>(window) + T - 1) : len_max);
     const uint64_t pre = window ? std::min(prefix_len, window) : prefix_len;
     const uint64_t rows = static_cast<uint64_t>(T) * (hq / hkv), heads = static_cast<uint64_t>(B) * hkv;
-    auto groups = [&](uint64_t keys) { return heads * ((rows + AS_WAVES / keys * 16 - 1) / (AS_WAVES / keys * 16)); };
-    while (p.keys > 1 && groups(p.keys) > cus && groups(p.keys / 2) < groups(p.keys)) p.keys /= 2;
-    if (p.keys != AS_WAVES) return p;
-    const uint64_t own_groups = groups(AS_WAVES), pre_groups = pre ? hkv * ((B * rows + 15) / 16) : 0;
+    auto groups = [&](uint64_t waves, uint64_t keys) { return heads * ((rows + waves / keys * 16 - 1) / (waves / keys * 16)); };
+    if (rows > 16 && groups(AS_WAVES, AS_WAVES) > cus) {
+        p.waves = p.keys = AS_FEW;
+        while (p.keys > 1 && groups(AS_FEW, p.keys) > 4 * cus && pre + own < 4 * tk * p.keys) p.keys /= 2;
+        return p;
+    }
+    const uint64_t own_groups = groups(AS_WAVES, AS_WAVES), pre_groups = pre ? hkv * ((B * rows + 15) / 16) : 0;
     const uint64_t share = (pre_groups * pre + own_groups * own) / (2 * cus), part = std::max<uint64_t>(share, 256);  // keys a workgroup, two a CU
     // At most 128 parts each, or the second kernel becomes the longer one.
     const uint64_t sp = pre ? std::min<uint64_t>(std::max<uint64_t>(1, pre / part), 128) : 0;
@@ -718,6 +724,7 @@ SharedPlan shared_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
     const uint64_t longest = std::max({share, pre ? pre / sp : 0, own / so});
     if (2 * longest + 1200 < (own_groups + cus - 1) / cus * (pre + own)) {
         p.apart = true;
+        p.waves = p.keys = AS_FEW;
         p.sp = static_cast<uint32_t>(sp);
         p.so = static_cast<uint32_t>(so);
         p.run = static_cast<uint32_t>((own + so * tk - 1) / (so * tk));
@@ -727,15 +734,15 @@ SharedPlan shared_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
 
 int launch_attention_shared(const SharedArgs &a, const SharedPlan &p, int ct, hipStream_t stream) {
     SharedArgs b = a;
-    b.keys = p.apart ? AS_PART_WAVES : p.keys;
+    b.keys = p.keys;
     b.sp = p.sp;
     b.so = p.so;
     b.run = p.run;
     b.group = a.hq / a.hkv;
     b.group_magic = static_cast<uint32_t>((1ull << 32) / b.group + 1);
-    if (ct == DT_F32) return launch_kind<DT_F32>(b, p.apart, stream);
-    if (ct == DT_F16) return launch_kind<DT_F16>(b, p.apart, stream);
-    return launch_kind<DT_F8>(b, p.apart, stream);
+    if (ct == DT_F32) return launch_kind<DT_F32>(b, p, stream);
+    if (ct == DT_F16) return launch_kind<DT_F16>(b, p, stream);
+    return launch_kind<DT_F8>(b, p, stream);
 }
 
 }  // namespace mt

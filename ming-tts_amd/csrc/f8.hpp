@@ -93,6 +93,7 @@ struct RowsArgs {
 
 // How mt_attention_shared places its work (shared_plan).
 struct SharedPlan {
+    uint32_t waves;     // of a workgroup
     uint32_t keys;      // waves of a workgroup that share rows and split their keys (the rest: other rows)
     bool apart;         // prefix and own keys in workgroups of their own, joined by a second kernel
     uint32_t sp, so;    // parts of the prefix's and of the own keys then
