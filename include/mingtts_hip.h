@@ -428,7 +428,7 @@ int mt_attention_decode(const float *q, uint32_t ldq, uint32_t B, uint32_t hq, u
  * (device, B uint32; NULL: zeros) gives each sequence's first row's slot in its own caches, so row t
  * stands at slot pos[b] + t; counts (device, B uint32; NULL: T each) how many of its T rows a
  * sequence brings.  Rows past that are padding: nothing is read, written or computed for them.
- * B T (hq + 2 hkv) must stay below 2^31.
+ * B T (hq + 2 hkv) must stay below 2^31, and in mt_attention_shared B T (hq / hkv)^2 below 2^32.
  */
 typedef struct mt_kv {
     void *k;
@@ -474,8 +474,8 @@ int mt_kv_copy(const mt_kv *src, const mt_kv *dst, uint32_t B, uint32_t T, uint3
  * aligned with 16-byte row strides and do not overlap.  Both caches are of one type.  Cache slots
  * that a row does not attend do not reach its result, whatever they hold.
  *
- * len_max is the caller's bound on the own keys, max(pos[b] + counts[b]) (0: cache_len).  It only
- * places the work (longer sequences give the same results, more slowly).  The keys are split over
+ * len_max is the caller's bound on the own keys, max(pos[b] + counts[b]) (0: cache_len, which is also what
+ * to ask the workspace for then).  It only places the work (longer sequences give the same results, more slowly).  The keys are split over
  * workgroups where rows are few and keys are many; their parts meet in `workspace`, 16-byte aligned device memory
  * of at least mt_attention_shared_workspace(the same sizes) bytes (0: none needed, NULL is fine), which
  * holds nothing between calls.  Calls that may overlap, captured graphs among them, need a workspace each.

@@ -186,6 +186,8 @@ int mt_quantize_f8(const void *x, mt_dtype xt, uint32_t rows, uint32_t K, uint32
     if (norm && K > 16 * F8_NORM_K) return set_error(MT_EINVAL, "%s: a norm over K %u > %u", who, K, 16 * F8_NORM_K);
     if (K == 0 || K % 16) return set_error(MT_EINVAL, "%s: K must be a positive multiple of 16, got %u", who, K);
     if (rows == 0) return MT_OK;
+    if (rows > 0x7FFFFFFFu || static_cast<uint64_t>(rows) * lds > 0x7FFFFFFFull * 16)
+        return set_error(MT_EINVAL, "%s: %u rows of %u blocks are too many", who, rows, lds);
     if (!x || !codes || !scales) return set_error(MT_EINVAL, "%s: null pointer", who);
     if (ldx < K || ldq < K) return set_error(MT_EINVAL, "%s: ldx %u or ldq %u < K %u", who, ldx, ldq, K);
     if (lds < 4 * ((K + 511) / 512) || lds % 4) return set_error(MT_EINVAL, "%s: lds %u must be a multiple of 4 of at least 4 ceil(K / 512)", who, lds);
@@ -212,6 +214,7 @@ int mt_linear_f8(const void *x, mt_dtype xt, const uint8_t *xs, uint32_t ldxs, c
     const bool gated = (flags & MT_SILU_GATE) != 0;
     if (gated && (!w2 || !w2s)) return set_error(MT_EINVAL, "%s: MT_SILU_GATE without w2", who);
     if (p.M == 0 || p.N == 0) return MT_OK;
+    if (p.M > 0x7FFFFFFFu || p.N > 0x7FFFFFFFu / (gated ? 2 : 1)) return set_error(MT_EINVAL, "%s: M %u x N %u is too large", who, p.M, p.N);
     if (!x || !w || !ws || !y) return set_error(MT_EINVAL, "%s: null x, w, ws or y", who);
     if (p.K == 0 || p.K % 16) return set_error(MT_EINVAL, "%s: K must be a positive multiple of 16, got %u", who, p.K);
     if (p.ldx < p.K || p.ldy < p.N) return set_error(MT_EINVAL, "%s: ldx %u < K %u or ldy %u < N %u", who, p.ldx, p.K, p.ldy, p.N);

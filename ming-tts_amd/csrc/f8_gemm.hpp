@@ -128,12 +128,14 @@ __global__ __launch_bounds__(64 * TL::WAVES * TL::KG, 2) void gemm_kernel(F8Line
         return __builtin_bit_cast(bf16x8v, u32x4v{f8_bf16x2<false>(w[2 * s], f), f8_bf16x2<true>(w[2 * s], f),
                                                   f8_bf16x2<false>(w[2 * s + 1], f), f8_bf16x2<true>(w[2 * s + 1], f)});
     };
-    auto compute = [&](const uint8_t *at, int c) {
+    // (block past the last one: codes of zeros, whose scale bytes may be anything)
+    auto compute = [&](const uint8_t *at, int c, uint32_t block) {
+        const uint32_t byte = block < blocks ? 255u : 0u;
         float fa[MB], fb[NB];
 #pragma unroll
-        for (int i = 0; i < MB; i++) fa[i] = f8_pow2((as[i] >> (8 * (c * KG + kg))) & 255u);
+        for (int i = 0; i < MB; i++) fa[i] = f8_pow2((as[i] >> (8 * (c * KG + kg))) & byte);
 #pragma unroll
-        for (int j = 0; j < NB; j++) fb[j] = f8_pow2((bs[j] >> (8 * (c * KG + kg))) & 255u);
+        for (int j = 0; j < NB; j++) fb[j] = f8_pow2((bs[j] >> (8 * (c * KG + kg))) & byte);
         Raw f[2];
         read(f[0], at, 0);
 #pragma unroll
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(64 * TL::WAVES * TL::KG, 2) void gemm_kernel(F8Line
             asm volatile("" ::: "memory");
             stage(i0 + c + P - 1, buffer == 0 ? P - 1 : buffer - 1);
             if (c == 0) scales(min((i0 + SC) * KG, (blocks - 1) & ~3u));
-            compute(lds + (buffer * KG + kg) * TL::STAGE, c);
+            compute(lds + (buffer * KG + kg) * TL::STAGE, c, (i0 + c) * KG + kg);
             buffer = buffer == P - 1 ? 0 : buffer + 1;
         }
     }

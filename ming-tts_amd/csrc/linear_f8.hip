@@ -284,7 +284,7 @@ int few_rows(const F8LinearArgs &a, int bt, hipStream_t stream) {
     const bool gated = (a.flags & F_SILU_GATE) != 0;
     const uint32_t codes = XT == DT_F8 ? 0 : waves * FEW_WAVE, sums = waves * 1024 * (gated ? 2 : 1);
     const uint32_t bytes = std::max(codes + (a.norm ? a.M * blocks * 4 : 0), sums);
-    const dim3 grid((a.N + 15) / 16, (a.M + 15) / 16), block(64 * waves);
+    const dim3 grid((a.N - 1) / 16 + 1, (a.M - 1) / 16 + 1), block(64 * waves);
     if (gated) hipLaunchKernelGGL((few_rows_kernel<XT, true>), grid, block, bytes, stream, a, bt);
     else hipLaunchKernelGGL((few_rows_kernel<XT, false>), grid, block, bytes, stream, a, bt);
     return check_launch("linear (8-bit, few rows)");
@@ -323,7 +323,7 @@ int launch_linear_f8(const F8LinearArgs &a, int xt, int bt, hipStream_t stream) 
     // (2912 waves of 256 CUs) 7.6 against 11.0, 64 of 1152 x 896 (2016) 4.5 against 5.0, 96 of 896 x 4864 (4368) 12.7 against
     // 11.0, 174 of 1152 x 896 (5544) 6.4 against 5.1, 64 of 2 x 4864 x 896 (8512) 10.2 against 6.5.
     const int cus = device_cus();
-    const uint64_t tiles = static_cast<uint64_t>((a.N + 15) / 16) * ((a.M + 15) / 16);
+    const uint64_t tiles = static_cast<uint64_t>((a.N - 1) / 16 + 1) * ((a.M - 1) / 16 + 1);
     if (tuning().f8_tile.load(std::memory_order_relaxed) == 0 && a.M <= 16 * 65535u &&
         tiles * few_waves(a.K) <= 16ull * (cus > 0 ? cus : 256))
         return few_rows<DT_F8>(a, bt, stream);

@@ -479,6 +479,7 @@ class KV:
         self.hkv, self.cache_len, self.type = k.shape[-3], k.shape[-2], t
         self.batch = k.shape[0] if k.dim() == 4 else 1
         batched = k.dim() == 4
+        self.device = k.get_device()
         self.struct = KvStruct(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), k.stride(0) if batched else 0,
                                k_scale.stride(0) if batched and t == F8 else 0, self.cache_len, t)
         self.ref = ctypes.byref(self.struct)
@@ -499,20 +500,39 @@ def _check_kv(kv, B, hkv):
         raise ValueError(f"caches of {kv.batch} sequences and {kv.hkv} heads for {B} and {hkv}")
 
 
+def _check_words(device, *tensors):
+    """Tensors of 4-byte elements (fp32, or int32 for pos and counts), all on one device."""
+    for t in tensors:
+        if t is not None and (t.element_size() != 4 or t.get_device() != device):
+            raise ValueError("activations are fp32, pos and counts int32, all on the caches' or weights' device")
+
+
+def _on(device, stream):
+    """The stream's handle; the kernels run on the current device, so it has to be the tensors'."""
+    s = _stream(stream)
+    if _current_device is not None and _current_device() != device:
+        raise ValueError("the tensors are not on the current device")
+    return s
+
+
 def rope_append(qkv, B, T, hq, hkv, pos, kv, inv_freq, q=None, counts=None, offset=0, ldq=None, ldo=None, stream=None) -> None:
     """mt_rope_append: B x T rows of qkv rotated at offset + pos[b] + t, their keys and values appended to ``kv`` at
     slot pos[b] + t (pos None: 0), the rotated queries written to q.  counts (int32 [B]): a sequence's rows of T."""
     _check_kv(kv, B, hkv)
+    _check_words(kv.device, qkv, pos, counts, inv_freq, q)
     check((_lib or load()).mt_rope_append(_ptr(qkv), qkv.stride(0) if ldq is None else ldq, B, T, hq, hkv, _ptr(pos), _ptr(counts),
                                 offset, kv.ref, _ptr(inv_freq), _ptr(q),
-                                ldo if ldo is not None else 0 if q is None else q.stride(0), _stream(stream)))
+                                ldo if ldo is not None else 0 if q is None else q.stride(0), _on(kv.device, stream)))
 
 
 def kv_copy(src, dst, B, T, pos=None, counts=None, stream=None) -> None:
     """mt_kv_copy: slots pos[b] .. pos[b] + counts[b] - 1 of ``src`` to the same slots of ``dst``, converted."""
     _check_kv(src, B, dst.hkv)
     _check_kv(dst, B, src.hkv)
-    check((_lib or load()).mt_kv_copy(src.ref, dst.ref, B, T, src.hkv, _ptr(pos), _ptr(counts), _stream(stream)))
+    _check_words(src.device, pos, counts)
+    if dst.device != src.device:
+        raise ValueError("src and dst are on different devices")
+    check((_lib or load()).mt_kv_copy(src.ref, dst.ref, B, T, src.hkv, _ptr(pos), _ptr(counts), _on(src.device, stream)))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -533,7 +553,10 @@ def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=Non
         _check_kv(prefix, 1, hkv)
         if prefix_len is None:
             prefix_len = prefix.cache_len
-    s = _stream(stream)
+        if prefix.device != kv.device:
+            raise ValueError("prefix and kv are on different devices")
+    _check_words(kv.device, q, out, pos, counts)
+    s = _on(kv.device, stream)
     need = _shared_need(B, T, hq, hkv, prefix_len, len_max or kv.cache_len, window, kv.type)
     if need and workspace is None:
         workspace = _scratch(need, q, stream)
@@ -564,6 +587,7 @@ class F8Matrix:
             raise ValueError("scales: [rows, 4 ceil(K / 512)] bytes")
         self.codes, self.scales, self.shape = codes, scales, (n, k)
         self.whole = codes.is_contiguous() and scales.is_contiguous()  # as weights have to be
+        self.device = codes.get_device()
         self.args = (_ptr(codes), codes.stride(0), _ptr(scales), scales.stride(0))
 
     @staticmethod
@@ -580,9 +604,11 @@ def quantize_f8(x, out, norm=None, eps=1e-6, stream=None) -> None:
     """mt_quantize_f8: the rows of x [rows, K], RMS-normalised with gain ``norm`` if given, into an F8Matrix."""
     if tuple(x.shape) != tuple(out.shape) or x.stride(1) != 1:
         raise ValueError("x and the matrix must be of one shape, x's rows contiguous")
+    if x.get_device() != out.device:
+        raise ValueError("x and the matrix are on different devices")
     check(load().mt_quantize_f8(_ptr(x), dtype_code(x), x.shape[0], x.shape[1], x.stride(0), _ptr(norm),
                                 dtype_code(norm) if norm is not None else F16, eps, _ptr(out.codes), out.codes.stride(0),
-                                _ptr(out.scales), out.scales.stride(0), _stream(stream)))
+                                _ptr(out.scales), out.scales.stride(0), _on(out.device, stream)))
 
 
 LINEAR_F8_ROWS, LINEAR_F8_NORM_K = 16, 32768  # most rows mt_linear_f8 quantises itself, most values a row it normalises
@@ -599,6 +625,9 @@ def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6,
         raise ValueError("x, w and w2 must agree in K, w and w2 in shape")
     if not w.whole or (w2 is not None and not w2.whole):
         raise ValueError("weights must be contiguous")
+    _check_words(w.device, y)
+    if (x.device if isinstance(x, F8Matrix) else x.get_device()) != w.device:
+        raise ValueError("x and w are on different devices")
     if not isinstance(x, F8Matrix) and (M > LINEAR_F8_ROWS or (norm is not None and K > LINEAR_F8_NORM_K)):
         x, norm = F8Matrix.quantize(x[:M], norm=norm, eps=eps, stream=stream), None
     b = bias if bias is not None else norm
@@ -613,7 +642,7 @@ def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6,
     wp, _, ws, _ = w.args
     up, _, us, _ = w2.args if w2 is not None else (None, 0, None, 0)
     p = GemvParams(M, N, K, ldx, y.stride(0) if ldy is None else ldy, flags, eps)
-    check((_lib or load()).mt_linear_f8(xp, xt, xs, ldxs, _ptr(norm), wp, ws, up, us, _ptr(bias), bt, _ptr(y), p, _stream(stream)))
+    check((_lib or load()).mt_linear_f8(xp, xt, xs, ldxs, _ptr(norm), wp, ws, up, us, _ptr(bias), bt, _ptr(y), p, _on(w.device, stream)))
 
 
 def dit_attention(qkv, B, S, H, inv_freq, out, ld=None, ldo=None, scale=0.125, stream=None) -> None:

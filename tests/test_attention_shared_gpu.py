@@ -298,3 +298,17 @@ def test_graph_replays_and_streams(gpu, shape):
     call(b, poss[1], streams[1])
     torch.cuda.synchronize()
     assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
+@pytest.mark.parametrize("byte", [0, 255])
+@pytest.mark.parametrize("P,window", [(0, 0), (70, 0), (6001, 0)])
+def test_stale_scale_bytes(gpu, byte, P, window):
+    """Scale bytes of slots that no row attends, behind a sequence's end and the prefix's, are not values: any byte may
+    stand there, in one pass and in parts."""
+    c = Case(gpu, "f8", 2, 2, 14, 2, 64, P, pos=[20, 45], counts=[2, 1])
+    want = c.run(window=window)
+    for _, scales, _ in c.own:
+        scales[0, :, 22:], scales[1, :, 46:] = byte, byte
+    for _, scales, _ in c.pre or ():
+        scales[:, P:] = byte
+    assert np.array_equal(c.run(window=window), want)

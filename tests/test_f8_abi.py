@@ -90,6 +90,8 @@ def attend(kv, prefix=None, q=1024 * MB, ldq=896, B=4, T=1, hq=14, hkv=2, prefix
     (dict(), dict(t=mt.F16), dict(prefix_len=3), "one type"),
     (dict(), dict(), dict(prefix_len=65), "past the prefix"),
     (dict(t=mt.BF16), None, {}, "f32, f16 or f8"),
+    (dict(), None, dict(hq=8194), "too many"),
+    (dict(), None, dict(B=1 << 20, T=100, hq=16, hkv=1, ldq=1024), "too many"),
 ])
 def test_attention_refuses(kv, prefix, call, needle):
     p = kv_struct(base=3072 * MB, **prefix) if prefix is not None else None
@@ -130,6 +132,8 @@ def quant(x=A, xt=mt.F32, rows=4, K=256, ldx=256, norm=None, nt=mt.F16, eps=1e-6
     (dict(norm=A, K=1 << 20, ldx=1 << 20, ldq=1 << 20, lds=1 << 13), "a norm over K"),
     (dict(codes=A), "overlap"),
     (dict(scales=1024 * MB + 16), "overlap"),
+    (dict(rows=1 << 31), "too many"),
+    (dict(rows=1 << 30, lds=64), "too many"),
 ])
 def test_quantize_refuses(call, needle):
     assert quant(**call) == mt.EINVAL
@@ -166,6 +170,10 @@ def lin(x=A, xt=mt.F8, xs=512 * MB, ldxs=4, norm=None, w=1024 * MB, ws=1536 * MB
     (dict(xt=mt.F32, norm=A, eps=-1.0), mt.EINVAL, "eps"),
     (dict(x=2048 * MB), mt.EINVAL, "x overlaps y"),
     (dict(xs=2048 * MB), mt.EINVAL, "xs overlaps y"),
+    (dict(M=1 << 31), mt.EINVAL, "too large"),
+    (dict(N=1 << 31, ldy=1 << 31), mt.EINVAL, "too large"),
+    (dict(K=1 << 23, ldx=1 << 23), mt.EINVAL, "past 2^22"),
+    (dict(ldx=1 << 23), mt.EINVAL, "past 2^22"),
 ])
 def test_linear_refuses(call, code, needle):
     assert lin(**call) == code
@@ -219,6 +227,15 @@ def test_python_classes_check():
         mt.linear_f8(z(2, 64), w, z(2, 4))
     with pytest.raises(ValueError):
         mt.linear_f8(z(2, 48), w, z(2, 4), M=3)
+    with pytest.raises(ValueError, match="fp32"):
+        mt.linear_f8(z(2, 48), w, z(2, 4, dtype=torch.float16))
+    q, o, pos = z(2, 896), z(2, 896), z(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="int32"):
+        mt.attention_shared(q, 2, 1, 14, 2, pos, kv, o)
+    with pytest.raises(ValueError, match="fp32"):
+        mt.attention_shared(q.half(), 2, 1, 14, 2, pos.int(), kv, o)
+    with pytest.raises(ValueError, match="int32"):
+        mt.rope_append(z(2, 1152), 2, 1, 14, 2, pos, kv, z(32))
 
 
 def test_the_oracle_of_the_format():

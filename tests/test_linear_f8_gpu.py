@@ -201,6 +201,22 @@ def test_scales_far_apart_and_nan_rows(gpu, M):
 
 
 @pytest.mark.parametrize("M", [2, 100])
+@pytest.mark.parametrize("K", [144, 640, 1040])
+def test_padding_scale_bytes_are_not_read(gpu, tile, M, K):
+    """The bytes behind a row's last block, up to the next multiple of four, may be anything."""
+    rng = np.random.default_rng(4)
+    w, _ = matrix(rng.standard_normal((70, K)) * 0.05, gpu)
+    x = mt.F8Matrix.quantize(torch.from_numpy(rng.standard_normal((M, K)).astype(np.float32)).to(gpu))
+    a, b = torch.zeros(M, 70, device=gpu), torch.zeros(M, 70, device=gpu)
+    mt.linear_f8(x, w, a)
+    n = (K + 127) // 128
+    for m in (x, w):
+        m.scales[:, n:] = 255
+    mt.linear_f8(x, w, b)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("M", [2, 100])
 def test_graph_and_streams(gpu, M):
     """Replays see new inputs; two streams at once give the bits of one after the other."""
     rng = np.random.default_rng(6)
