@@ -94,7 +94,7 @@ struct RowsArgs {
 // How mt_attention_shared places its work (shared_plan).
 struct SharedPlan {
     uint32_t waves;     // of a workgroup
-    uint32_t keys;      // waves of a workgroup that share rows and split their keys (the rest: other rows)
+    uint32_t keys;      // waves of a workgroup that share rows and split their keys (the rest: other rows): all, 2 or 1
     bool apart;         // prefix and own keys in workgroups of their own, joined by a second kernel
     uint32_t sp, so;    // parts of the prefix's and of the own keys then
     uint32_t run;       // tiles of own keys a part
