@@ -261,9 +261,19 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(F8LinearArgs a, int bt) 
         const uint32_t row = m0 + i / 16, nn = n0 + (i & 15);
         if (nn >= a.N) continue;
         float s = 0.0f, s2 = 0.0f;
-        for (uint32_t w = 0; w < waves; w++) {
-            s += part[w * PW + i];
-            if constexpr (GATED) s2 += part[w * PW + 256 + i];
+        for (uint32_t w0 = 0; w0 < waves; w0 += 4) {  // four waves' sums read at once
+            float v[4], v2[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t w = min(w0 + j, waves - 1);
+                v[j] = part[w * PW + i];
+                if constexpr (GATED) v2[j] = part[w * PW + 256 + i];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                s += w0 + j < waves ? v[j] : 0.0f;
+                if constexpr (GATED) s2 += w0 + j < waves ? v2[j] : 0.0f;
+            }
         }
         const float b = !(a.flags & F_BIAS) ? 0.0f : bt == DT_BF16 ? dec1<DT_BF16>(a.bias[nn]) : dec1<DT_F16>(a.bias[nn]);
         float *y = a.y + static_cast<size_t>(row) * a.ldy + nn;
