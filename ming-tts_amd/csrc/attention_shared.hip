@@ -1,5 +1,32 @@
 // Attention of B sequences, T query rows each, over keys that all of them share and then over their
-// own (mt_attention_shared), for caches of fp32, fp16 and 8 bits.
+// own (mt_attention_shared), for caches of fp32, fp16 and 8 bits (f8.hpp).
+//
+// out = sum_j p_j v_j / sum_j p_j with p_j = 2^(s_j - max s), s_j = log2(e) scale q . k_j, over the keys of the row: one pass
+// with a running maximum, on the matrix cores.
+//
+//   - Rows: the query heads of a key head's group are rows of their own, (sequence, t, head of the group) in order, 16 to
+//     an MFMA tile, so a decode step's 7 heads read a key once and so do the rows of many sequences over the prefix.
+//   - Scores: S^T = K Q^T with v_mfma_f32_16x16x32.  Lane (l16, g) reads dims 16 g .. + 15 of key l16 (one 16-byte load of an
+//     8-bit row: 16 keys an instruction, whole rows); the dims' order is free as long as q follows it.  The accumulator gives
+//     the lane keys 4 g .. + 3 of its own row l16, so the softmax is in-lane but for one exchange of the maximum a step.
+//   - p . v: O^T = V^T P^T.  The weights stay where the scores stood; a lane reads dims 4 l16 .. + 3 of those keys' values and
+//     byte permutes put two keys side by side.
+//   - 8 bits: a key's codes become bf16 with its scale in the conversion (exact); a value's scale goes into its
+//     weight, whose pieces are then the weight times a power of two.  bf16 has the range for any scale.
+//   - Precision: q and the weights as three bf16 pieces (24 bits) against 8-bit and fp32 caches, those in three pieces too,
+//     the 6 products above 2^-24; two fp16 pieces (22 bits) against fp16 caches.  All sums in fp32; a step's p . v starts from
+//     zero and joins the running sum in one rounding.  Normwise error against fp64 1e-7 to 4e-7 up to 131072 keys (the plain fp32
+//     form: 2e-7 to 2e-6).
+//   - A step is 64 keys (32 of fp32), eight or four waves a workgroup take every keys-th one and meet in LDS in wave order.  The next
+//     step's keys are requested behind the scores, its values behind p . v, through buffer descriptors that end with the keys:
+//     what stands behind them is never read.  Keys inside that are not a row's (causal, window) weigh exactly zero;
+//     where such a key or value is not finite, a row's outputs are not either, and it is done again from its own keys alone.
+//   - Few rows over many keys, or a prefix for many sequences: parts of the keys go to workgroups of their own and a second
+//     kernel joins them (shared_plan).  Sums meet in a fixed order everywhere: the same call gives the same bits.
+//   - Bound: instructions.  A step of 64 8-bit keys is about 380 vector instructions and 48 MFMAs a wave whether 7 or 16 rows
+//     are used (waves busy 60 %, waiting for memory 35 %), so long caches run at 2.2-3.2 TB/s where a large copy reaches
+//     4.9; 128 sequences of up to 4096 keys (68 MB) take 20.4 us, 64 of them 15.6, one of 131072 15.6, the guided pair's step over
+//     512 keys 6.1 (graph replay; an empty launch is 1.7), 1 prompt of 300 rows 6.8, of 2048 rows 34.
 #include <algorithm>
 #include <type_traits>
 

@@ -10,7 +10,8 @@
 //     fp32 rotation's error tips over is off by a whole step of 2^-3 (about one in a million values).
 //   - Eight lanes a head: lane r holds dims 4 r .. + 3 and 32 + 4 r .. + 3, both halves of its four
 //     pairs.  The block's largest value is three DPP steps, the codes two words a lane.
-//   - Bound: launch latency for a decode step's rows, the bytes of qkv for prompts.
+//   - Bound: launch latency for a decode step's rows (1.9 us for two), the bytes of qkv and q for prompts (16 sequences of
+//     up to 330 rows, 33 MB: 8-10 us, and 2.2-4 for their copy to fp16).
 #include "f8.hpp"
 #include "mt_internal.hpp"
 

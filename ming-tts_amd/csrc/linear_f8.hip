@@ -1,5 +1,10 @@
 // Matrices in 8 bits (f8.hpp: a block is 128 consecutive values of a row): the quantiser
-// (mt_quantize_f8) and the linears over such weights (mt_linear_f8).
+// (mt_quantize_f8) and the linears over such weights (mt_linear_f8): few rows here, more in f8_gemm.hpp.
+//
+// Quantiser: 4096 x 4096 fp32 in 17.5 us (84 MB, 4.8 TB/s: a large copy's rate), 512 x 896 in 2.
+// Few rows: gate|up (2 x 4864 x 896) of two fp32 rows 5.6 us, 4.9 of rows that come quantised (8.7 MB; 1.7 us at a large
+// copy's rate and 1.7 for an empty launch); down (896 x 4864) of 16 fp32 rows 9.1 us, 7.4 quantised: 56 workgroups that each
+// quantise all of x.  Bound: latency at two rows, the quantising at sixteen.
 #include <algorithm>
 
 #include "f8_linear.hpp"
