@@ -495,22 +495,26 @@ class KV:
         return KV(k, torch.zeros_like(k), s, torch.ones_like(s))
 
 
-def _check_kv(kv, B, hkv):
-    if kv.hkv != hkv or kv.batch < B:
-        raise ValueError(f"caches of {kv.batch} sequences and {kv.hkv} heads for {B} and {hkv}")
+def _refuse_kv(kv, B, hkv):
+    raise ValueError(f"caches of {kv.batch} sequences and {kv.hkv} heads for {B} and {hkv}")
 
 
-def _check_words(device, *tensors):
-    """Tensors of 4-byte elements (fp32, or int32 for pos and counts), all on one device."""
-    for t in tensors:
-        if t is not None and (t.element_size() != 4 or t.get_device() != device):
-            raise ValueError("activations are fp32, pos and counts int32, all on the caches' or weights' device")
+def _words(device, t):
+    """The address of a tensor of 4-byte elements (fp32, or int32 for pos and counts) on the given device."""
+    if t.element_size() != 4 or t.get_device() != device:
+        raise ValueError("activations are fp32, pos and counts int32, all on the caches' or weights' device")
+    return t.data_ptr()
 
 
 def _on(device, stream):
     """The stream's handle; the kernels run on the current device, so it has to be the tensors'."""
-    s = _stream(stream)
-    if _current_device is not None and _current_device() != device:
+    if stream is None and _raw_stream is not None:
+        current = _current_device()
+        s = _raw_stream(current)
+    else:
+        s = _stream(stream)
+        current = device if _current_device is None else _current_device()
+    if current != device:
         raise ValueError("the tensors are not on the current device")
     return s
 
@@ -518,21 +522,28 @@ def _on(device, stream):
 def rope_append(qkv, B, T, hq, hkv, pos, kv, inv_freq, q=None, counts=None, offset=0, ldq=None, ldo=None, stream=None) -> None:
     """mt_rope_append: B x T rows of qkv rotated at offset + pos[b] + t, their keys and values appended to ``kv`` at
     slot pos[b] + t (pos None: 0), the rotated queries written to q.  counts (int32 [B]): a sequence's rows of T."""
-    _check_kv(kv, B, hkv)
-    _check_words(kv.device, qkv, pos, counts, inv_freq, q)
-    check((_lib or load()).mt_rope_append(_ptr(qkv), qkv.stride(0) if ldq is None else ldq, B, T, hq, hkv, _ptr(pos), _ptr(counts),
-                                offset, kv.ref, _ptr(inv_freq), _ptr(q),
-                                ldo if ldo is not None else 0 if q is None else q.stride(0), _on(kv.device, stream)))
+    if kv.hkv != hkv or kv.batch < B:
+        _refuse_kv(kv, B, hkv)
+    d = kv.device
+    rc = (_lib or load()).mt_rope_append(
+        _words(d, qkv), qkv.stride(0) if ldq is None else ldq, B, T, hq, hkv, None if pos is None else _words(d, pos),
+        None if counts is None else _words(d, counts), offset, kv.ref, _words(d, inv_freq), None if q is None else _words(d, q),
+        ldo if ldo is not None else 0 if q is None else q.stride(0), _on(d, stream))
+    if rc < 0:
+        check(rc)
 
 
 def kv_copy(src, dst, B, T, pos=None, counts=None, stream=None) -> None:
     """mt_kv_copy: slots pos[b] .. pos[b] + counts[b] - 1 of ``src`` to the same slots of ``dst``, converted."""
-    _check_kv(src, B, dst.hkv)
-    _check_kv(dst, B, src.hkv)
-    _check_words(src.device, pos, counts)
-    if dst.device != src.device:
+    if src.hkv != dst.hkv or src.batch < B or dst.batch < B:
+        _refuse_kv(src if src.batch < B else dst, B, src.hkv)
+    d = src.device
+    if dst.device != d:
         raise ValueError("src and dst are on different devices")
-    check((_lib or load()).mt_kv_copy(src.ref, dst.ref, B, T, src.hkv, _ptr(pos), _ptr(counts), _on(src.device, stream)))
+    rc = (_lib or load()).mt_kv_copy(src.ref, dst.ref, B, T, src.hkv, None if pos is None else _words(d, pos),
+                                     None if counts is None else _words(d, counts), _on(d, stream))
+    if rc < 0:
+        check(rc)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -546,33 +557,39 @@ def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=Non
     """mt_attention_shared: the rows' attention over ``prefix`` (one sequence's KV, its first prefix_len slots; all
     by default) and then their own keys in ``kv`` up to their slot.  The workspace, where the split of the keys
     needs one, comes from torch's allocator (so a captured graph keeps its own) unless given as a uint8 tensor."""
-    _check_kv(kv, B, hkv)
+    if kv.hkv != hkv or kv.batch < B:
+        _refuse_kv(kv, B, hkv)
+    d = kv.device
     if prefix is None:
-        prefix_len = 0
+        prefix_len, pre = 0, None
     else:
-        _check_kv(prefix, 1, hkv)
+        if prefix.hkv != hkv:
+            _refuse_kv(prefix, 1, hkv)
+        if prefix.device != d:
+            raise ValueError("prefix and kv are on different devices")
         if prefix_len is None:
             prefix_len = prefix.cache_len
-        if prefix.device != kv.device:
-            raise ValueError("prefix and kv are on different devices")
-    _check_words(kv.device, q, out, pos, counts)
-    s = _on(kv.device, stream)
+        pre = prefix.ref
     need = _shared_need(B, T, hq, hkv, prefix_len, len_max or kv.cache_len, window, kv.type)
     if need and workspace is None:
         workspace = _scratch(need, q, stream)
-    check(_lib.mt_attention_shared(_ptr(q), q.stride(0) if ldq is None else ldq, B, T, hq, hkv, _ptr(pos), _ptr(counts), kv.ref,
-                                prefix.ref if prefix is not None else None, prefix_len, len_max, window, _ptr(out),
-                                out.stride(0) if ldo is None else ldo, scale, _ptr(workspace),
-                                workspace.numel() if workspace is not None else 0, s))
+    rc = (_lib or load()).mt_attention_shared(
+        _words(d, q), q.stride(0) if ldq is None else ldq, B, T, hq, hkv, None if pos is None else _words(d, pos),
+        None if counts is None else _words(d, counts), kv.ref, pre, prefix_len, len_max, window, _words(d, out),
+        out.stride(0) if ldo is None else ldo, scale, None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _on(d, stream))
+    if rc < 0:
+        check(rc)
 
 
 def _scratch(nbytes, like, stream):
-    """Device memory for one call on ``stream``, from torch's allocator."""
+    """Device memory for one call on ``stream``, from that stream's pool of torch's allocator: what is freed there is
+    used again in the stream's order only."""
     import torch
-    t = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    if stream is not None:  # the allocator only orders its reuse on the current stream
-        t.record_stream(stream if not isinstance(stream, int) else torch.cuda.ExternalStream(stream))
-    return t
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
 
 
 class F8Matrix:
@@ -625,24 +642,29 @@ def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6,
         raise ValueError("x, w and w2 must agree in K, w and w2 in shape")
     if not w.whole or (w2 is not None and not w2.whole):
         raise ValueError("weights must be contiguous")
-    _check_words(w.device, y)
-    if (x.device if isinstance(x, F8Matrix) else x.get_device()) != w.device:
-        raise ValueError("x and w are on different devices")
     if not isinstance(x, F8Matrix) and (M > LINEAR_F8_ROWS or (norm is not None and K > LINEAR_F8_NORM_K)):
         x, norm = F8Matrix.quantize(x[:M], norm=norm, eps=eps, stream=stream), None
     b = bias if bias is not None else norm
     bt = dtype_code(b) if b is not None else F16
     if bias is not None and norm is not None and dtype_code(norm) != bt:
         raise ValueError("bias and norm must be of one type")
+    d = w.device
     if isinstance(x, F8Matrix):
         xp, ldx, xs, ldxs = x.args
-        xt = F8
+        xt, on = F8, x.device
     else:
-        xp, xt, xs, ldx, ldxs = x.data_ptr(), dtype_code(x), None, x.stride(0), 0
+        ldx, unit = x.stride()
+        if unit != 1:
+            raise ValueError("x's rows must be contiguous")
+        xp, xt, xs, ldxs, on = x.data_ptr(), dtype_code(x), None, 0, x.get_device()
+    if on != d or (w2 is not None and w2.device != d):
+        raise ValueError("x, w and w2 are on different devices")
     wp, _, ws, _ = w.args
     up, _, us, _ = w2.args if w2 is not None else (None, 0, None, 0)
-    p = GemvParams(M, N, K, ldx, y.stride(0) if ldy is None else ldy, flags, eps)
-    check((_lib or load()).mt_linear_f8(xp, xt, xs, ldxs, _ptr(norm), wp, ws, up, us, _ptr(bias), bt, _ptr(y), p, _on(w.device, stream)))
+    rc = (_lib or load()).mt_linear_f8(xp, xt, xs, ldxs, _ptr(norm), wp, ws, up, us, _ptr(bias), bt, _words(d, y),
+                                       GemvParams(M, N, K, ldx, y.stride(0) if ldy is None else ldy, flags, eps), _on(d, stream))
+    if rc < 0:
+        check(rc)
 
 
 def dit_attention(qkv, B, S, H, inv_freq, out, ld=None, ldo=None, scale=0.125, stream=None) -> None:

@@ -238,6 +238,13 @@ def test_python_classes_check():
         mt.rope_append(z(2, 1152), 2, 1, 14, 2, pos, kv, z(32))
 
 
+def test_python_refuses_strided_rows():
+    w = mt.F8Matrix(torch.zeros(4, 48, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8))
+    for x in (torch.zeros(48, 2).t(), torch.zeros(2, 96)[:, ::2]):
+        with pytest.raises(ValueError, match="contiguous"):
+            mt.linear_f8(x, w, torch.zeros(2, 4))
+
+
 def test_the_oracle_of_the_format():
     """Every code is its own nearest code at scale 1, midpoints go to the even one, blocks take the least scale."""
     x = np.where(np.isnan(U.TABLE), 0, U.TABLE)
