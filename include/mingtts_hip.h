@@ -429,6 +429,7 @@ int mt_attention_decode(const float *q, uint32_t ldq, uint32_t B, uint32_t hq, u
  * stands at slot pos[b] + t; counts (device, B uint32; NULL: T each) how many of its T rows a
  * sequence brings.  Rows past that are padding: nothing is read, written or computed for them.
  * B T (hq + 2 hkv) must stay below 2^31, and in mt_attention_shared B T (hq / hkv)^2 below 2^32.
+ * These and the matrices' sizes are bounded too by the 2^32 threads of a launch (else MT_EINVAL).
  */
 typedef struct mt_kv {
     void *k;

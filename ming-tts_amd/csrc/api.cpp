@@ -42,6 +42,13 @@ int check_launch(const char *what) {
     return MT_OK;
 }
 
+int check_grid(const char *what, uint64_t groups, uint32_t threads) {
+    if (groups * threads > 0xFFFFFFFFull)
+        return set_error(MT_EINVAL, "%s: %llu workgroups of %u threads are too many for one launch", what,
+                         static_cast<unsigned long long>(groups), threads);
+    return MT_OK;
+}
+
 // Checks one linear's arguments; fills `a` (with the bias flag set from the pointer,
 // Kernels.swift:135).  Returns MT_OK or MT_EINVAL with the reason.
 static int validate_linear(const char *who, const void *x, int xt, const void *w, const void *w2, int wt,

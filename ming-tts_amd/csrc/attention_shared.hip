@@ -716,16 +716,22 @@ int launch_kind(const SharedArgs &a, const SharedPlan &p, hipStream_t stream) {
     const uint32_t span = p.waves / a.keys * 16, B = a.rows.B, T = a.rows.T;
     const uint64_t own = static_cast<uint64_t>(B) * a.hkv * ((T * a.group + span - 1) / span);
     const dim3 grid(static_cast<uint32_t>(own)), block(64 * p.waves);
+    int rc;
     if (!p.apart) {
+        rc = check_grid("attention shared", own, block.x);
+        if (rc) return rc;
         if (p.waves == AS_WAVES) hipLaunchKernelGGL((attention_shared_kernel<CT, false, AS_WAVES>), grid, block, 0, stream, a);
         else hipLaunchKernelGGL((attention_shared_kernel<CT, false, AS_FEW>), grid, block, 0, stream, a);
         return check_launch("attention shared");
     }
     const uint64_t pre = static_cast<uint64_t>(a.sp) * a.hkv * ((static_cast<uint64_t>(B) * T * a.group + span - 1) / span);
-    hipLaunchKernelGGL((attention_shared_kernel<CT, true, AS_FEW>), dim3(static_cast<uint32_t>(pre + own * a.so)), block, 0, stream, a);
-    int rc = check_launch("attention shared (parts)");
-    if (rc) return rc;
     const uint32_t waves = std::min(AJ_WAVES, (a.sp + a.so + 1) / 2);
+    rc = check_grid("attention shared (parts)", pre + own * a.so, block.x);
+    if (!rc) rc = check_grid("attention shared (join)", static_cast<uint64_t>(B) * T * a.hq, 64 * waves);
+    if (rc) return rc;
+    hipLaunchKernelGGL((attention_shared_kernel<CT, true, AS_FEW>), dim3(static_cast<uint32_t>(pre + own * a.so)), block, 0, stream, a);
+    rc = check_launch("attention shared (parts)");
+    if (rc) return rc;
     hipLaunchKernelGGL(attention_join_kernel<CT>, dim3(B * T * a.hq), dim3(64 * waves), 0, stream, a);
     return check_launch("attention shared (join)");
 }

@@ -183,6 +183,8 @@ int launch_rope_append(const float *qkv, uint32_t ldq, const RowsArgs &rows, uin
     // One row a workgroup while that leaves CUs free, else the rows that share the angles' set-up.
     const uint32_t per = all <= 512 ? 1 : KV_ROWS;
     const dim3 grid((all + per - 1) / per);
+    const int rc = check_grid("rope append", grid.x, KV_THREADS);
+    if (rc) return rc;
     if (ct == DT_F32)
         hipLaunchKernelGGL(rope_append_kernel<DT_F32>, grid, dim3(KV_THREADS), 0, stream, qkv, ldq, rows, hq, hkv, offset, kv,
                            inv_freq, q, ldo, per);
@@ -198,6 +200,8 @@ int launch_rope_append(const float *qkv, uint32_t ldq, const RowsArgs &rows, uin
 int launch_kv_copy(const KvArgs &src, int st, const KvArgs &dst, int dt, const RowsArgs &rows, uint32_t hkv, hipStream_t stream) {
     const uint64_t octets = static_cast<uint64_t>(rows.B) * rows.T * hkv * 2;
     const dim3 grid(static_cast<uint32_t>((octets + KV_OCTETS - 1) / KV_OCTETS));
+    const int rc = check_grid("kv copy", grid.x, KV_THREADS);
+    if (rc) return rc;
     if (st == DT_F32) copy_from<DT_F32>(src, dst, dt, rows, hkv, grid, stream);
     else if (st == DT_F16) copy_from<DT_F16>(src, dst, dt, rows, hkv, grid, stream);
     else copy_from<DT_F8>(src, dst, dt, rows, hkv, grid, stream);

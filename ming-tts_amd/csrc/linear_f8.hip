@@ -300,6 +300,8 @@ int few_rows(const F8LinearArgs &a, int bt, hipStream_t stream) {
     const uint32_t codes = XT == DT_F8 ? 0 : waves * FEW_WAVE, sums = waves * 1024 * (gated ? 2 : 1);
     const uint32_t bytes = std::max(codes + (a.norm ? a.M * blocks * 4 : 0), sums);
     const dim3 grid((a.N - 1) / 16 + 1, (a.M - 1) / 16 + 1), block(64 * waves);
+    const int rc = check_grid("linear (8-bit, few rows)", grid.x, block.x);
+    if (rc) return rc;
     if (gated) hipLaunchKernelGGL((few_rows_kernel<XT, true>), grid, block, bytes, stream, a, bt);
     else hipLaunchKernelGGL((few_rows_kernel<XT, false>), grid, block, bytes, stream, a, bt);
     return check_launch("linear (8-bit, few rows)");
@@ -309,6 +311,9 @@ int few_rows(const F8LinearArgs &a, int bt, hipStream_t stream) {
 
 int launch_quantize_f8(const void *x, int xt, uint32_t rows, uint32_t K, uint32_t ldx, const uint16_t *norm, int nt, float eps,
                        uint8_t *codes, uint32_t ldq, uint8_t *scales, uint32_t lds, hipStream_t stream) {
+    const uint64_t all = static_cast<uint64_t>(rows) * lds;
+    const int rc = check_grid("quantize", norm ? rows : (all + 15) / 16, 256);
+    if (rc) return rc;
     if (norm) {
         const uint32_t shared = (K + 127) / 128 * 4;
 #define QUANTIZE(XT) \
@@ -319,7 +324,6 @@ int launch_quantize_f8(const void *x, int xt, uint32_t rows, uint32_t K, uint32_
 #undef QUANTIZE
         return check_launch("quantize (norm)");
     }
-    const uint64_t all = static_cast<uint64_t>(rows) * lds;
     const dim3 grid(static_cast<uint32_t>((all + 15) / 16));
 #define QUANTIZE(XT) hipLaunchKernelGGL(quantize_kernel<XT>, grid, dim3(256), 0, stream, x, all, K, ldx, codes, ldq, scales, lds)
     if (xt == DT_F32) QUANTIZE(DT_F32);

@@ -11,7 +11,8 @@ int launch_tile(const F8LinearArgs &a, int bt, hipStream_t stream) {
     static_assert(TL::KG * TL::P * TL::STAGE <= 160 * 1024, "LDS of a CU");
     const uint32_t feat = GATED ? TL::BN / 2 : TL::BN;
     const uint32_t tm = (a.M - 1) / TL::BM + 1, tn = (a.N - 1) / feat + 1;
-    if (static_cast<uint64_t>(tm) * tn > 0x7FFFFFFFull) return set_error(MT_EINVAL, "mt_linear_f8: M %u x N %u is too large", a.M, a.N);
+    const int rc = check_grid("linear (8-bit GEMM)", static_cast<uint64_t>(tm) * tn, 64 * TL::WAVES * TL::KG);
+    if (rc) return rc;
     hipLaunchKernelGGL((f8::gemm_kernel<TL, GATED>), dim3(tm * tn), dim3(64 * TL::WAVES * TL::KG), TL::KG * TL::P * TL::STAGE, stream, a, bt,
                        tm, tn);
     return check_launch("linear (8-bit GEMM)");

@@ -18,6 +18,8 @@ struct FixedWs;  // a fixed split-K scratch (below)
 int set_error(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 // hipGetLastError after a launch, as an ABI return code.
 int check_launch(const char *what);
+// A launch holds fewer than 2^32 threads an axis: refuses more, before any HIP call.
+int check_grid(const char *what, uint64_t groups, uint32_t threads);
 
 // Process-wide tuning (mt_set_tuning).  Every field is read and written atomically
 // (relaxed), so host threads launching on distinct streams may call mt_set_tuning

@@ -262,3 +262,23 @@ def test_the_oracle_of_the_format():
     assert np.isfinite(back).all()
     c, s = U.encode(np.array([[1.0, np.inf, -np.inf, np.nan] + [0.0] * 60]), 64)
     assert s[0, 0] == U.encode(np.array([[1.0] + [0.0] * 63]), 64)[1][0, 0] and list(c[0][1:3]) == [127, 255]
+
+
+def test_sizes_past_a_launch_are_refused():
+    """Sizes whose pointers and strides are sound but whose threads do not fit one launch."""
+    lib, far, big = mt.load(), 1 << 44, 1 << 28
+    kv, long, dst = kv_struct(hkv=1), kv_struct(hkv=1, cache_len=4096), kv_struct(base=256 * MB, hkv=1)
+    calls = [
+        lambda: lib.mt_rope_append(far, 192, 1, big, 1, 1, None, None, 0, ref(kv), A, None, 0, None),
+        lambda: lib.mt_kv_copy(ref(kv), ref(dst), 1, big, 1, None, None, None),
+        lambda: lib.mt_attention_shared(far, 64, 1, big, 1, 1, None, None, ref(long), None, 0, 0, 0, 2 * far, 64, 0.125, None, 0, None),
+        lambda: lib.mt_quantize_f8(far, mt.F16, 1 << 27, 16, 16, None, mt.F16, 1e-6, 2 * far, 16, 3 * far, 4, None),
+        lambda: lib.mt_quantize_f8(far, mt.F16, 1 << 25, 16, 16, A, mt.F16, 1e-6, 2 * far, 16, 3 * far, 4, None),
+        lambda: lib.mt_linear_f8(A, mt.F32, None, 0, None, far, 2 * far, None, None, None, mt.F16, 3 * far,
+                                 mt.GemvParams(1, 1 << 30, 16, 16, 1 << 30, 0, 0.0), None),
+        lambda: lib.mt_linear_f8(far, mt.F8, 2 * far, 4, None, 3 * far, 4 * far, None, None, None, mt.F16, 5 * far,
+                                 mt.GemvParams(1 << 28, 1024, 16, 16, 1024, 0, 0.0), None),
+    ]
+    for c in calls:
+        assert c() == mt.EINVAL
+        assert "too many" in mt.last_error(), mt.last_error()
