@@ -94,7 +94,7 @@ def attend(kv, prefix=None, q=1024 * MB, ldq=896, B=4, T=1, hq=14, hkv=2, prefix
     (dict(), None, dict(B=1 << 20, T=100, hq=16, hkv=1, ldq=1024), "too many"),
 ])
 def test_attention_refuses(kv, prefix, call, needle):
-    p = kv_struct(base=3072 * MB, **prefix) if prefix is not None else None
+    p = kv_struct(base=2816 * MB, **prefix) if prefix is not None else None
     assert attend(kv_struct(**kv), p, **call) == mt.EINVAL
     assert needle in mt.last_error(), mt.last_error()
 
