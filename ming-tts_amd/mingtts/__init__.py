@@ -588,7 +588,9 @@ def _scratch(nbytes, like, stream):
     import torch
     if stream is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream):
+    if isinstance(stream, int):  # (torch takes a zero handle for a stream of its own pool)
+        stream = torch.cuda.ExternalStream(stream, device=like.device) if stream else torch.cuda.default_stream(like.device)
+    with torch.cuda.stream(stream):
         return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
 
 

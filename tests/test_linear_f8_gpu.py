@@ -245,3 +245,18 @@ def test_graph_and_streams(gpu, M):
     torch.cuda.synchronize()
     for a, b in zip(ys, want):
         assert torch.equal(a, b)
+
+
+def test_scratch_belongs_to_the_calls_stream(gpu):
+    """Memory that a call takes comes from its own stream's pool (the null stream's for handle 0), so that what is freed
+    is used again in that stream's order."""
+    x = torch.randn(4, 4096, device=gpu)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream, owner in ((None, 0), (0, 0), (side, side.cuda_stream), (side.cuda_stream, side.cuda_stream)):
+        m = mt.F8Matrix.quantize(x, stream=stream)
+        at = m.codes.data_ptr()
+        segments = [g for g in torch.cuda.memory_snapshot() if g["address"] <= at < g["address"] + g["total_size"]]
+        assert len(segments) == 1 and segments[0]["stream"] == owner
+        torch.cuda.synchronize()
+        assert torch.equal(m.codes, mt.F8Matrix.quantize(x).codes)
