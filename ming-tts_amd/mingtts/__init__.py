@@ -475,6 +475,8 @@ class KV:
             raise ValueError("caches hold heads of 64 fp32, fp16 or 8-bit values")
         if t == F8 and (k_scale.shape != k.shape[:-1] or k_scale.element_size() != 1):
             raise ValueError("one scale byte a head and position")
+        if any(x is not None and x.device != k.device for x in (v, k_scale, v_scale)):
+            raise ValueError("caches and scales must be on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.hkv, self.cache_len, self.type = k.shape[-3], k.shape[-2], t
         self.batch = k.shape[0] if k.dim() == 4 else 1
@@ -604,6 +606,8 @@ class F8Matrix:
         n, k = codes.shape
         if tuple(scales.shape) != (n, 4 * ((k + 511) // 512)) or scales.element_size() != 1 or scales.stride(1) != 1:
             raise ValueError("scales: [rows, 4 ceil(K / 512)] bytes")
+        if scales.device != codes.device:
+            raise ValueError("codes and scales must be on one device")
         self.codes, self.scales, self.shape = codes, scales, (n, k)
         self.whole = codes.is_contiguous() and scales.is_contiguous()  # as weights have to be
         self.device = codes.get_device()
@@ -623,8 +627,10 @@ def quantize_f8(x, out, norm=None, eps=1e-6, stream=None) -> None:
     """mt_quantize_f8: the rows of x [rows, K], RMS-normalised with gain ``norm`` if given, into an F8Matrix."""
     if tuple(x.shape) != tuple(out.shape) or x.stride(1) != 1:
         raise ValueError("x and the matrix must be of one shape, x's rows contiguous")
-    if x.get_device() != out.device:
-        raise ValueError("x and the matrix are on different devices")
+    if x.get_device() != out.device or (norm is not None and norm.get_device() != out.device):
+        raise ValueError("x, norm and the matrix must be on one device")
+    if norm is not None and norm.numel() < x.shape[1]:
+        raise ValueError("norm holds K values")
     check(load().mt_quantize_f8(_ptr(x), dtype_code(x), x.shape[0], x.shape[1], x.stride(0), _ptr(norm),
                                 dtype_code(norm) if norm is not None else F16, eps, _ptr(out.codes), out.codes.stride(0),
                                 _ptr(out.scales), out.scales.stride(0), _on(out.device, stream)))
@@ -642,6 +648,8 @@ def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6,
     rows, k = x.shape
     if k != K or rows < M or (w2 is not None and w2.shape != w.shape):
         raise ValueError("x, w and w2 must agree in K, w and w2 in shape")
+    if (bias is not None and bias.numel() < N) or (norm is not None and norm.numel() < K):
+        raise ValueError("bias holds N values, norm K")
     if not w.whole or (w2 is not None and not w2.whole):
         raise ValueError("weights must be contiguous")
     if not isinstance(x, F8Matrix) and (M > LINEAR_F8_ROWS or (norm is not None and K > LINEAR_F8_NORM_K)):
@@ -659,8 +667,9 @@ def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6,
         if unit != 1:
             raise ValueError("x's rows must be contiguous")
         xp, xt, xs, ldxs, on = x.data_ptr(), dtype_code(x), None, 0, x.get_device()
-    if on != d or (w2 is not None and w2.device != d):
-        raise ValueError("x, w and w2 are on different devices")
+    if on != d or (w2 is not None and w2.device != d) \
+            or (bias is not None and bias.get_device() != d) or (norm is not None and norm.get_device() != d):
+        raise ValueError("x, w, w2, bias and norm must be on one device")
     wp, _, ws, _ = w.args
     up, _, us, _ = w2.args if w2 is not None else (None, 0, None, 0)
     rc = (_lib or load()).mt_linear_f8(xp, xt, xs, ldxs, _ptr(norm), wp, ws, up, us, _ptr(bias), bt, _words(d, y),

@@ -245,6 +245,22 @@ def test_python_refuses_strided_rows():
             mt.linear_f8(x, w, torch.zeros(2, 4))
 
 
+def test_python_refuses_short_vectors():
+    w = mt.F8Matrix(torch.zeros(4, 48, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8))
+    for more in (dict(bias=torch.zeros(3, dtype=torch.float16)), dict(norm=torch.zeros(47, dtype=torch.float16))):
+        with pytest.raises(ValueError, match="holds"):
+            mt.linear_f8(torch.zeros(2, 48), w, torch.zeros(2, 4), **more)
+
+
+def test_python_refuses_two_devices():
+    c, s = torch.zeros(2, 2, 8, 64, dtype=torch.uint8), torch.ones(2, 2, 8, dtype=torch.uint8)
+    for bad in ((c, c.to("meta"), s, s), (c, c, s, s.to("meta"))):
+        with pytest.raises(ValueError, match="one device"):
+            mt.KV(*bad)
+    with pytest.raises(ValueError, match="one device"):
+        mt.F8Matrix(torch.zeros(4, 48, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8, device="meta"))
+
+
 def test_the_oracle_of_the_format():
     """Every code is its own nearest code at scale 1, midpoints go to the even one, blocks take the least scale."""
     x = np.where(np.isnan(U.TABLE), 0, U.TABLE)

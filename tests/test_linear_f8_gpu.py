@@ -260,3 +260,18 @@ def test_scratch_belongs_to_the_calls_stream(gpu):
         assert len(segments) == 1 and segments[0]["stream"] == owner
         torch.cuda.synchronize()
         assert torch.equal(m.codes, mt.F8Matrix.quantize(x).codes)
+
+
+@pytest.mark.parametrize("M", [2, 40])
+def test_operands_on_the_host_are_refused(gpu, M):
+    w, _ = matrix(np.ones((32, 256)), gpu)
+    x, y, host = torch.ones(M, 256, device=gpu), torch.zeros(M, 32, device=gpu), torch.ones(256, dtype=torch.float16)
+    for more in (dict(bias=host[:32]), dict(norm=host)):
+        with pytest.raises(ValueError, match="one device"):
+            mt.linear_f8(x, w, y, **more)
+    with pytest.raises(ValueError):
+        mt.linear_f8(x.cpu(), w, y)
+    with pytest.raises(ValueError):
+        mt.linear_f8(x, w, y.cpu())
+    torch.cuda.synchronize()
+    assert not y.any()
