@@ -473,7 +473,8 @@ int mt_kv_copy(const mt_kv *src, const mt_kv *dst, uint32_t B, uint32_t T, uint3
  * i (window 0 = unlimited).  q rows (stride ldq) hold hq heads of 64, already rotated; out
  * rows stride ldo; scores scaled by `scale`, max-subtracted softmax; q and out are 16-byte
  * aligned with 16-byte row strides and do not overlap.  Both caches are of one type.  Cache slots
- * that a row does not attend do not reach its result, whatever they hold.
+ * that a row does not attend do not reach its result, whatever they hold.  A NaN or +infinity among the scores
+ * that it does attend makes its head NaN; a score of -infinity is no weight.
  *
  * len_max is the caller's bound on the own keys, max(pos[b] + counts[b]) (0: cache_len, which is also what
  * to ask the workspace for then).  It only places the work (longer sequences give the same results, more slowly).  The keys are split over

@@ -21,6 +21,7 @@
 //     step's keys are requested behind the scores, its values behind p . v, through buffer descriptors that end with the keys:
 //     what stands behind them is never read.  Keys inside that are not a row's (causal, window) weigh exactly zero;
 //     where such a key or value is not finite, a row's outputs are not either, and it is done again from its own keys alone.
+//     A NaN among a row's own scores is in the weights' sum, so the row is NaN wherever its keys are placed.
 //   - Few rows over many keys, or a prefix for many sequences: parts of the keys go to workgroups of their own and a second
 //     kernel joins them (shared_plan).  Sums meet in a fixed order everywhere: the same call gives the same bits.
 //   - Bound: instructions.  A step of 64 8-bit keys is about 380 vector instructions and 48 MFMAs a wave whether 7 or 16 rows
@@ -87,7 +88,8 @@ __device__ __forceinline__ float cached(const char *base, const uint8_t *scales,
 }
 
 // One query head over keys [lo, hi) (prefix first) by one wave, touching those keys only: each lane a
-// key's score, then each lane a dim's sum.  An online softmax in fp32, 64 keys at a time.
+// key's score, then each lane a dim's sum.  An online softmax in fp32, 64 keys at a time.  (The maximum takes no notice of
+// NaN, so a NaN score has to become its weight by itself where no other score of its keys is above -infinity.)
 template <int CT>
 __device__ __forceinline__ void attend_wave(const float *q, const HeadKv &h, uint32_t lo, uint32_t hi, float scale, float *out) {
     const uint32_t lane = threadIdx.x & 63;
@@ -104,7 +106,7 @@ __device__ __forceinline__ void attend_wave(const float *q, const HeadKv &h, uin
         }
         const float mn = fmaxf(m, wave_max(s));
         const float al = m == -INFINITY ? 0.0f : exp_hw(m - mn);
-        const float p = key >= hi || mn == -INFINITY ? 0.0f : exp_hw(s - mn);
+        const float p = key >= hi ? 0.0f : mn == -INFINITY ? (s != s ? s : 0.0f) : exp_hw(s - mn);
         m = mn;
         l = fmaf(l, al, group_sum(p, 64));
         o *= al;
@@ -441,6 +443,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
             const int ex = min(267 - static_cast<int>(__float_as_uint(mx) >> 23), 253);
             f = __uint_as_float(static_cast<uint32_t>(ex) << 23);
             c = fabsf(c0) * __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+            if (c < 0x1p-126f) c = 0x1p-126f;  // not 0, so that a key outside weighs 0 (-infinity times c); scores are below 2^37
             if (c0 < 0.0f) f = -f;
         }
 #pragma unroll
@@ -675,7 +678,9 @@ __global__ __launch_bounds__(64 * AJ_WAVES) void attention_join_kernel(SharedArg
         }
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
-            if (s0 + i * waves >= S || e[i].x == INFINITY) continue;  // (a part without a key of the row has no sums)
+            // A part without a key of the row, or with scores of -infinity alone, has no sums; one of NaN scores alone has no
+            // maximum either, but a sum that is NaN.
+            if (s0 + i * waves >= S || (e[i].x == INFINITY && e[i].y == 0.0f)) continue;
             const float mn = fminf(m, e[i].x);
             const float f = m == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mn - m), k = __builtin_amdgcn_exp2f(mn - e[i].x);
             m = mn;
