@@ -7,7 +7,8 @@
 //   - Angles: position times frequency is exact in 64 bits, and its turns are taken off there, so a far position
 //     costs no bits (an fp32 product is off by 2^-24 of the angle: 0.008 radians at position 131072).  Sine,
 //     cosine and rotation stay in 64 bits up to the one rounding into q or the cache: an 8-bit code that an
-//     fp32 rotation's error tips over is off by a whole step of 2^-3 (about one in a million values).
+//     fp32 rotation's error tips over is off by a whole step of 2^-3 (about one in a million values), and about one in 2^14
+//     fp16 keys would be the wrong neighbour of a tie if it were rounded to fp32 first.
 //   - Eight lanes a head: lane r holds dims 4 r .. + 3 and 32 + 4 r .. + 3, both halves of its four
 //     pairs.  The block's largest value is three DPP steps, the codes two words a lane.
 //   - Bound: launch latency for a decode step's rows (1.9 us for two), the bytes of qkv and q for prompts (16 sequences of
@@ -102,8 +103,8 @@ __global__ __launch_bounds__(KV_THREADS) void rope_append_kernel(const float *qk
                 const double a = x[e], b2 = x[4 + e];
                 const double lo2 = fma(-b2, t.y, a * t.x), hi2 = fma(a, t.y, b2 * t.x);
                 // (a NaN among the odd ones stays one; infinities are exact)
-                x[e] = CT == DT_F8 && !is_q ? to_odd(lo2) : static_cast<float>(lo2);
-                x[4 + e] = CT == DT_F8 && !is_q ? to_odd(hi2) : static_cast<float>(hi2);
+                x[e] = CT != DT_F32 && !is_q ? to_odd(lo2) : static_cast<float>(lo2);
+                x[4 + e] = CT != DT_F32 && !is_q ? to_odd(hi2) : static_cast<float>(hi2);
             }
         }
         if (is_q) {
