@@ -415,7 +415,10 @@ int mt_attention_decode(const float *q, uint32_t ldq, uint32_t B, uint32_t hq, u
  * least scale, 2^-126 or more, at which its largest finite |x| is at most 448, and x / scale
  * rounded to nearest, ties to even; infinities and NaN become NaN.  Scale bytes are 1 .. 254 (written
  * ones at most 247).  A stored value is off by at most 2^-4 of itself, or 2^-10 of the scale where that is
- * more, and is exactly a bf16 number.  In a cache a block is the 64 values of one head at one position; in a
+ * more (a finite |x| of 248 2^120 = 3.3e38 or more is stored as 2^128 and read as infinity).  From scale byte 3 on it is
+ * exactly a bf16 number; under bytes 1 and 2 (blocks within 448 2^-125 = 1.05e-35) the matrix products take it rounded
+ * to a multiple of 2^-133, and attention's sums are off by up to 2^-125 a key under scale bytes below 17.
+ * In a cache a block is the 64 values of one head at one position; in a
  * matrix it is 128 consecutive values of a row (the last block of a row may be shorter).
  *
  * mt_kv -- the caches of one layer for a batch of sequences: k and v [hkv, cache_len, 64] of type
@@ -502,7 +505,7 @@ int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, ui
  * up to 16 rows of fp32, fp16 or bf16 values, which the call quantises on the way in, after the RMSNorm
  * with gain `norm` and p.eps if norm is given (more rows, or a norm over K > 32768: MT_ENOTSUP, quantise
  * them first; a norm takes K <= 524288 there).  The same
- * bytes as mt_quantize_f8 of x enter the product.  Products are exact and sums fp32.  bias and norm are of type bt (MT_F16 or
+ * bytes as mt_quantize_f8 of x enter the product.  Products are exact (of the values as mt_kv has them) and sums fp32.  bias and norm are of type bt (MT_F16 or
  * MT_BF16); flags, bias, epilogue, y and overlap rules as mt_linear; K a multiple of 16 up to 2^22 (and ldx of codes); codes 16-byte
  * aligned, scales 4-byte aligned.
  */

@@ -11,8 +11,9 @@
 //     the lane keys 4 g .. + 3 of its own row l16, so the softmax is in-lane but for one exchange of the maximum a step.
 //   - p . v: O^T = V^T P^T.  The weights stay where the scores stood; a lane reads dims 4 l16 .. + 3 of those keys' values and
 //     byte permutes put two keys side by side.
-//   - 8 bits: a key's codes become bf16 with its scale in the conversion (exact); a value's scale goes into its
-//     weight, whose pieces are then the weight times a power of two.  bf16 has the range for any scale.
+//   - 8 bits: a key's codes become bf16 with its scale in the conversion (exact from scale byte 3 on); a value's scale goes
+//     into its weight, whose pieces are then the weight times a power of two.  bf16 has the range for any scale, but its
+//     steps end at 2^-133: what a weight's pieces lose there is below 2^-134, times a code below 2^-125 a key.
 //   - Precision: q and the weights as three bf16 pieces (24 bits) against 8-bit and fp32 caches, those in three pieces too,
 //     the 6 products above 2^-24; two fp16 pieces (22 bits) against fp16 caches.  All sums in fp32; a step's p . v starts from
 //     zero and joins the running sum in one rounding.  Normwise error against fp64 1e-7 to 4e-7 up to 131072 keys (the plain fp32
@@ -84,7 +85,7 @@ __device__ __forceinline__ float cached(const char *base, const uint8_t *scales,
     const char *row = base + slot * Cached<CT>::ROW;
     if constexpr (CT == DT_F32) return reinterpret_cast<const float *>(row)[e];
     else if constexpr (CT == DT_F16) return (float)reinterpret_cast<const _Float16 *>(row)[e];
-    else return bf16_lo(f8_bf16x2<false>(reinterpret_cast<const uint8_t *>(row)[e], f8_pow2(scales[slot])));
+    else return bf16_lo(f8_bf16x2<false>(reinterpret_cast<const uint8_t *>(row)[e], 1.0f)) * f8_pow2(scales[slot]);
 }
 
 // One query head over keys [lo, hi) (prefix first) by one wave, touching those keys only: each lane a

@@ -4,9 +4,11 @@
 // A block's scale is the least power of two, 2^-126 or more, that brings its largest finite |x| to
 // 448 or less; the codes are x / scale to nearest, ties to even.  Both steps are exact but for that
 // one rounding (half a step of 3 mantissa bits: 2^-4 of the value), so every way of computing the
-// same x gives the same bytes, and a code times its scale is a bf16 number: the conversion
-// instructions that take the scale (v_cvt_scalef32_pk_bf16_fp8) give the value without a rounding.
-// Infinities and NaN become NaN codes and do not count for the scale.
+// same x gives the same bytes, and a code times its scale is a bf16 number from scale byte 3 on: the conversion
+// instructions that take the scale (v_cvt_scalef32_pk_bf16_fp8) give the value without a rounding.  Under bytes 1 and 2
+// (blocks whose largest |x| is at most 448 2^-125) the least codes are finer than bf16, whose steps end at 2^-133.
+// Infinities and NaN become NaN codes and do not count for the scale.  A finite |x| of 248 2^120 or more is rounded
+// to 2^128, which fp32 and bf16 read as infinity.
 #pragma once
 
 #include "mt_device.hpp"
@@ -46,11 +48,11 @@ __device__ __forceinline__ uint32_t f8_bf16x2(uint32_t w, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w), scale, HI));
 }
 
-// Four codes of a word times the scale as fp32.
+// Four codes of a word times the scale as fp32, exactly: the least product, 2^-9 2^-126, is an fp32 number.
 __device__ __forceinline__ void f8_decode4(uint32_t w, float scale, float *o) {
-    const uint32_t a = f8_bf16x2<false>(w, scale), b = f8_bf16x2<true>(w, scale);
-    o[0] = bf16_lo(a); o[1] = bf16_hi(a);
-    o[2] = bf16_lo(b); o[3] = bf16_hi(b);
+    const uint32_t a = f8_bf16x2<false>(w, 1.0f), b = f8_bf16x2<true>(w, 1.0f);
+    o[0] = bf16_lo(a) * scale; o[1] = bf16_hi(a) * scale;
+    o[2] = bf16_lo(b) * scale; o[3] = bf16_hi(b) * scale;
 }
 
 // A wave's LDS writes before it stand before its reads behind it.
