@@ -425,7 +425,8 @@ int mt_attention_decode(const float *q, uint32_t ldq, uint32_t B, uint32_t hq, u
  * cache_t (MT_F32, MT_F16 or MT_F8), 16-byte aligned, each sequence's `stride` elements behind the
  * one before (a multiple of 16; not read for one sequence); with MT_F8 also k_scale and v_scale
  * [hkv, cache_len] bytes, 4-byte aligned, scale_stride bytes a sequence (a multiple of 4), and
- * cache_len a multiple of 4.  cache_len is at most 2^30.
+ * cache_len a multiple of 4.  cache_len is at most 2^30.  k, v and the scales do not overlap; with one stride (in bytes)
+ * they may lie between each other, a sequence's keys, values and scales side by side.
  *
  * Rows: the calls below take B sequences of T rows each, row b T + t being sequence b's row t.  pos
  * (device, B uint32; NULL: zeros) gives each sequence's first row's slot in its own caches, so row t

@@ -16,6 +16,23 @@ bool meet(const void *a, uint64_t an, const void *b, uint64_t bn) {
     return an && bn && x < y + bn && y < x + an;
 }
 
+// The keys, values or scales of B sequences: `each` bytes a sequence, `stride` bytes from one to the next.
+struct Runs {
+    const void *p;
+    uint64_t each, stride;
+    uint32_t B;
+    uint64_t all() const { return each ? (B - 1) * stride + each : 0; }
+};
+// Do two of them meet?  Those of one stride may lie between each other (a sequence's keys and values side by side): they are
+// apart if, from a run of a on, the next run of b starts behind it and ends before a's next one.
+bool meet(const Runs &a, const Runs &b) {
+    if (!meet(a.p, a.all(), b.p, b.all())) return false;
+    if (a.B == 1 || a.stride != b.stride) return true;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    const uint64_t s = a.stride, at = y >= x ? (y - x) % s : (s - (x - y) % s) % s;
+    return at < a.each || at + b.each > s;
+}
+
 uint64_t elem_bytes(int t) { return t == DT_F32 ? 4 : t == DT_F8 ? 1 : 2; }
 
 // Bytes from the first to the last element of `rows` rows of `width` elements of `size` bytes.
@@ -51,13 +68,23 @@ int validate_kv(const char *who, const char *what, const mt_kv *c, uint32_t B, u
     return MT_OK;
 }
 
-// Bytes of the values, and of the scales, of B sequences' keys (or values).
-uint64_t kv_bytes(const KvArgs &c, int ct, uint32_t B, uint32_t hkv) {
-    return ((B - 1) * c.stride + static_cast<uint64_t>(hkv) * c.len * 64) * elem_bytes(ct);
-}
-uint64_t scale_bytes(const KvArgs &c, int ct, uint32_t B, uint32_t hkv) {
-    return ct == DT_F8 ? (B - 1) * c.sstride + static_cast<uint64_t>(hkv) * c.len : 0;
-}
+// The memory of B sequences' caches: keys, values and, in 8 bits, their scales.
+struct KvRuns {
+    Runs r[4];
+    KvRuns(const KvArgs &c, int ct, uint32_t B, uint32_t hkv) {
+        const uint64_t slots = static_cast<uint64_t>(hkv) * c.len, es = elem_bytes(ct), scales = ct == DT_F8 ? slots : 0;
+        r[0] = Runs{c.k, slots * 64 * es, c.stride * es, B};
+        r[1] = Runs{c.v, slots * 64 * es, c.stride * es, B};
+        r[2] = Runs{c.ks, scales, c.sstride, B};
+        r[3] = Runs{c.vs, scales, c.sstride, B};
+    }
+    bool meet_each_other() const {
+        for (int i = 1; i < 4; i++)
+            for (int j = 0; j < i; j++)
+                if (meet(r[i], r[j])) return true;
+        return false;
+    }
+};
 
 }  // namespace
 
@@ -87,15 +114,11 @@ int mt_rope_append(const float *qkv, uint32_t ldq, uint32_t B, uint32_t T, uint3
     const uint64_t in = span(all, width, ldq, 4), outb = q ? span(all, static_cast<uint64_t>(hq) * 64, ldo, 4) : 0;
     if (q && !(q == qkv && ldo == ldq) && meet(qkv, in, q, outb))
         return set_error(MT_EINVAL, "%s: q overlaps qkv (in place: q = qkv and ldo = ldq)", who);
-    const uint64_t kb = kv_bytes(c, kv->cache_t, B, hkv), sb = scale_bytes(c, kv->cache_t, B, hkv);
-    const void *caches[4] = {c.k, c.v, c.ks, c.vs};
-    for (int i = 0; i < 4; i++) {
-        const uint64_t n = i < 2 ? kb : sb;
-        if (meet(caches[i], n, qkv, in) || meet(caches[i], n, q, outb))
+    const KvRuns caches(c, kv->cache_t, B, hkv);
+    for (const Runs &r : caches.r)
+        if (meet(r.p, r.all(), qkv, in) || meet(r.p, r.all(), q, outb))
             return set_error(MT_EINVAL, "%s: the caches overlap qkv or q", who);
-        for (int j = 0; j < i; j++)
-            if (meet(caches[i], n, caches[j], j < 2 ? kb : sb)) return set_error(MT_EINVAL, "%s: the caches overlap each other", who);
-    }
+    if (caches.meet_each_other()) return set_error(MT_EINVAL, "%s: the caches overlap each other", who);
     return launch_rope_append(qkv, ldq, rows, hq, hkv, offset, c, kv->cache_t, inv_freq, q, ldo,
                               reinterpret_cast<hipStream_t>(stream));
 }
@@ -110,15 +133,11 @@ int mt_kv_copy(const mt_kv *src, const mt_kv *dst, uint32_t B, uint32_t T, uint3
     rc = validate_kv(who, "src", src, B, hkv, s);
     if (!rc) rc = validate_kv(who, "dst", dst, B, hkv, d);
     if (rc) return rc;
-    const uint64_t n[2] = {kv_bytes(s, src->cache_t, B, hkv), scale_bytes(s, src->cache_t, B, hkv)};
-    const uint64_t m[2] = {kv_bytes(d, dst->cache_t, B, hkv), scale_bytes(d, dst->cache_t, B, hkv)};
-    const void *from[4] = {s.k, s.v, s.ks, s.vs}, *to[4] = {d.k, d.v, d.ks, d.vs};
-    for (int i = 0; i < 4; i++) {
-        for (int j = 0; j < 4; j++) {
-            if (meet(from[i], n[i / 2], to[j], m[j / 2])) return set_error(MT_EINVAL, "%s: src and dst overlap", who);
-            if (j < i && meet(to[i], m[i / 2], to[j], m[j / 2])) return set_error(MT_EINVAL, "%s: dst's caches overlap each other", who);
-        }
-    }
+    const KvRuns from(s, src->cache_t, B, hkv), to(d, dst->cache_t, B, hkv);
+    for (const Runs &a : from.r)
+        for (const Runs &b : to.r)
+            if (meet(a, b)) return set_error(MT_EINVAL, "%s: src and dst overlap", who);
+    if (to.meet_each_other()) return set_error(MT_EINVAL, "%s: dst's caches overlap each other", who);
     return launch_kv_copy(s, src->cache_t, d, dst->cache_t, RowsArgs{pos, counts, B, T}, hkv, reinterpret_cast<hipStream_t>(stream));
 }
 
