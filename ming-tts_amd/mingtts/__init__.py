@@ -447,12 +447,17 @@ def attention_decode(q, ldq, B, hq, hkv, lens, window, kc, vc, cache_len, cache_
 
 # ----------------------------------- 8-bit storage and shared prefixes --
 
+_slot_types: tuple = ()  # torch types of pos and counts
+
+
 def _storage_code(t) -> int:
-    """dtype_code, and F8 for codes (uint8 or float8_e4m3fn)."""
-    if t.element_size() == 1:
-        import torch
-        if t.dtype in (torch.uint8, torch.float8_e4m3fn):
-            return F8
+    """dtype_code, and F8 for codes (uint8 or float8_e4m3fn).  Every cache and matrix passes here, so the types that
+    the calls check are known behind it."""
+    global _slot_types
+    import torch
+    _slot_types = (torch.int32, torch.uint32)
+    if t.dtype in (torch.uint8, torch.float8_e4m3fn):
+        return F8
     return dtype_code(t)
 
 
@@ -502,9 +507,18 @@ def _refuse_kv(kv, B, hkv):
 
 
 def _words(device, t):
-    """The address of a tensor of 4-byte elements (fp32, or int32 for pos and counts) on the given device."""
+    """The address of a tensor of 4-byte elements (fp32) on the given device."""
     if t.element_size() != 4 or t.get_device() != device:
-        raise ValueError("activations are fp32, pos and counts int32, all on the caches' or weights' device")
+        raise ValueError("activations are fp32, on the caches' or weights' device")
+    return t.data_ptr()
+
+
+def _slots(device, t, B):
+    """The address of pos or counts (None: none), a number a sequence."""
+    if t is None:
+        return None
+    if t.dtype not in _slot_types or t.get_device() != device or t.numel() < B or not t.is_contiguous():
+        raise ValueError("pos and counts are int32, one a sequence side by side, on the caches' device")
     return t.data_ptr()
 
 
@@ -528,8 +542,8 @@ def rope_append(qkv, B, T, hq, hkv, pos, kv, inv_freq, q=None, counts=None, offs
         _refuse_kv(kv, B, hkv)
     d = kv.device
     rc = (_lib or load()).mt_rope_append(
-        _words(d, qkv), qkv.stride(0) if ldq is None else ldq, B, T, hq, hkv, None if pos is None else _words(d, pos),
-        None if counts is None else _words(d, counts), offset, kv.ref, _words(d, inv_freq), None if q is None else _words(d, q),
+        _words(d, qkv), qkv.stride(0) if ldq is None else ldq, B, T, hq, hkv, _slots(d, pos, B),
+        _slots(d, counts, B), offset, kv.ref, _words(d, inv_freq), None if q is None else _words(d, q),
         ldo if ldo is not None else 0 if q is None else q.stride(0), _on(d, stream))
     if rc < 0:
         check(rc)
@@ -542,8 +556,8 @@ def kv_copy(src, dst, B, T, pos=None, counts=None, stream=None) -> None:
     d = src.device
     if dst.device != d:
         raise ValueError("src and dst are on different devices")
-    rc = (_lib or load()).mt_kv_copy(src.ref, dst.ref, B, T, src.hkv, None if pos is None else _words(d, pos),
-                                     None if counts is None else _words(d, counts), _on(d, stream))
+    rc = (_lib or load()).mt_kv_copy(src.ref, dst.ref, B, T, src.hkv, _slots(d, pos, B),
+                                     _slots(d, counts, B), _on(d, stream))
     if rc < 0:
         check(rc)
 
@@ -576,8 +590,8 @@ def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=Non
     if need and workspace is None:
         workspace = _scratch(need, q, stream)
     rc = (_lib or load()).mt_attention_shared(
-        _words(d, q), q.stride(0) if ldq is None else ldq, B, T, hq, hkv, None if pos is None else _words(d, pos),
-        None if counts is None else _words(d, counts), kv.ref, pre, prefix_len, len_max, window, _words(d, out),
+        _words(d, q), q.stride(0) if ldq is None else ldq, B, T, hq, hkv, _slots(d, pos, B),
+        _slots(d, counts, B), kv.ref, pre, prefix_len, len_max, window, _words(d, out),
         out.stride(0) if ldo is None else ldo, scale, None if workspace is None else workspace.data_ptr(),
         0 if workspace is None else workspace.numel() * workspace.element_size(), _on(d, stream))
     if rc < 0:

@@ -1,0 +1,85 @@
+"""What the Python calls of the 8-bit and shared-prefix operators refuse before they pass an address on, and what they take,
+without a GPU: a call whose operands are accepted gets as far as asking for the stream."""
+import pytest
+import torch
+
+import mingtts as mt
+
+
+class Reached(Exception):
+    pass
+
+
+@pytest.fixture(autouse=True)
+def no_launch(monkeypatch):
+    def on(device, stream):
+        raise Reached
+
+    monkeypatch.setattr(mt, "_on", on)
+
+
+z = torch.zeros
+B, T, HQ, HKV, CAP, K, N = 3, 2, 4, 2, 8, 48, 24
+
+
+def i32(*shape):
+    return z(*shape, dtype=torch.int32)
+
+
+def caches(batch=B):
+    c, s = z(batch, HKV, CAP, 64, dtype=torch.uint8), z(batch, HKV, CAP, dtype=torch.uint8)
+    return mt.KV(c, c.clone(), s, s.clone())
+
+
+def append(**over):
+    a = dict(qkv=z(B * T, 512), B=B, T=T, hq=HQ, hkv=HKV, pos=i32(B), kv=caches(), inv_freq=z(32), q=z(B * T, 256), counts=i32(B))
+    mt.rope_append(**{**a, **over})
+
+
+def copy(**over):
+    a = dict(src=caches(), dst=caches(), B=B, T=T, pos=i32(B), counts=i32(B))
+    mt.kv_copy(**{**a, **over})
+
+
+def attend(**over):
+    a = dict(q=z(B * T, 256), B=B, T=T, hq=HQ, hkv=HKV, pos=i32(B), kv=caches(), out=z(B * T, 256), counts=i32(B))
+    mt.attention_shared(**{**a, **over})
+
+
+def matrix(rows=N):
+    return mt.F8Matrix(z(rows, K, dtype=torch.uint8), z(rows, 4, dtype=torch.uint8))
+
+
+def linear(**over):
+    a = dict(x=z(4, K), w=matrix(), y=z(4, N))
+    mt.linear_f8(**{**a, **over})
+
+
+def quantize(**over):
+    a = dict(x=z(N, K), out=matrix())
+    mt.quantize_f8(**{**a, **over})
+
+
+CALLS = [append, copy, attend, linear, quantize]
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_the_plain_calls_are_taken(call):
+    with pytest.raises(Reached):
+        call()
+
+
+@pytest.mark.parametrize("call", [append, copy, attend])
+@pytest.mark.parametrize("name", ["pos", "counts"])
+@pytest.mark.parametrize("bad", [z(B), z(B, dtype=torch.int64), i32(B - 1), i32(2 * B)[::2], i32(B, 2)[:, 0]],
+                         ids=["fp32", "int64", "short", "strided", "column"])
+def test_positions_and_counts(call, name, bad):
+    with pytest.raises(ValueError, match="int32"):
+        call(**{name: bad})
+
+
+@pytest.mark.parametrize("call", [append, copy, attend])
+@pytest.mark.parametrize("good", [None, i32(B + 2), i32(B, 1), z(B, dtype=torch.uint32), i32(9)[3:]], ids=str)
+def test_positions_and_counts_that_are_taken(call, good):
+    with pytest.raises(Reached):
+        call(pos=good, counts=good)
