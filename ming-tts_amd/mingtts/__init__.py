@@ -448,14 +448,15 @@ def attention_decode(q, ldq, B, hq, hkv, lens, window, kc, vc, cache_len, cache_
 # ----------------------------------- 8-bit storage and shared prefixes --
 
 _slot_types: tuple = ()  # torch types of pos and counts
+_row_type = None         # and of activations
 
 
 def _storage_code(t) -> int:
     """dtype_code, and F8 for codes (uint8 or float8_e4m3fn).  Every cache and matrix passes here, so the types that
     the calls check are known behind it."""
-    global _slot_types
+    global _slot_types, _row_type
     import torch
-    _slot_types = (torch.int32, torch.uint32)
+    _slot_types, _row_type = (torch.int32, torch.uint32), torch.float32
     if t.dtype in (torch.uint8, torch.float8_e4m3fn):
         return F8
     return dtype_code(t)
@@ -506,10 +507,37 @@ def _refuse_kv(kv, B, hkv):
     raise ValueError(f"caches of {kv.batch} sequences and {kv.hkv} heads for {B} and {hkv}")
 
 
-def _words(device, t):
-    """The address of a tensor of 4-byte elements (fp32) on the given device."""
-    if t.element_size() != 4 or t.get_device() != device:
+def _rows(device, t, rows, width, ld=None):
+    """The address and row stride of `rows` fp32 rows of `width` values: a tensor [rows, width] or larger (leading
+    dimensions count as one where they can), or any tensor that holds them at a stride `ld` from its first element on."""
+    if t.dtype is not _row_type or t.get_device() != device:
         raise ValueError("activations are fp32, on the caches' or weights' device")
+    if ld is None:
+        shape = t.shape
+        if len(shape) == 2 and shape[0] >= rows and shape[1] >= width:
+            ld, unit = t.stride()
+            if unit == 1 or width == 1:
+                return t.data_ptr(), ld
+        return _folded_rows(device, t, rows, width)
+    if rows and (rows - 1) * ld + width > t.untyped_storage().nbytes() // 4 - t.storage_offset():
+        raise ValueError(f"no {rows} rows of {width} values at a stride of {ld} in {tuple(t.shape)}")
+    return t.data_ptr(), ld
+
+
+def _folded_rows(device, t, rows, width):
+    if rows == 0:
+        return t.data_ptr(), width
+    if t.dim() > 2:
+        try:
+            return _rows(device, t.view(-1, t.shape[-1]), rows, width)
+        except RuntimeError:  # leading dimensions that are not one
+            pass
+    raise ValueError(f"not {rows} rows of {width} values side by side: {tuple(t.shape)} at strides {t.stride()}")
+
+
+def _frequencies(device, t):
+    if t.dtype is not _row_type or t.get_device() != device or t.numel() < 32 or not t.is_contiguous():
+        raise ValueError("inv_freq holds 32 fp32 values side by side, on the caches' device")
     return t.data_ptr()
 
 
@@ -541,10 +569,10 @@ def rope_append(qkv, B, T, hq, hkv, pos, kv, inv_freq, q=None, counts=None, offs
     if kv.hkv != hkv or kv.batch < B:
         _refuse_kv(kv, B, hkv)
     d = kv.device
-    rc = (_lib or load()).mt_rope_append(
-        _words(d, qkv), qkv.stride(0) if ldq is None else ldq, B, T, hq, hkv, _slots(d, pos, B),
-        _slots(d, counts, B), offset, kv.ref, _words(d, inv_freq), None if q is None else _words(d, q),
-        ldo if ldo is not None else 0 if q is None else q.stride(0), _on(d, stream))
+    src, ldq = _rows(d, qkv, B * T, (hq + 2 * hkv) * 64, ldq)
+    dst, ldo = (None, 0) if q is None else _rows(d, q, B * T, hq * 64, ldo)
+    rc = (_lib or load()).mt_rope_append(src, ldq, B, T, hq, hkv, _slots(d, pos, B), _slots(d, counts, B), offset, kv.ref,
+                                         _frequencies(d, inv_freq), dst, ldo, _on(d, stream))
     if rc < 0:
         check(rc)
 
@@ -586,13 +614,14 @@ def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=Non
         if prefix_len is None:
             prefix_len = prefix.cache_len
         pre = prefix.ref
+    src, ldq = _rows(d, q, B * T, hq * 64, ldq)
+    dst, ldo = _rows(d, out, B * T, hq * 64, ldo)
     need = _shared_need(B, T, hq, hkv, prefix_len, len_max or kv.cache_len, window, kv.type)
     if need and workspace is None:
         workspace = _scratch(need, q, stream)
     rc = (_lib or load()).mt_attention_shared(
-        _words(d, q), q.stride(0) if ldq is None else ldq, B, T, hq, hkv, _slots(d, pos, B),
-        _slots(d, counts, B), kv.ref, pre, prefix_len, len_max, window, _words(d, out),
-        out.stride(0) if ldo is None else ldo, scale, None if workspace is None else workspace.data_ptr(),
+        src, ldq, B, T, hq, hkv, _slots(d, pos, B), _slots(d, counts, B), kv.ref, pre, prefix_len, len_max, window, dst, ldo,
+        scale, None if workspace is None else workspace.data_ptr(),
         0 if workspace is None else workspace.numel() * workspace.element_size(), _on(d, stream))
     if rc < 0:
         check(rc)
@@ -684,10 +713,11 @@ def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6,
     if on != d or (w2 is not None and w2.device != d) \
             or (bias is not None and bias.get_device() != d) or (norm is not None and norm.get_device() != d):
         raise ValueError("x, w, w2, bias and norm must be on one device")
+    yp, ldy = _rows(d, y, M, N, ldy)
     wp, _, ws, _ = w.args
     up, _, us, _ = w2.args if w2 is not None else (None, 0, None, 0)
-    rc = (_lib or load()).mt_linear_f8(xp, xt, xs, ldxs, _ptr(norm), wp, ws, up, us, _ptr(bias), bt, _words(d, y),
-                                       GemvParams(M, N, K, ldx, y.stride(0) if ldy is None else ldy, flags, eps), _on(d, stream))
+    rc = (_lib or load()).mt_linear_f8(xp, xt, xs, ldxs, _ptr(norm), wp, ws, up, us, _ptr(bias), bt, yp,
+                                       GemvParams(M, N, K, ldx, ldy, flags, eps), _on(d, stream))
     if rc < 0:
         check(rc)
 

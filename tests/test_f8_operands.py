@@ -83,3 +83,46 @@ def test_positions_and_counts(call, name, bad):
 def test_positions_and_counts_that_are_taken(call, good):
     with pytest.raises(Reached):
         call(pos=good, counts=good)
+
+
+# A row operand: its call, its name, and the rows and columns that the call reads or writes.
+ROWS = [(append, "qkv", B * T, 512), (append, "q", B * T, 256), (attend, "q", B * T, 256), (attend, "out", B * T, 256),
+        (linear, "y", 4, N)]
+
+
+@pytest.mark.parametrize("call,name,rows,width", ROWS)
+def test_rows(call, name, rows, width):
+    bad = [z(rows - 1, width), z(rows, width - 1), z(rows, 2 * width)[:, ::2], z(width, rows).t(), z(rows * width - 1),
+           z(2, rows // 2, width - 1), z(2, rows, width)[:, ::2, 1:], z(rows // 2, 2, width).transpose(0, 1), z(())]
+    for t in bad:
+        with pytest.raises(ValueError, match="rows of"):
+            call(**{name: t})
+    for t in (z(rows, width, dtype=torch.float16), z(rows, width, dtype=torch.int32), z(rows, width, dtype=torch.float64)):
+        with pytest.raises(ValueError, match="fp32"):
+            call(**{name: t})
+
+
+@pytest.mark.parametrize("call,name,rows,width", ROWS)
+def test_rows_that_are_taken(call, name, rows, width):
+    for t in (z(rows + 1, width + 4), z(rows, 2 * width)[:, :width], z(2 * rows, width)[::2], z(2, rows // 2, width),
+              z(2, rows // 2, 2 * width)[:, :, :width], z(rows, 1, width), z(1, rows, 2 * width)[..., width:]):
+        with pytest.raises(Reached):
+            call(**{name: t})
+
+
+@pytest.mark.parametrize("call,name,rows,width,ld", [r + (ld,) for r, ld in zip(ROWS, ("ldq", "ldo", "ldq", "ldo", "ldy"))])
+def test_rows_at_a_given_stride(call, name, rows, width, ld):
+    """A tensor of any shape, from its first element on."""
+    most = (rows - 1) * (width + 4) + width
+    for t in (z(most), z(rows, width + 4), z(most + 5)[5:], z(2, rows, width)):
+        with pytest.raises(Reached):
+            call(**{name: t, ld: width + 4})
+    for t in (z(most - 1), z(most + 5)[6:], z(rows, width)):
+        with pytest.raises(ValueError, match="rows of"):
+            call(**{name: t, ld: width + 4})
+
+
+@pytest.mark.parametrize("bad", [z(31), z(64)[::2], z(32, dtype=torch.float64), z(32, dtype=torch.int32)], ids=["short", "strided", "fp64", "int32"])
+def test_frequencies(bad):
+    with pytest.raises(ValueError, match="32 fp32"):
+        append(inv_freq=bad)
