@@ -672,8 +672,8 @@ def quantize_f8(x, out, norm=None, eps=1e-6, stream=None) -> None:
         raise ValueError("x and the matrix must be of one shape, x's rows contiguous")
     if x.get_device() != out.device or (norm is not None and norm.get_device() != out.device):
         raise ValueError("x, norm and the matrix must be on one device")
-    if norm is not None and norm.numel() < x.shape[1]:
-        raise ValueError("norm holds K values")
+    if norm is not None and (norm.numel() < x.shape[1] or not norm.is_contiguous()):
+        raise ValueError("norm holds K values side by side")
     check(load().mt_quantize_f8(_ptr(x), dtype_code(x), x.shape[0], x.shape[1], x.stride(0), _ptr(norm),
                                 dtype_code(norm) if norm is not None else F16, eps, _ptr(out.codes), out.codes.stride(0),
                                 _ptr(out.scales), out.scales.stride(0), _on(out.device, stream)))
@@ -691,8 +691,9 @@ def linear_f8(x, w, y, M=None, flags=0, w2=None, bias=None, norm=None, eps=1e-6,
     rows, k = x.shape
     if k != K or rows < M or (w2 is not None and w2.shape != w.shape):
         raise ValueError("x, w and w2 must agree in K, w and w2 in shape")
-    if (bias is not None and bias.numel() < N) or (norm is not None and norm.numel() < K):
-        raise ValueError("bias holds N values, norm K")
+    if (bias is not None and (bias.numel() < N or not bias.is_contiguous())) \
+            or (norm is not None and (norm.numel() < K or not norm.is_contiguous())):
+        raise ValueError("bias holds N values, norm K, side by side")
     if not w.whole or (w2 is not None and not w2.whole):
         raise ValueError("weights must be contiguous")
     if not isinstance(x, F8Matrix) and (M > LINEAR_F8_ROWS or (norm is not None and K > LINEAR_F8_NORM_K)):

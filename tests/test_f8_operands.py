@@ -126,3 +126,23 @@ def test_rows_at_a_given_stride(call, name, rows, width, ld):
 def test_frequencies(bad):
     with pytest.raises(ValueError, match="32 fp32"):
         append(inv_freq=bad)
+
+
+def h16(*shape):
+    return z(*shape, dtype=torch.float16)
+
+
+@pytest.mark.parametrize("call,name,n", [(linear, "bias", N), (linear, "norm", K), (quantize, "norm", K)])
+def test_vectors(call, name, n):
+    for t in (h16(2 * n)[::2], h16(n, 2)[:, 0], h16(n - 1), h16(1).expand(n)):
+        with pytest.raises(ValueError, match="values"):
+            call(**{name: t})
+    for t in (h16(n), h16(n + 8), h16(2 * n)[n:]):
+        with pytest.raises(Reached):
+            call(**{name: t})
+
+
+@pytest.mark.parametrize("rows", [4, 20])  # quantised on the way in, and by a call before
+def test_a_strided_norm_of_many_rows(rows):
+    with pytest.raises(ValueError, match="values"):
+        linear(x=z(rows, K), y=z(rows, N), norm=h16(2 * K)[::2])
