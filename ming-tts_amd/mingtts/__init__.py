@@ -605,6 +605,8 @@ def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=Non
         _refuse_kv(kv, B, hkv)
     d = kv.device
     if prefix is None:
+        if prefix_len:
+            raise ValueError(f"prefix_len {prefix_len} without a prefix")
         prefix_len, pre = 0, None
     else:
         if prefix.hkv != hkv:

@@ -146,3 +146,12 @@ def test_vectors(call, name, n):
 def test_a_strided_norm_of_many_rows(rows):
     with pytest.raises(ValueError, match="values"):
         linear(x=z(rows, K), y=z(rows, N), norm=h16(2 * K)[::2])
+
+
+def test_a_prefix_length_without_a_prefix():
+    with pytest.raises(ValueError, match="prefix"):
+        attend(prefix_len=5)
+    one = mt.KV(*[t[0] for t in (caches().k, caches().v, caches().k_scale, caches().v_scale)])
+    for over in (dict(prefix_len=0), dict(prefix=one), dict(prefix=one, prefix_len=5)):
+        with pytest.raises(Reached):
+            attend(**over)
