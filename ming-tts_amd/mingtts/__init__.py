@@ -619,7 +619,10 @@ def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=Non
     src, ldq = _rows(d, q, B * T, hq * 64, ldq)
     dst, ldo = _rows(d, out, B * T, hq * 64, ldo)
     need = _shared_need(B, T, hq, hkv, prefix_len, len_max or kv.cache_len, window, kv.type)
-    if need and workspace is None:
+    if workspace is not None:
+        if workspace.get_device() != d or not workspace.is_contiguous():
+            raise ValueError("the workspace is contiguous and on the caches' device")
+    elif need:
         workspace = _scratch(need, q, stream)
     rc = (_lib or load()).mt_attention_shared(
         src, ldq, B, T, hq, hkv, _slots(d, pos, B), _slots(d, counts, B), kv.ref, pre, prefix_len, len_max, window, dst, ldo,

@@ -155,3 +155,22 @@ def test_a_prefix_length_without_a_prefix():
     for over in (dict(prefix_len=0), dict(prefix=one), dict(prefix=one, prefix_len=5)):
         with pytest.raises(Reached):
             attend(**over)
+
+
+@pytest.mark.parametrize("bad", [z(1 << 21, dtype=torch.uint8)[::2], z(1 << 10, 1 << 12, dtype=torch.uint8)[:, :1 << 11]], ids=["strided", "columns"])
+def test_a_workspace_that_is_not_one_run(bad):
+    with pytest.raises(ValueError, match="workspace"):
+        attend(workspace=bad)
+
+
+def test_a_workspace_on_another_device():
+    """(a host tensor stands for the caches' device here, so this one says that it is elsewhere)"""
+    class Elsewhere(torch.Tensor):
+        def get_device(self):
+            return 1
+
+    with pytest.raises(ValueError, match="workspace"):
+        attend(workspace=z(1 << 20, dtype=torch.uint8).as_subclass(Elsewhere))
+    for good in (z(1 << 20, dtype=torch.uint8), z(1 << 18)):
+        with pytest.raises(Reached):
+            attend(workspace=good)
