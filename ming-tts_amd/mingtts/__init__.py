@@ -672,9 +672,13 @@ class F8Matrix:
 
 
 def quantize_f8(x, out, norm=None, eps=1e-6, stream=None) -> None:
-    """mt_quantize_f8: the rows of x [rows, K], RMS-normalised with gain ``norm`` if given, into an F8Matrix."""
+    """mt_quantize_f8: the rows of x [rows, K], RMS-normalised with gain ``norm`` if given, into an F8Matrix.  The bytes
+    between the rows of strided scales are set to 0, up to the last row's whole stride."""
     if tuple(x.shape) != tuple(out.shape) or x.stride(1) != 1:
         raise ValueError("x and the matrix must be of one shape, x's rows contiguous")
+    s = out.scales
+    if s.storage_offset() + s.shape[0] * s.stride(0) > s.untyped_storage().nbytes():
+        raise ValueError("the scales end before their last row's stride")
     if x.get_device() != out.device or (norm is not None and norm.get_device() != out.device):
         raise ValueError("x, norm and the matrix must be on one device")
     if norm is not None and (norm.numel() < x.shape[1] or not norm.is_contiguous()):

@@ -174,3 +174,16 @@ def test_a_workspace_on_another_device():
     for good in (z(1 << 20, dtype=torch.uint8), z(1 << 18)):
         with pytest.raises(Reached):
             attend(workspace=good)
+
+
+def test_scales_that_end_before_their_last_rows_stride():
+    """mt_quantize_f8 clears a row's bytes up to its stride, the last row's too."""
+    wide = z(N, 8, dtype=torch.uint8)
+    codes = z(N, K, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="stride"):
+        quantize(out=mt.F8Matrix(codes, wide[:, 4:]))
+    with pytest.raises(ValueError, match="stride"):
+        quantize(out=mt.F8Matrix(codes[1:], wide[1:, 4:]), x=z(N - 1, K))
+    for out, n in ((mt.F8Matrix(codes, wide[:, :4]), N), (mt.F8Matrix(codes[1:], wide[:-1, 4:]), N - 1)):
+        with pytest.raises(Reached):
+            quantize(out=out, x=z(n, K))
