@@ -666,7 +666,8 @@ class F8Matrix:
         """mt_quantize_f8 of x [rows, K] into new tensors."""
         import torch
         n, k = x.shape
-        m = F8Matrix(_scratch(n * k, x, stream).view(n, k), _scratch(n * 4 * ((k + 511) // 512), x, stream).view(n, -1))
+        lds = 4 * ((k + 511) // 512)
+        m = F8Matrix(_scratch(n * k, x, stream).view(n, k), _scratch(n * lds, x, stream).view(n, lds))
         quantize_f8(x, m, norm=norm, eps=eps, stream=stream)
         return m
 

@@ -187,3 +187,11 @@ def test_scales_that_end_before_their_last_rows_stride():
     for out, n in ((mt.F8Matrix(codes, wide[:, :4]), N), (mt.F8Matrix(codes[1:], wide[:-1, 4:]), N - 1)):
         with pytest.raises(Reached):
             quantize(out=out, x=z(n, K))
+
+
+def test_a_matrix_of_no_rows(monkeypatch):
+    """Nothing to do, as in the C call."""
+    monkeypatch.setattr(mt, "_on", lambda device, stream: 0)
+    for k in (K, 1024):
+        m = mt.F8Matrix.quantize(z(0, k))
+        assert m.shape == (0, k) and tuple(m.scales.shape) == (0, 4 * ((k + 511) // 512))
