@@ -497,7 +497,7 @@ int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, ui
  * mt_quantize_f8 -- `rows` rows of K values x (type xt, row stride ldx) as a matrix in 8 bits: codes
  * [rows, ldq] and scales [rows, lds], lds >= 4 ceil(K / 512) and a multiple of 4 (the bytes past
  * the row's blocks are set to 0).  With norm ([K] of type nt, as mt_linear_rmsnorm's) the rows are
- * x * rsqrt(mean(x^2) + eps) * norm.  K a multiple of 16; x, norm and codes 16-byte aligned with 16-byte row
+ * x * rsqrt(mean(x^2) + eps) * norm.  K a multiple of 16 up to 2^31, lds up to 2^24; x, norm and codes 16-byte aligned with 16-byte row
  * strides, scales 4-byte aligned.  codes and scales must not overlap x.
  *
  * mt_linear_f8 -- mt_linear with weights in 8 bits: y = epilogue(x w^T), w and the gate partner w2

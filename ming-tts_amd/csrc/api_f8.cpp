@@ -204,6 +204,8 @@ int mt_quantize_f8(const void *x, mt_dtype xt, uint32_t rows, uint32_t K, uint32
     if (norm && !(eps >= 0.0f)) return set_error(MT_EINVAL, "%s: RMSNorm eps must be >= 0", who);
     if (norm && K > 16 * F8_NORM_K) return set_error(MT_EINVAL, "%s: a norm over K %u > %u", who, K, 16 * F8_NORM_K);
     if (K == 0 || K % 16) return set_error(MT_EINVAL, "%s: K must be a positive multiple of 16, got %u", who, K);
+    // A block's first value is 128 times its number: 32 bits hold both.
+    if (K > (1u << 31) || lds > (1u << 24)) return set_error(MT_EINVAL, "%s: K %u past 2^31 or lds %u past 2^24", who, K, lds);
     if (rows == 0) return MT_OK;
     if (rows > 0x7FFFFFFFu || static_cast<uint64_t>(rows) * lds > 0x7FFFFFFFull * 16)
         return set_error(MT_EINVAL, "%s: %u rows of %u blocks are too many", who, rows, lds);
