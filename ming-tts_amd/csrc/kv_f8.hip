@@ -4,7 +4,7 @@
 //
 // Reference kernel replaced: ropeCache (Shaders.swift:451-486), for rows of many sequences.
 //
-//   - Angles: position times frequency is exact in 64 bits, and its turns are taken off there, so a far position
+//   - Angles: position times frequency is exact in 64 bits (up to position 2^29), and its turns are taken off there, so a far position
 //     costs no bits (an fp32 product is off by 2^-24 of the angle: 0.008 radians at position 131072).  Sine,
 //     cosine and rotation stay in 64 bits up to the one rounding into q or the cache: an 8-bit code that an
 //     fp32 rotation's error tips over is off by a whole step of 2^-3 (about one in a million values), and about one in 2^14
