@@ -744,9 +744,11 @@ int launch_kind(const SharedArgs &a, const SharedPlan &p, hipStream_t stream) {
 
 }  // namespace
 
-// Where the work goes.  A CU holds one workgroup of eight waves or three of four (168 registers a lane); eight waves
-// take about 2 us for each 512 keys of their rows, and the second kernel of the split form costs about as much as
-// 1200 keys.
+// Where the work goes, from the sizes alone: 256 compute units are an MI355X's, not asked for, so that a workspace sized once
+// fits wherever the call runs.  A CU holds one workgroup of eight waves, or of four waves three with 8-bit and fp16 caches
+// (at most 168 registers a lane) and two with fp32 ones (184); the rule is measured on 8 bits and used for all three.
+// Eight waves take about 2 us for each 512 keys of their rows, and the second kernel of the split form costs about as much
+// as 1200 keys.
 //   - One row tile (16 rows) a workgroup of eight waves that split its keys, while that fills at most every CU once: 4
 //     sequences of 40 rows over 500 + 300 keys (144 workgroups) 8.8 us, with two tiles a workgroup 13.2, four 19.4.
 //   - More row tiles: four waves a tile, and two or four tiles a workgroup only where that would leave a wave less
@@ -757,6 +759,10 @@ int launch_kind(const SharedArgs &a, const SharedPlan &p, hipStream_t stream) {
 //     longest workgroup then costs less than the longest in one pass.  Measured, one pass against apart: 64 sequences
 //     of up to 4096 keys 21.0 against 16.2 us, 128 of them 20.8 against 26, 16 sequences over 8192 + 512 keys
 //     36.5 against 11.5, 128 over 2048 + 512 14.9 against 14.7, 256 over 4096 + 1024 47 against 29.3.
+// What the estimate does not see: parts are whole, and a key costs the same whether 7 or 16 rows of a tile use it.  So the choice
+// is not steady where the two forms cost about the same: over 2048 + 512 keys up to 64 sequences share the prefix, 96 and 128 do
+// not, 129 to 160 do, 192 to 256 do not.  Row tiles of many rows (the second rule) never share it; only one row a sequence and
+// prompts were measured there, nothing between.
 SharedPlan shared_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t prefix_len, uint32_t len_max, uint32_t window,
                        int ct) {
     const uint64_t tk = ct == DT_F32 ? Raw<DT_F32>::TK : Raw<DT_F8>::TK, cus = 256;

@@ -10,7 +10,7 @@
 //   - A buffer descriptor ends with the tile's rows and the loads of chunks past K are out of its bounds: both read as zeros,
 //     no branch in the loop.
 //   - Bound: the MFMAs (54 % busy at 4096^3), the conversions beside them (3 vector instructions an MFMA) and a barrier a stage.
-//     4096 x 4096 x 4096: 109-117 us a launch, depending on the box, 1.17-1.26 PFLOP/s; the library's bf16 product of that size
+//     4096 x 4096 x 4096: 109-117 us a launch, depending on the machine, 1.17-1.26 PFLOP/s; the library's bf16 product of that size
 //     takes 98 us (1.40) here.  Without the conversions 106, without the LDS reads 96, without the global loads 96; raised
 //     priority for the MFMAs, fixed orders of conversions and MFMAs, deeper pipelines of smaller stages all came out slower.
 #pragma once

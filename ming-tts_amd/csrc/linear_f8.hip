@@ -200,8 +200,8 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(F8LinearArgs a, int bt) 
     }
 
     f32x4v acc = {0.f, 0.f, 0.f, 0.f}, acc2 = acc;
-    // A block's loads are issued as soon as the registers of the block before are converted, so a wave with several
-    // blocks waits for memory once.
+    // A block's loads are issued as soon as the registers of the block before are converted: one round trip to memory a
+    // block, each begun before the products of the block ahead of it (a wave has one block up to K 2048, three at K 4864).
     RowCodes w, u, xc;
     float v[4][8];
     auto load_w = [&](uint32_t kb) {
