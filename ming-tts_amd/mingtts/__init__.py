@@ -508,8 +508,9 @@ def _refuse_kv(kv, B, hkv):
 
 
 def _rows(device, t, rows, width, ld=None):
-    """The address and row stride of `rows` fp32 rows of `width` values: a tensor [rows, width] or larger (leading
-    dimensions count as one where they can), or any tensor that holds them at a stride `ld` from its first element on."""
+    """The address and row stride of `rows` fp32 rows of `width` values: a tensor [rows, width] or larger (several
+    dimensions count as one where they can, before the rows' values and in them), or any tensor that holds them at a
+    stride `ld` from its first element on."""
     if t.dtype is not _row_type or t.get_device() != device:
         raise ValueError("activations are fp32, on the caches' or weights' device")
     if ld is None:
@@ -527,10 +528,15 @@ def _rows(device, t, rows, width, ld=None):
 def _folded_rows(device, t, rows, width):
     if rows == 0:
         return t.data_ptr(), width
-    if t.dim() > 2:
+    if t.dim() > 2 and t.numel():
+        w = 1  # the last dimensions that hold a row
+        for n in reversed(t.shape):
+            w *= n
+            if w >= width:
+                break
         try:
-            return _rows(device, t.view(-1, t.shape[-1]), rows, width)
-        except RuntimeError:  # leading dimensions that are not one
+            return _rows(device, t.view(-1, w), rows, width)
+        except RuntimeError:  # dimensions that are not one
             pass
     raise ValueError(f"not {rows} rows of {width} values side by side: {tuple(t.shape)} at strides {t.stride()}")
 

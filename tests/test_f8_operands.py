@@ -195,3 +195,17 @@ def test_a_matrix_of_no_rows(monkeypatch):
     for k in (K, 1024):
         m = mt.F8Matrix.quantize(z(0, k))
         assert m.shape == (0, k) and tuple(m.scales.shape) == (0, 4 * ((k + 511) // 512))
+
+
+@pytest.mark.parametrize("call,name,rows,width", ROWS)
+def test_rows_of_several_dimensions(call, name, rows, width):
+    """Heads as a dimension of their own, slices of wider rows, both with leading dimensions of their own."""
+    h = width // 8
+    wide = z(2, rows // 2, 12, h)
+    for t in (z(rows, 8, h), z(2, rows // 2, 8, h), wide[:, :, :8], wide[:, :, 4:], z(rows, 12, h)[:, 2:10], z(rows, 1, 8, h)):
+        with pytest.raises(Reached):
+            call(**{name: t})
+    for t in (z(rows, 7, h), z(rows, 8, 2 * h)[:, :, :h], z(rows, h, 8).transpose(1, 2), z(8, rows, h).transpose(0, 1), z(rows - 1, 8, h),
+              z(rows, 0, h)):
+        with pytest.raises(ValueError, match="rows of"):
+            call(**{name: t})
