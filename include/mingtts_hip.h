@@ -494,6 +494,66 @@ int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, ui
                         mt_stream_t stream);
 
 /*
+ * Caches in pages, and windows that keep the first positions in sight.  No counterpart in the reference.
+ *
+ * mt_paged_kv -- the caches of one layer for many sequences as pages of one pool: k and v [pages, hkv, page_len, 64] of type
+ * cache_t (MT_F32, MT_F16 or MT_F8), 16-byte aligned, each page `stride` elements behind the one before (a multiple of 16);
+ * with MT_F8 also k_scale and v_scale [pages, hkv, page_len] bytes, 4-byte aligned, scale_stride bytes a page (a multiple of 4).
+ * Slot s of sequence b is row s % page_len of page table[b table_stride + s / page_len] (device, uint32; table_len entries a
+ * sequence, so it has table_len page_len slots, at most 2^30; table_stride is not read for one sequence).  page_len is a multiple
+ * of 16 up to 32768.  An entry of `pages` or more (0xFFFFFFFF, say) is no page: nothing is read or written for its slots.  Entries
+ * of slots that a call neither writes nor attends are not read for anything but that.  Several entries may name one page, such as
+ * a prompt that many sequences share; a page that one call appends to through two entries holds either's rows.  k, v and the
+ * scales overlap neither each other nor the table; with one stride (in bytes) they may lie between each other, a page's keys and
+ * values side by side.  B sequences of T rows, pos and counts are as at mt_kv.
+ *
+ * mt_rope_append_paged -- mt_rope_append into such caches: the same rotation and rounding, so the same bits.  A slot past
+ * the table or without a page appends nothing (the query heads are still rotated).
+ */
+typedef struct mt_paged_kv {
+    void *k;
+    void *v;
+    uint8_t *k_scale;
+    uint8_t *v_scale;
+    uint64_t stride;
+    uint64_t scale_stride;
+    const uint32_t *table;
+    uint32_t pages;
+    uint32_t page_len;
+    uint32_t table_len;
+    uint32_t table_stride;
+    int32_t cache_t; /* mt_dtype */
+} mt_paged_kv;
+
+int mt_rope_append_paged(const float *qkv, uint32_t ldq, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, const uint32_t *pos,
+                         const uint32_t *counts, uint32_t offset, const mt_paged_kv *kv, const float *inv_freq, float *q,
+                         uint32_t ldo, mt_stream_t stream);
+
+/*
+ * mt_attention_paged, mt_attention_sinks -- grouped-query attention of the rows over their sequence's own keys, in pages or in
+ * contiguous caches: row t of sequence b, at slot i = pos[b] + t (or the cache's last where that is past it), attends slots j <= i,
+ * and where a window is given those of them with j > i - window or j < sinks (window 0 = all; then sinks has no effect).  So a
+ * stream that runs past its window keeps its first positions, a voice prompt say, in sight, and the pages between them
+ * and the window can be given back: their entries are not read.  q rows (stride ldq) hold hq heads of 64,
+ * already rotated; out rows stride ldo; scores scaled by `scale`, max-subtracted softmax; q and out 16-byte aligned with 16-byte
+ * row strides, out apart from q and the caches.  Slots that a row does not attend do not reach its result, whatever they hold; nor do
+ * slots without a page.  A NaN or +infinity among the scores that it does attend makes its head NaN; a score of -infinity is no
+ * weight; a head without any weight is zeros.
+ *
+ * len_max (the caller's bound on max(pos[b] + counts[b]); 0: all slots) and the workspace are as at mt_attention_shared: len_max
+ * only places the work, the workspace holds nothing between calls, and calls that may overlap need one each.  The workspace is
+ * sized for the caches' type and the same B, T, hq, hkv, len_max (0: the number of slots), window and sinks.
+ */
+uint64_t mt_attention_window_workspace(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window,
+                                       uint32_t sinks, mt_dtype cache_t);
+int mt_attention_paged(const float *q, uint32_t ldq, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, const uint32_t *pos,
+                       const uint32_t *counts, const mt_paged_kv *kv, uint32_t len_max, uint32_t window, uint32_t sinks, float *out,
+                       uint32_t ldo, float scale, void *workspace, uint64_t workspace_bytes, mt_stream_t stream);
+int mt_attention_sinks(const float *q, uint32_t ldq, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, const uint32_t *pos,
+                       const uint32_t *counts, const mt_kv *kv, uint32_t len_max, uint32_t window, uint32_t sinks, float *out,
+                       uint32_t ldo, float scale, void *workspace, uint64_t workspace_bytes, mt_stream_t stream);
+
+/*
  * mt_quantize_f8 -- `rows` rows of K values x (type xt, row stride ldx) as a matrix in 8 bits: codes
  * [rows, ldq] and scales [rows, lds], lds >= 4 ceil(K / 512) and a multiple of 4 (the bytes past
  * the row's blocks are set to 0).  With norm ([K] of type nt, as mt_linear_rmsnorm's) the rows are

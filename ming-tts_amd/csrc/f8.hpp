@@ -93,6 +93,34 @@ struct RowsArgs {
     }
 };
 
+// Caches in pages (mt_paged_kv), or, without a table, contiguous ones (mt_kv) as one page a sequence.
+struct PagedArgs {
+    void *k, *v;
+    uint8_t *ks, *vs;
+    uint64_t stride, sstride;  // elements and scale bytes from page to page
+    const uint32_t *table;
+    uint32_t pages, page_len;  // page_len without a table: the cache's slots
+    uint32_t len, table_stride;  // slots and entries of a sequence
+    uint64_t page_magic;         // 2^37 / (page_len / 16) + 1
+
+    // The entry of slot `s`: s / page_len = (s / 16) / (page_len / 16), both whole numbers, the second at most 2^11.  The product
+    // of s / 16 < 2^26 with the magic number, off by at most 2^11 2^-37 of itself, stays below 2^64 and its quotient exact.
+    __host__ __device__ __forceinline__ uint32_t entry(uint32_t s) const {
+        return static_cast<uint32_t>(((s >> 4) * page_magic) >> 37);
+    }
+};
+
+// The operands of mt_attention_paged and mt_attention_sinks.
+struct WindowArgs {
+    const float *q;
+    float *out;
+    uint32_t ldq, ldo, hq, hkv, window, sinks;
+    RowsArgs rows;
+    PagedArgs kv;
+    float scale;
+    uint32_t group, group_magic;  // as in SharedArgs
+};
+
 // How mt_attention_shared places its work (shared_plan).
 struct SharedPlan {
     uint32_t waves;     // of a workgroup

@@ -1,6 +1,6 @@
-// The caches' writers: RoPE and append of new rows (mt_rope_append) and the copy of positions from
-// one cache to another (mt_kv_copy), for caches of fp32, fp16 and 8 bits (f8.hpp: a block is the 64
-// values of one head at one position).
+// The caches' writers: RoPE and append of new rows into contiguous caches (mt_rope_append) and into pages
+// (mt_rope_append_paged), and the copy of positions from one cache to another (mt_kv_copy), for caches of fp32, fp16 and
+// 8 bits (f8.hpp: a block is the 64 values of one head at one position).
 //
 // Reference kernel replaced: ropeCache (Shaders.swift:451-486), for rows of many sequences.
 //
@@ -70,9 +70,27 @@ __device__ __forceinline__ void store_row(const float *x, void *cache, uint8_t *
     }
 }
 
-template <int CT>
+// Where the rows of slot `slot` of sequence b stand: the first key head's row and scale, in elements and bytes from the
+// caches' start, and the rows from one key head to the next; false: nowhere.
+struct Place {
+    uint64_t row, scale;
+    uint32_t step;
+};
+__device__ __forceinline__ bool place(const KvArgs &kv, uint32_t b, uint64_t slot, Place &p) {
+    p = Place{b * kv.stride + slot * 64, b * kv.sstride + slot, kv.len};
+    return slot < kv.len;
+}
+__device__ __forceinline__ bool place(const PagedArgs &kv, uint32_t b, uint64_t slot, Place &p) {
+    if (slot >= kv.len) return false;
+    const uint32_t s = static_cast<uint32_t>(slot), e = kv.entry(s), in = s - e * kv.page_len;
+    const uint32_t page = kv.table[static_cast<size_t>(b) * kv.table_stride + e];
+    p = Place{page * kv.stride + in * 64, page * kv.sstride + in, kv.page_len};
+    return page < kv.pages;
+}
+
+template <int CT, class KV>
 __global__ __launch_bounds__(KV_THREADS) void rope_append_kernel(const float *qkv, uint32_t ldq, RowsArgs rows, uint32_t hq,
-                                                                 uint32_t hkv, uint32_t offset, KvArgs kv,
+                                                                 uint32_t hkv, uint32_t offset, KV kv,
                                                                  const float *inv_freq, float *q, uint32_t ldo,
                                                                  uint32_t per_group) {
     __shared__ double2 cs[KV_ROWS][32];
@@ -92,7 +110,8 @@ __global__ __launch_bounds__(KV_THREADS) void rope_append_kernel(const float *qk
         uint64_t slot;
         if (!rows.at(row, b, slot)) continue;
         const bool is_q = h < hq;
-        if (is_q ? q == nullptr : slot >= kv.len) continue;
+        Place at;
+        if (is_q ? q == nullptr : !place(kv, b, slot, at)) continue;
         const float *src = qkv + static_cast<size_t>(row) * ldq + h * 64 + 4 * r;
         const float4 lo = *reinterpret_cast<const float4 *>(src), hi = *reinterpret_cast<const float4 *>(src + 32);
         float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
@@ -113,12 +132,11 @@ __global__ __launch_bounds__(KV_THREADS) void rope_append_kernel(const float *qk
             *reinterpret_cast<float4 *>(dst + 32) = make_float4(x[4], x[5], x[6], x[7]);
         } else {
             const bool is_k = h < hq + hkv;
-            const uint32_t kh = is_k ? h - hq : h - hq - hkv;
-            const size_t at = static_cast<size_t>(kh) * kv.len + slot;
+            const size_t kh = is_k ? h - hq : h - hq - hkv;
             constexpr size_t ES = CT == DT_F32 ? 4 : CT == DT_F16 ? 2 : 1;
-            char *cache = static_cast<char *>(is_k ? kv.k : kv.v) + b * kv.stride * ES;
-            uint8_t *scales = CT == DT_F8 ? (is_k ? kv.ks : kv.vs) + b * kv.sstride : nullptr;
-            store_row<CT>(x, cache, scales, at, 4 * r, 32 + 4 * r, r);
+            char *cache = static_cast<char *>(is_k ? kv.k : kv.v) + at.row * ES;
+            uint8_t *scales = CT == DT_F8 ? (is_k ? kv.ks : kv.vs) + at.scale : nullptr;
+            store_row<CT>(x, cache, scales, kh * at.step, 4 * r, 32 + 4 * r, r);
         }
     }
 }
@@ -177,26 +195,37 @@ void copy_from(const KvArgs &src, const KvArgs &dst, int dt, const RowsArgs &row
         hipLaunchKernelGGL((kv_copy_kernel<ST, DT_F8>), grid, dim3(KV_THREADS), 0, stream, src, dst, rows, hkv);
 }
 
-}  // namespace
-
-int launch_rope_append(const float *qkv, uint32_t ldq, const RowsArgs &rows, uint32_t hq, uint32_t hkv, uint32_t offset,
-                       const KvArgs &kv, int ct, const float *inv_freq, float *q, uint32_t ldo, hipStream_t stream) {
+template <class KV>
+int launch_append(const char *what, const float *qkv, uint32_t ldq, const RowsArgs &rows, uint32_t hq, uint32_t hkv, uint32_t offset,
+                  const KV &kv, int ct, const float *inv_freq, float *q, uint32_t ldo, hipStream_t stream) {
     const uint32_t all = rows.B * rows.T;
     // One row a workgroup while that leaves CUs free, else the rows that share the angles' set-up.
     const uint32_t per = all <= 512 ? 1 : KV_ROWS;
     const dim3 grid((all + per - 1) / per);
-    const int rc = check_grid("rope append", grid.x, KV_THREADS);
+    const int rc = check_grid(what, grid.x, KV_THREADS);
     if (rc) return rc;
     if (ct == DT_F32)
-        hipLaunchKernelGGL(rope_append_kernel<DT_F32>, grid, dim3(KV_THREADS), 0, stream, qkv, ldq, rows, hq, hkv, offset, kv,
+        hipLaunchKernelGGL((rope_append_kernel<DT_F32, KV>), grid, dim3(KV_THREADS), 0, stream, qkv, ldq, rows, hq, hkv, offset, kv,
                            inv_freq, q, ldo, per);
     else if (ct == DT_F16)
-        hipLaunchKernelGGL(rope_append_kernel<DT_F16>, grid, dim3(KV_THREADS), 0, stream, qkv, ldq, rows, hq, hkv, offset, kv,
+        hipLaunchKernelGGL((rope_append_kernel<DT_F16, KV>), grid, dim3(KV_THREADS), 0, stream, qkv, ldq, rows, hq, hkv, offset, kv,
                            inv_freq, q, ldo, per);
     else
-        hipLaunchKernelGGL(rope_append_kernel<DT_F8>, grid, dim3(KV_THREADS), 0, stream, qkv, ldq, rows, hq, hkv, offset, kv,
+        hipLaunchKernelGGL((rope_append_kernel<DT_F8, KV>), grid, dim3(KV_THREADS), 0, stream, qkv, ldq, rows, hq, hkv, offset, kv,
                            inv_freq, q, ldo, per);
-    return check_launch("rope append");
+    return check_launch(what);
+}
+
+}  // namespace
+
+int launch_rope_append(const float *qkv, uint32_t ldq, const RowsArgs &rows, uint32_t hq, uint32_t hkv, uint32_t offset,
+                       const KvArgs &kv, int ct, const float *inv_freq, float *q, uint32_t ldo, hipStream_t stream) {
+    return launch_append("rope append", qkv, ldq, rows, hq, hkv, offset, kv, ct, inv_freq, q, ldo, stream);
+}
+
+int launch_rope_append_paged(const float *qkv, uint32_t ldq, const RowsArgs &rows, uint32_t hq, uint32_t hkv, uint32_t offset,
+                             const PagedArgs &kv, int ct, const float *inv_freq, float *q, uint32_t ldo, hipStream_t stream) {
+    return launch_append("rope append paged", qkv, ldq, rows, hq, hkv, offset, kv, ct, inv_freq, q, ldo, stream);
 }
 
 int launch_kv_copy(const KvArgs &src, int st, const KvArgs &dst, int dt, const RowsArgs &rows, uint32_t hkv, hipStream_t stream) {

@@ -34,7 +34,8 @@ EXPORTS = (
     "mt_seq_destroy", "mt_seq_groups", "mt_seq_kernel", "mt_seq_check", "mt_rope_cache", "mt_rope_cache_decode",
     "mt_attention", "mt_attention_decode", "mt_rope_attention", "mt_dit_attention", "mt_dit_attention_linear", "mt_flow_assemble",
     "mt_flow_euler", "mt_flow_euler_assemble", "mt_rope_append", "mt_kv_copy", "mt_attention_shared",
-    "mt_attention_shared_workspace", "mt_quantize_f8", "mt_linear_f8",
+    "mt_attention_shared_workspace", "mt_rope_append_paged", "mt_attention_window_workspace", "mt_attention_paged",
+    "mt_attention_sinks", "mt_quantize_f8", "mt_linear_f8",
     "mt_upsample4", "mt_istft_frames", "mt_istft_emit", "mt_st_open", "mt_st_close", "mt_st_count", "mt_st_name", "mt_st_find", "mt_arena_create", "mt_arena_tensor",
     "mt_arena_padded", "mt_arena_bytes", "mt_arena_upload", "mt_arena_audit", "mt_arena_destroy",
     "mt_last_error", "mt_version",
@@ -102,6 +103,14 @@ class KvStruct(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
                 ("v_scale", ctypes.c_void_p), ("stride", ctypes.c_uint64), ("scale_stride", ctypes.c_uint64),
                 ("cache_len", ctypes.c_uint32), ("cache_t", ctypes.c_int32)]
+
+
+class PagedKvStruct(ctypes.Structure):
+    """mt_paged_kv: the caches of one layer as pages of one pool."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("stride", ctypes.c_uint64), ("scale_stride", ctypes.c_uint64),
+                ("table", ctypes.c_void_p), ("pages", ctypes.c_uint32), ("page_len", ctypes.c_uint32),
+                ("table_len", ctypes.c_uint32), ("table_stride", ctypes.c_uint32), ("cache_t", ctypes.c_int32)]
 
 
 class StEntry(ctypes.Structure):
@@ -184,6 +193,15 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     L.mt_attention_shared_workspace.restype = u64
     L.mt_attention_shared.argtypes = [vp, u32, u32, u32, u32, u32, vp, vp, kv, kv, u32, u32, u32, vp, u32, f32, vp, u64, vp]
     L.mt_attention_shared.restype = i32
+    paged = ctypes.POINTER(PagedKvStruct)
+    L.mt_rope_append_paged.argtypes = [vp, u32, u32, u32, u32, u32, vp, vp, u32, paged, vp, vp, u32, vp]
+    L.mt_rope_append_paged.restype = i32
+    L.mt_attention_window_workspace.argtypes = [u32, u32, u32, u32, u32, u32, u32, i32]
+    L.mt_attention_window_workspace.restype = u64
+    L.mt_attention_paged.argtypes = [vp, u32, u32, u32, u32, u32, vp, vp, paged, u32, u32, u32, vp, u32, f32, vp, u64, vp]
+    L.mt_attention_paged.restype = i32
+    L.mt_attention_sinks.argtypes = [vp, u32, u32, u32, u32, u32, vp, vp, kv, u32, u32, u32, vp, u32, f32, vp, u64, vp]
+    L.mt_attention_sinks.restype = i32
     L.mt_quantize_f8.argtypes = [vp, i32, u32, u32, u32, vp, i32, f32, vp, u32, vp, u32, vp]
     L.mt_quantize_f8.restype = i32
     L.mt_linear_f8.argtypes = [vp, i32, vp, u32, vp, vp, vp, vp, vp, vp, i32, vp, GemvParams, vp]
@@ -636,6 +654,112 @@ def attention_shared(q, B, T, hq, hkv, pos, kv, out, prefix=None, prefix_len=Non
         0 if workspace is None else workspace.numel() * workspace.element_size(), _on(d, stream))
     if rc < 0:
         check(rc)
+
+
+class PagedKV:
+    """The caches of one layer as pages of one pool (mt_paged_kv): k and v torch tensors [pages, hkv, page_len, 64], fp32, fp16
+    or 8-bit codes (uint8 or float8_e4m3fn), page_len a multiple of 16; 8-bit caches have scale bytes k_scale and v_scale
+    [pages, hkv, page_len].  A page is contiguous; the pages may be strided, the same way for k and v (and for both scales).
+    table [B, entries] (int32 or uint32, a sequence's entries side by side): slot s of sequence b is row s % page_len of
+    page table[b, s // page_len]; -1 or any number past the pool is no page.  The caller changes the table in place as
+    sequences grow and end."""
+
+    def __init__(self, k, v, table, k_scale=None, v_scale=None):
+        t = _storage_code(k)
+        for name, x, y, inner in (("k and v", k, v, 3), ("k_scale and v_scale", k_scale, v_scale, 2)):
+            if inner == 2 and t != F8:
+                continue
+            if x is None or y is None or x.shape != y.shape or x.dtype != y.dtype or x.stride() != y.stride():
+                raise ValueError(f"{name} must be two tensors of one shape, type and layout")
+            if x.dim() != inner + 1 or x.shape[0] == 0 or not x[0].is_contiguous():
+                raise ValueError(f"{name}: [pages, hkv, page_len{', 64' if inner == 3 else ''}], contiguous but for the pages")
+        if k.shape[-1] != 64 or t == BF16:
+            raise ValueError("caches hold heads of 64 fp32, fp16 or 8-bit values")
+        if t == F8 and (k_scale.shape != k.shape[:-1] or k_scale.element_size() != 1):
+            raise ValueError("one scale byte a head and position")
+        if table.dim() != 2 or table.dtype not in _slot_types or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError("table: [B, entries] int32, a sequence's entries side by side")
+        if any(x is not None and x.device != k.device for x in (v, table, k_scale, v_scale)):
+            raise ValueError("caches, scales and table must be on one device")
+        self.k, self.v, self.k_scale, self.v_scale, self.table = k, v, k_scale, v_scale, table
+        self.hkv, self.page_len, self.type = k.shape[1], k.shape[2], t
+        self.batch, entries = table.shape
+        self.cache_len = entries * self.page_len  # slots of a sequence
+        self.device = k.get_device()
+        one = k.shape[0] == 1  # (a stride that torch does not keep)
+        self.struct = PagedKvStruct(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), k[0].numel() if one else k.stride(0),
+                                    0 if t != F8 else k_scale[0].numel() if one else k_scale.stride(0), _ptr(table),
+                                    k.shape[0], self.page_len, entries, table.stride(0), t)
+        self.ref = ctypes.byref(self.struct)
+
+    @staticmethod
+    def empty(pages, hkv, page_len, table, dtype):
+        """Zeroed pages of torch type ``dtype`` (uint8: 8 bits) on the table's device."""
+        import torch
+        k = torch.zeros(pages, hkv, page_len, 64, dtype=dtype, device=table.device)
+        if _storage_code(k) != F8:
+            return PagedKV(k, torch.zeros_like(k), table)
+        s = torch.ones(pages, hkv, page_len, dtype=torch.uint8, device=table.device)
+        return PagedKV(k, torch.zeros_like(k), table, s, torch.ones_like(s))
+
+
+def rope_append_paged(qkv, B, T, hq, hkv, pos, kv, inv_freq, q=None, counts=None, offset=0, ldq=None, ldo=None,
+                      stream=None) -> None:
+    """mt_rope_append_paged: rope_append into the pages of ``kv`` (a PagedKV)."""
+    if kv.__class__ is not PagedKV:
+        raise ValueError("rope_append_paged takes a PagedKV")
+    if kv.hkv != hkv or kv.batch < B:
+        _refuse_kv(kv, B, hkv)
+    d = kv.device
+    src, ldq = _rows(d, qkv, B * T, (hq + 2 * hkv) * 64, ldq)
+    dst, ldo = (None, 0) if q is None else _rows(d, q, B * T, hq * 64, ldo)
+    rc = (_lib or load()).mt_rope_append_paged(src, ldq, B, T, hq, hkv, _slots(d, pos, B), _slots(d, counts, B), offset, kv.ref,
+                                               _frequencies(d, inv_freq), dst, ldo, _on(d, stream))
+    if rc < 0:
+        check(rc)
+
+
+@functools.lru_cache(maxsize=4096)
+def _window_need(*sizes) -> int:
+    """mt_attention_window_workspace: the sizes alone decide."""
+    return load().mt_attention_window_workspace(*sizes)
+
+
+def _attend_window(call, kind, q, B, T, hq, hkv, pos, kv, out, len_max, window, sinks, counts, scale, ldq, ldo, workspace, stream):
+    if kv.__class__ is not kind:
+        raise ValueError(f"takes a {kind.__name__}")
+    if kv.hkv != hkv or kv.batch < B:
+        _refuse_kv(kv, B, hkv)
+    d = kv.device
+    src, ldq = _rows(d, q, B * T, hq * 64, ldq)
+    dst, ldo = _rows(d, out, B * T, hq * 64, ldo)
+    need = _window_need(B, T, hq, hkv, len_max or kv.cache_len, window, sinks, kv.type)
+    if workspace is not None:
+        if workspace.get_device() != d or not workspace.is_contiguous():
+            raise ValueError("the workspace is contiguous and on the caches' device")
+    elif need:
+        workspace = _scratch(need, q, stream)
+    rc = call(src, ldq, B, T, hq, hkv, _slots(d, pos, B), _slots(d, counts, B), kv.ref, len_max, window, sinks, dst, ldo, scale,
+              None if workspace is None else workspace.data_ptr(),
+              0 if workspace is None else workspace.numel() * workspace.element_size(), _on(d, stream))
+    if rc < 0:
+        check(rc)
+
+
+def attention_paged(q, B, T, hq, hkv, pos, kv, out, len_max=0, window=0, sinks=0, counts=None, scale=0.125, ldq=None, ldo=None,
+                    workspace=None, stream=None) -> None:
+    """mt_attention_paged: the rows' attention over the pages of ``kv`` (a PagedKV) up to their slot; with a window, over its last
+    ``window`` slots and the first ``sinks``.  The workspace, where the split of the keys needs one, comes from torch's
+    allocator (so a captured graph keeps its own) unless given as a uint8 tensor."""
+    _attend_window((_lib or load()).mt_attention_paged, PagedKV, q, B, T, hq, hkv, pos, kv, out, len_max, window, sinks, counts,
+                   scale, ldq, ldo, workspace, stream)
+
+
+def attention_sinks(q, B, T, hq, hkv, pos, kv, out, len_max=0, window=0, sinks=0, counts=None, scale=0.125, ldq=None, ldo=None,
+                    workspace=None, stream=None) -> None:
+    """mt_attention_sinks: attention_paged over the contiguous caches of ``kv`` (a KV)."""
+    _attend_window((_lib or load()).mt_attention_sinks, KV, q, B, T, hq, hkv, pos, kv, out, len_max, window, sinks, counts,
+                   scale, ldq, ldo, workspace, stream)
 
 
 def _scratch(nbytes, like, stream):
