@@ -58,6 +58,11 @@ struct PagedRuns {
     }
 };
 
+// The workspace of a plan: its parts' sums of 64, maxima and weights' sums.
+uint64_t window_bytes(const WindowPlan &p, uint32_t B, uint32_t T, uint32_t hq) {
+    return p.parts > 1 ? static_cast<uint64_t>(B) * T * hq * p.parts * (64 + 2) * 4 : 0;
+}
+
 // What mt_attention_paged and mt_attention_sinks check alike, behind their caches: `a` has those, `caches` their memory.
 int attend(const char *who, WindowArgs &a, int ct, const Runs *caches, int n_caches, const float *q, uint32_t ldq, uint32_t B, uint32_t T,
            uint32_t hq, uint32_t hkv, const uint32_t *pos, const uint32_t *counts, uint32_t len_max, uint32_t window,
@@ -71,7 +76,8 @@ int attend(const char *who, WindowArgs &a, int ct, const Runs *caches, int n_cac
     if (meet(q, span(all, w, ldq, 4), out, ob)) return set_error(MT_EINVAL, "%s: out overlaps q", who);
     for (int i = 0; i < n_caches; i++)
         if (meet(caches[i].p, caches[i].all(), out, ob)) return set_error(MT_EINVAL, "%s: out overlaps the caches", who);
-    const uint64_t need = mt_attention_window_workspace(B, T, hq, hkv, len_max ? len_max : a.kv.len, window, sinks, static_cast<mt_dtype>(ct));
+    const WindowPlan plan = window_plan(B, T, hq, hkv, len_max ? len_max : a.kv.len, window, sinks, ct);
+    const uint64_t need = window_bytes(plan, B, T, hq);
     if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return set_error(MT_EINVAL, "%s: needs %llu bytes of 16-byte aligned workspace, got %llu", who,
                          static_cast<unsigned long long>(need), static_cast<unsigned long long>(workspace ? workspace_bytes : 0));
@@ -87,7 +93,8 @@ int attend(const char *who, WindowArgs &a, int ct, const Runs *caches, int n_cac
     a.scale = scale;
     a.group = hq / hkv;
     a.group_magic = static_cast<uint32_t>((1ull << 32) / a.group + 1);
-    return launch_attention_window(a, ct, reinterpret_cast<hipStream_t>(stream));
+    a.part = static_cast<float *>(workspace);
+    return launch_attention_window(a, plan, ct, reinterpret_cast<hipStream_t>(stream));
 }
 
 int validate_heads(const char *who, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv) {
@@ -133,7 +140,7 @@ int mt_rope_append_paged(const float *qkv, uint32_t ldq, uint32_t B, uint32_t T,
 uint64_t mt_attention_window_workspace(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window,
                                        uint32_t sinks, mt_dtype cache_t) {
     if (validate_heads("mt_attention_window_workspace", B, T, hq, hkv) || B == 0 || T == 0) return 0;
-    return 0;
+    return window_bytes(window_plan(B, T, hq, hkv, len_max, window, sinks, cache_t), B, T, hq);
 }
 
 int mt_attention_paged(const float *q, uint32_t ldq, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, const uint32_t *pos,

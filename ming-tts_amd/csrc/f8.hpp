@@ -118,7 +118,17 @@ struct WindowArgs {
     RowsArgs rows;
     PagedArgs kv;
     float scale;
+    float *part;    // split keys: [B T, hq, parts] sums of 64 and behind them as many pairs (minus the maximum, the weights' sum)
+    uint32_t parts, run;  // parts of a row tile's keys, and the key tiles of each (the last: all that is left)
+    uint32_t keys;        // waves of a workgroup that share rows and split their keys (the rest: other rows)
+    uint32_t seq_tiles;   // row tiles of a sequence and key head
     uint32_t group, group_magic;  // as in SharedArgs
+};
+
+// How mt_attention_paged and mt_attention_sinks place their work (window_plan).
+struct WindowPlan {
+    uint32_t waves, keys;  // waves of a workgroup, those that share rows and split their keys
+    uint32_t parts, run;   // parts of 1: one pass; more: joined by a second kernel
 };
 
 // How mt_attention_shared places its work (shared_plan).

@@ -200,7 +200,9 @@ int launch_attention_shared(const SharedArgs &a, const SharedPlan &p, int ct, hi
 // The same into pages, and attention over pages or contiguous caches in a window.
 int launch_rope_append_paged(const float *qkv, uint32_t ldq, const RowsArgs &rows, uint32_t hq, uint32_t hkv, uint32_t offset,
                              const PagedArgs &kv, int ct, const float *inv_freq, float *q, uint32_t ldo, hipStream_t stream);
-int launch_attention_window(const WindowArgs &a, int ct, hipStream_t stream);
+struct WindowPlan;
+WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window, uint32_t sinks, int ct);
+int launch_attention_window(const WindowArgs &a, const WindowPlan &p, int ct, hipStream_t stream);
 int launch_quantize_f8(const void *x, int xt, uint32_t rows, uint32_t K, uint32_t ldx, const uint16_t *norm, int nt, float eps,
                        uint8_t *codes, uint32_t ldq, uint8_t *scales, uint32_t lds, hipStream_t stream);
 int launch_linear_f8(const F8LinearArgs &a, int xt, int bt, hipStream_t stream);
