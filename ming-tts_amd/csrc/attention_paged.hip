@@ -7,6 +7,7 @@
 //   - One wave a row and query head: 64 keys at a time, each lane a key's score, then each lane a dim's sum, an online softmax
 //     in fp32.
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "attend_tiles.hpp"
@@ -86,7 +87,10 @@ __device__ __forceinline__ void attend_wave(const WindowArgs &a, uint32_t b, uin
 
 // ---------------------------------------------------------------- matrix cores --
 
-constexpr uint32_t AW_WAVES = 8, AW_FEW = 4;  // waves of a workgroup
+// v / G (WindowArgs)
+__device__ __forceinline__ uint32_t by_group(const WindowArgs &a, uint32_t v) {
+    return a.group == 1 ? v : __umulhi(v, a.group_magic);
+}
 
 // The key tiles of a row tile: those of the first keys, then those of the window (one run where they touch).
 struct Tiles {
@@ -111,64 +115,178 @@ __device__ __forceinline__ Tiles tiles_of(const WindowArgs &a, uint32_t b, uint3
     return t;
 }
 
-// A tile of keys in pieces of `LEN` slots, each within one page: where each stands, and how many of its slots some row may see.
-template <int PIECES>
-struct Pieces {
-    uint64_t row[PIECES], scale[PIECES];  // as in find()
-    uint32_t n[PIECES];
-    uint32_t none;  // bit i: piece i has no page
+// Where a run of LEN slots within one page stands: bytes from the caches' (and scales') start, and how many of its slots some row may
+// see.  A wave holds 64 of them, a lane each, made at once: what a tile needs are lane reads and additions (address arithmetic a
+// tile, on scalars, was 280 scalar instructions a tile beside 210 vector ones).
+struct Spans {
+    uint32_t lo, hi, n, scale_lo, scale_hi;
+    uint64_t holes;  // lanes whose run has no page
+    static __device__ __forceinline__ uint32_t lane_of(uint32_t v, uint32_t i) {
+        return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), static_cast<int>(i)));
+    }
+    __device__ __forceinline__ uint64_t at(uint32_t i) const { return lane_of(lo, i) | static_cast<uint64_t>(lane_of(hi, i)) << 32; }
+    __device__ __forceinline__ uint64_t scale(uint32_t i) const {
+        return lane_of(scale_lo, i) | static_cast<uint64_t>(lane_of(scale_hi, i)) << 32;
+    }
+    __device__ __forceinline__ uint32_t rows(uint32_t i) const { return lane_of(n, i); }
 };
 
-// (the table is read through the scalar cache: nothing writes it while a kernel runs)
-typedef const __attribute__((address_space(4))) uint32_t *ScalarTable;
+// The table's entry of slot s of sequence b.
+template <bool PAGED>
+__device__ __forceinline__ uint32_t entry_of(const WindowArgs &a, uint32_t b, uint32_t s) {
+    if constexpr (!PAGED) return b;
+    return a.kv.table[static_cast<size_t>(b) * a.kv.table_stride + a.kv.entry(min(s, a.kv.len - 1))];
+}
 
-template <bool PAGED, int PIECES, uint32_t TK>
-__device__ __forceinline__ void entries_of(const WindowArgs &a, uint32_t b, uint32_t tile, uint32_t *page) {
-    if constexpr (PAGED) {
-        const ScalarTable table = (ScalarTable)(a.kv.table + static_cast<size_t>(b) * a.kv.table_stride);
+// The lane's run: LEN slots from s on (none, unless `have`), of the given entry.
+template <int CT, bool PAGED, uint32_t LEN>
+__device__ __forceinline__ Spans span_run(const WindowArgs &a, const Tiles &t, uint32_t kvh, uint32_t s, bool have, uint32_t entry) {
+    const bool bad = PAGED && entry >= a.kv.pages, there = have && !bad && s < t.hi && (s < a.sinks || s + LEN > t.lo);
+    const uint64_t page = there ? entry : 0u, in = there ? s - (PAGED ? a.kv.entry(s) * a.kv.page_len : 0u) : 0u;
+    const uint64_t at = static_cast<uint64_t>(kvh) * a.kv.page_len + in, byte = (page * a.kv.stride + at * 64) * Cached<CT>::ES;
+    Spans p{};
+    p.lo = static_cast<uint32_t>(byte);
+    p.hi = static_cast<uint32_t>(byte >> 32);
+    if constexpr (CT == DT_F8) {
+        const uint64_t sc = page * a.kv.sstride + at;
+        p.scale_lo = static_cast<uint32_t>(sc);
+        p.scale_hi = static_cast<uint32_t>(sc >> 32);
+    }
+    p.n = there ? min(t.hi - s, LEN) : 0;
+    p.holes = PAGED ? __ballot(bad) : 0;
+    return p;
+}
+
+// A row's query as the operand's pieces, scaled so that the scores are base-2 exponents (`scaled`: times c, 1 / c = unit).  Lane
+// (l16, g) holds dims 16 g .. + 15, or, in halves, 8 g .. + 7 and 32 + 8 g .. + 7.
+template <int CT>
+struct Query {
+    u32x4v f[2][Kind<CT>::NQ];
+    float c, unit;
+    bool scaled;
+};
+struct RawQuery {
+    float4 v[4];
+};
+template <bool HALVES>
+__device__ __forceinline__ RawQuery load_query(const float *q, uint32_t g, bool have) {
+    const float4 *p = reinterpret_cast<const float4 *>(q + (HALVES ? 8 : 16) * g);
+    RawQuery r;
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const uint32_t s = min(tile * TK + i * (TK / PIECES), a.kv.len - 1);
-            page[i] = table[a.kv.entry(s)];
+    for (int e = 0; e < 4; e++) r.v[e] = have ? p[HALVES ? 8 * (e / 2) + (e & 1) : e] : make_float4(0.f, 0.f, 0.f, 0.f);
+    return r;
+}
+template <int CT>
+__device__ __forceinline__ Query<CT> query_of(const RawQuery &r, float scale) {
+    Query<CT> x;
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        v[4 * e] = r.v[e].x; v[4 * e + 1] = r.v[e].y; v[4 * e + 2] = r.v[e].z; v[4 * e + 3] = r.v[e].w;
+    }
+    const float c0 = scale * 1.4426950408889634f;
+    float f = c0;
+    x.c = x.unit = 1.0f;
+    x.scaled = false;
+    if constexpr (CT == DT_F16) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; e++) mx = fmaxf(mx, fabsf(v[e]));
+        mx = rows_max(mx);
+        // Two pieces hold 22 bits of q times the scale where the row's largest is 1/8 to 2^14, or next to nothing.
+        const float top = mx * fabsf(c0);
+        x.scaled = __any(!(top >= 0.125f && top < 16384.0f) && top != 0.0f);
+        if (x.scaled) {  // the row's largest |q| to 2^13 .. 2^14
+            const int ex = min(267 - static_cast<int>(__float_as_uint(mx) >> 23), 253);
+            f = __uint_as_float(static_cast<uint32_t>(ex) << 23);
+            // (not 0: scores times less than 2^-100 are next to nothing all the same, being below 2^37)
+            x.c = fmaxf(fabsf(c0) * __uint_as_float(static_cast<uint32_t>(254 - ex) << 23), 0x1p-100f);
+            x.unit = 1.0f / x.c;
+            if (c0 < 0.0f) f = -f;
         }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e++) v[e] *= f;
+#pragma unroll
+    for (int kk = 0; kk < 2; kk++) split8<CT>(v + 8 * kk, x.f[kk]);
+    return x;
+}
+
+// The running sums of a row.  Weights are 2^(s + ref) of its scores s (as base-2 exponents): ref brings the largest score so far to
+// BASE, or, since it changes only where a score would be past BASE + AHEAD, to BASE + AHEAD at most, once the row has a score
+// (begun).  Most tiles then neither rescale the sums nor subtract a maximum: `below`, ref as the products' starting sum, does that.
+// Weights of fp16 pieces are up to 2^15; one of 2^-21 of the largest or less loses what is below 2^-31 of that.
+constexpr float AHEAD = 8.0f;
+template <int CT>
+constexpr float BASE = CT == DT_F16 ? 7.0f : 0.0f;
+
+struct Sums {
+    float ref = 0.0f, ls = 0.0f;  // ls: the lane's share of the weights' sum
+    bool begun = false;
+    f32x4v below = {0.f, 0.f, 0.f, 0.f}, o[4] = {};  // o[d]: dims 16 d + 4 g .. + 3 (or those of load_values)
+    // What the join of parts takes: minus the reference, or infinity.
+    __device__ __forceinline__ float mark() const { return begun ? ref : INFINITY; }
+};
+
+// Scores s[u][e], of key 16 u + 4 g + e of a tile from slot k0 on, that the row (or, from `top` on, none) does not see.
+template <int NK>
+__device__ __forceinline__ void hide(f32x4v (&s)[NK], uint32_t k0, uint32_t g, uint32_t lo, uint32_t hi, uint32_t sinks, uint32_t none, int runs) {
+#pragma unroll
+    for (int u = 0; u < NK; u++) {
+        const uint32_t key = k0 + 16 * u + 4 * g, top = (none >> (u * runs / NK)) & 1 ? 0 : hi;
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[u][e] = (key + e >= lo || key + e < sinks) && key + e < top ? s[u][e] : -INFINITY;
     }
 }
 
-template <bool PAGED, int PIECES, uint32_t TK>
-__device__ __forceinline__ void pieces_of(const WindowArgs &a, const Tiles &t, uint32_t b, uint32_t kvh, uint32_t tile, bool have,
-                                          const uint32_t *page, Pieces<PIECES> &p) {
-    constexpr uint32_t LEN = TK / PIECES;
-    p.none = 0;
+// The scores' reference, a new one where they need it.
+template <int CT, int NK>
+__device__ __forceinline__ void refer(f32x4v (&s)[NK], Sums &m, float unit) {
+    float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < PIECES; i++) {
-        const uint32_t s = tile * TK + i * LEN;
-        uint64_t pg = b;
-        uint32_t in = s;
-        bool there = have && s < t.hi && (s < a.sinks || s + LEN > t.lo);
-        if constexpr (PAGED) {
-            pg = page[i];
-            in -= a.kv.entry(s) * a.kv.page_len;
-            if (page[i] >= a.kv.pages) {
-                there = false;
-                p.none |= 1u << i;
-            }
-        }
-        if (!there) pg = in = 0;
-        const uint64_t r = static_cast<uint64_t>(kvh) * a.kv.page_len + in;
-        p.row[i] = pg * a.kv.stride + r * 64;
-        p.scale[i] = pg * a.kv.sstride + r;
-        p.n[i] = there ? min(t.hi - s, LEN) : 0;
+    for (int u = 0; u < NK; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[u][e]);
+    if (!__any(mx > (m.begun ? BASE<CT> + AHEAD : -INFINITY))) return;
+    mx = rows_max(mx);
+    const float up = mx > (m.begun ? BASE<CT> : -INFINITY) ? mx - BASE<CT> : 0.0f, al = m.begun ? __builtin_amdgcn_exp2f(-up) : 1.0f;
+    m.ref -= up;
+    m.begun = m.begun || mx > -INFINITY;
+    m.ls *= al;
+    const float at = m.ref * unit;
+    m.below = f32x4v{at, at, at, at};
+#pragma unroll
+    for (int u = 0; u < NK; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[u][e] -= up;
+#pragma unroll
+    for (int d = 0; d < 4; d++) m.o[d] *= al;
+}
+
+// Eight weights as pieces.
+template <int CT>
+__device__ __forceinline__ void weights8(const float *x, u32x4v *p) {
+    if constexpr (CT != DT_F16) return split8<CT>(x, p);
+    // The upper piece is the weight cut to 11 bits, so the rest is exact (two cycles an instruction each; one that subtracts the packed
+    // half, v_fma_mixlo_f16, takes eight).
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float a = x[2 * e], b = x[2 * e + 1];
+        const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+        p[0][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ah, bh));
+        p[1][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2v{a - ah, b - bh}, f16x2t));
     }
 }
 
-// The keys (values) of a tile's pieces; zeros, which the buffers' bounds give, for slots that no row sees and without a page.
+// The keys (values) of a tile's pieces, whose spans lanes `first` and on hold; zeros, which the buffers' bounds give, for slots that
+// no row sees and without a page.
 template <int CT, int PIECES>
-__device__ __forceinline__ void load_keys(Raw<CT> &r, const WindowArgs &a, const Pieces<PIECES> &p, uint32_t l16, uint32_t g) {
+__device__ __forceinline__ void load_keys(Raw<CT> &r, const WindowArgs &a, const Spans &p, uint32_t first, uint32_t l16, uint32_t g) {
     constexpr uint32_t ROW = Cached<CT>::ROW;
     constexpr int GROUPS = 2 * Raw<CT>::SUB, EACH = GROUPS / PIECES;  // groups of 16 keys, those of a piece
 #pragma unroll
     for (int i = 0; i < PIECES; i++) {
-        const __amdgpu_buffer_rsrc_t b = span_of(static_cast<const char *>(a.kv.k) + p.row[i] * Cached<CT>::ES, p.n[i] * ROW);
+        const __amdgpu_buffer_rsrc_t b = span_of(static_cast<const char *>(a.kv.k) + p.at(first + i), p.rows(first + i) * ROW);
 #pragma unroll
         for (int u = 0; u < EACH; u++)
 #pragma unroll
@@ -176,19 +294,19 @@ __device__ __forceinline__ void load_keys(Raw<CT> &r, const WindowArgs &a, const
                 r.k[(EACH * i + u) * Kind<CT>::KW + w] =
                     __builtin_amdgcn_raw_buffer_load_b128(b, l16 * ROW + 16 * Cached<CT>::ES * g + 16 * ROW * u + 16 * w, 0, 0);
         if constexpr (CT == DT_F8) {
-            const __amdgpu_buffer_rsrc_t s = span_of(a.kv.ks + p.scale[i], p.n[i]);
+            const __amdgpu_buffer_rsrc_t s = span_of(a.kv.ks + p.scale(first + i), p.rows(first + i));
 #pragma unroll
             for (int u = 0; u < EACH; u++) r.ks[EACH * i + u] = __builtin_amdgcn_raw_buffer_load_b8(s, l16 + 16 * u, 0, 0);
         }
     }
 }
 template <int CT, int PIECES>
-__device__ __forceinline__ void load_values(Raw<CT> &r, const WindowArgs &a, const Pieces<PIECES> &p, uint32_t l16, uint32_t g) {
+__device__ __forceinline__ void load_values(Raw<CT> &r, const WindowArgs &a, const Spans &p, uint32_t first, uint32_t l16, uint32_t g) {
     constexpr uint32_t ROW = Cached<CT>::ROW;
     constexpr int GROUPS = 2 * Raw<CT>::SUB, EACH = GROUPS / PIECES;
 #pragma unroll
     for (int i = 0; i < PIECES; i++) {
-        const __amdgpu_buffer_rsrc_t b = span_of(static_cast<const char *>(a.kv.v) + p.row[i] * Cached<CT>::ES, p.n[i] * ROW);
+        const __amdgpu_buffer_rsrc_t b = span_of(static_cast<const char *>(a.kv.v) + p.at(first + i), p.rows(first + i) * ROW);
 #pragma unroll
         for (int j = 0; j < 4 * EACH; j++) {
             const uint32_t at = 4 * g * ROW + 4 * Cached<CT>::ES * l16 + (16 * (j >> 2) + (j & 3)) * ROW;
@@ -206,27 +324,23 @@ __device__ __forceinline__ void load_values(Raw<CT> &r, const WindowArgs &a, con
             }
         }
         if constexpr (CT == DT_F8) {  // four keys' bytes a load: up to three past n, which the caches' whole words hold
-            const __amdgpu_buffer_rsrc_t s = span_of(a.kv.vs + p.scale[i], (p.n[i] + 3) & ~3u);
+            const __amdgpu_buffer_rsrc_t s = span_of(a.kv.vs + p.scale(first + i), (p.rows(first + i) + 3) & ~3u);
 #pragma unroll
             for (int u = 0; u < EACH; u++) r.vs[EACH * i + u] = __builtin_amdgcn_raw_buffer_load_b32(s, 4 * g + 16 * u, 0, 0);
         }
     }
 }
 
-// v / G (WindowArgs)
-__device__ __forceinline__ uint32_t by_group(const WindowArgs &a, uint32_t v) {
-    return a.group == 1 ? v : __umulhi(v, a.group_magic);
-}
+constexpr uint32_t AW_WAVES = 8, AW_FEW = 4;  // waves of a workgroup
 
-// Grid: x the sequences' row tiles, y the key heads, z the parts.
+// Few rows.  Grid: x the sequences' row tiles, y the key heads, z the parts.
 template <int CT, bool PAGED, int PIECES, bool APART, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) void attention_window_kernel(WindowArgs a) {
     typedef Kind<CT> KD;
-    constexpr int SUB = Raw<CT>::SUB;
+    constexpr int SUB = Raw<CT>::SUB, NK = 2 * SUB;
     constexpr uint32_t TK = Raw<CT>::TK;
     __shared__ __attribute__((aligned(16))) float part[WAVES * 16 * AT_LD];
     __shared__ float ms[WAVES * 16], sums[WAVES * 16];
-    __shared__ uint32_t redo[WAVES / 2];
     const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t wk = wave % a.keys, wr = wave / a.keys;
@@ -238,17 +352,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     const uint32_t r0 = (a.seq_tiles - 1 - (blockIdx.x - b * a.seq_tiles)) * span, r1 = min(n * G, r0 + span);
     if (r0 >= r1) return;
 
-    // The lane's row (all four g's the same one), its query's 16 dims and its keys [lo, hi) and those before a.sinks.
+    // The lane's row (all four g's the same one) and its keys [lo, hi) and those before a.sinks.
     const uint32_t rw = r0 + wr * 16, r = rw + l16, t = by_group(a, r), head = kvh * G + r - t * G;
+    const bool have = r < r1;
+    // What does not wait for the sequence's position goes first: the query, and, where no window moves the first tile, its entries.
+    const RawQuery rq = load_query<false>(a.q + (static_cast<size_t>(b) * T + t) * a.ldq + head * 64, g, have);
+    constexpr uint32_t EACH = 64 / PIECES, LEN = TK / PIECES;  // tiles whose spans a wave holds, slots of a piece
+    uint32_t early = 0;
+    if (PAGED && a.window == 0) {
+        const uint32_t tile = (APART ? blockIdx.z * a.run : 0) + wk + lane / PIECES * a.keys;
+        early = entry_of<PAGED>(a, b, tile * TK + lane % PIECES * LEN);  // (window_plan keeps it within 32 bits)
+    }
     const uint64_t pos = a.rows.pos ? a.rows.pos[b] : 0u;
     uint32_t lo = 0, hi = 0, first;
-    float4 qv[4] = {};
-    if (r < r1) {
-        const float4 *p = reinterpret_cast<const float4 *>(a.q + (static_cast<size_t>(b) * T + t) * a.ldq + head * 64 + 16 * g);
-#pragma unroll
-        for (int e = 0; e < 4; e++) qv[e] = p[e];
-        row_keys(a, pos + t, first, lo, hi);
-    }
+    if (have) row_keys(a, pos + t, first, lo, hi);
     Tiles tl{};
     uint32_t i = 0, end = 0;  // this wave's tiles: every keys-th one from i on
     if (rw < r1) {
@@ -263,65 +380,36 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     }
 
     Raw<CT> raw;
-    uint32_t page[PIECES] = {};  // the entries of the tile after the one whose keys are on their way
-    Pieces<PIECES> pc;
-    auto entries = [&](uint32_t j) { entries_of<PAGED, PIECES, TK>(a, b, tl.at(min(j, end - 1)), page); };
-    auto pieces = [&](uint32_t j) { pieces_of<PAGED, PIECES, TK>(a, tl, b, kvh, tl.at(min(j, end - 1)), j < end, page, pc); };
+    // The spans of EACH tiles of this wave, and the entries of the next ones.
+    const uint32_t i0 = i;
+    auto slot_of = [&](uint32_t q) { return tl.at(min(i0 + (q + lane / PIECES) * a.keys, end - 1)) * TK + lane % PIECES * LEN; };
+    auto spans = [&](uint32_t q, uint32_t entry) {
+        return span_run<CT, PAGED, LEN>(a, tl, kvh, slot_of(q), i0 + (q + lane / PIECES) * a.keys < end, entry);
+    };
+    Spans sp{};
+    uint32_t q = 0, next_entry = 0;  // this wave's tiles so far
     // Loads of a tile past the last one are issued too, of no bytes: with as many loads in flight on every path, the waits for
     // the values leave the next keys on their way.
-    if (end > 0) {
-        entries(i);
-        pieces(i);
+    if (i < end) {
+        sp = spans(0, PAGED && a.window == 0 ? early : entry_of<PAGED>(a, b, slot_of(0)));
         __builtin_amdgcn_sched_barrier(0);  // in this order, as in the loop, or its first wait is for all of them
-        load_keys<CT>(raw, a, pc, l16, g);
+        load_keys<CT, PIECES>(raw, a, sp, 0, l16, g);
         __builtin_amdgcn_sched_barrier(0);
-        load_values<CT>(raw, a, pc, l16, g);
+        load_values<CT, PIECES>(raw, a, sp, 0, l16, g);
         __builtin_amdgcn_sched_barrier(0);
+        if (i + EACH * a.keys < end) next_entry = entry_of<PAGED>(a, b, slot_of(EACH));
     }
+    const Query<CT> qu = query_of<CT>(rq, a.scale);
 
-    // The query as the operand's pieces, scaled so that the scores are base-2 exponents (fp16 pieces: times c).
-    u32x4v qf[2][KD::NQ];
-    const float c0 = a.scale * 1.4426950408889634f;
-    float c = 1.0f;
-    {
-        float v[16];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            v[4 * e] = qv[e].x; v[4 * e + 1] = qv[e].y; v[4 * e + 2] = qv[e].z; v[4 * e + 3] = qv[e].w;
-        }
-        float f = c0;
-        if constexpr (CT == DT_F16) {  // the row's largest |q| to 2^13 .. 2^14
-            float mx = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; e++) mx = fmaxf(mx, fabsf(v[e]));
-            mx = rows_max(mx);
-            const int ex = min(267 - static_cast<int>(__float_as_uint(mx) >> 23), 253);
-            f = __uint_as_float(static_cast<uint32_t>(ex) << 23);
-            c = fabsf(c0) * __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
-            if (c < 0x1p-126f) c = 0x1p-126f;  // not 0, so that a key outside weighs 0 (-infinity times c); scores are below 2^37
-            if (c0 < 0.0f) f = -f;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; e++) v[e] *= f;
-#pragma unroll
-        for (int kk = 0; kk < 2; kk++) split8<CT>(v + 8 * kk, qf[kk]);
-    }
-
-    f32x4v o[4];
-    float sub = INFINITY, ls = 0.0f;  // minus the running maximum (+infinity: no key yet), the lane's share of the weights' sum
-#pragma unroll
-    for (int d = 0; d < 4; d++) o[d] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    for (; i < end; i += a.keys) {
-        const uint32_t k0 = tl.at(i) * TK, none = pc.none;
-        entries(i + a.keys);
-        f32x4v s[2 * SUB];
-#pragma unroll
-        for (int u = 0; u < 2 * SUB; u++) s[u] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    Sums m;
+    for (; i < end; i += a.keys, q++) {
+        const uint32_t k0 = tl.at(i) * TK, none = PAGED ? static_cast<uint32_t>(sp.holes >> (q % EACH * PIECES)) & ((1u << PIECES) - 1) : 0;
+        f32x4v s[NK];
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
-            u32x4v kf[2 * SUB][KD::NC];
+            u32x4v kf[NK][KD::NC];
 #pragma unroll
-            for (int u = 0; u < 2 * SUB; u++) {
+            for (int u = 0; u < NK; u++) {
                 if constexpr (CT == DT_F8) {
                     const float f = f8_pow2(raw.ks[u]);
                     const uint32_t w0 = raw.k[u][2 * kk], w1 = raw.k[u][2 * kk + 1];
@@ -338,53 +426,46 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
                         for (int x = 0; x < 3; x++) kf[u][x][e] = p[x];
                     }
                 }
+                if (kk == 0) s[u] = m.below;
             }
-            dots<CT, 2 * SUB>(kf, qf[kk], s);
+            dots<CT, NK>(kf, qu.f[kk], s);
         }
-        pieces(i + a.keys);
-        load_keys<CT>(raw, a, pc, l16, g);
+        const uint32_t at = (q + 1) % EACH;
+        if (at == 0 && i + a.keys < end) {
+            sp = spans(q + 1, next_entry);
+            if (i + (1 + EACH) * a.keys < end) next_entry = entry_of<PAGED>(a, b, slot_of(q + 1 + EACH));
+        } else if (i + a.keys >= end) {
+            sp.n = 0;
+        }
+        load_keys<CT, PIECES>(raw, a, sp, at * PIECES, l16, g);
 
         if (!((k0 >= tl.in_lo || k0 + TK <= a.sinks) && k0 + TK <= tl.in_hi) || none) {
+            hide<NK>(s, k0, g, lo, hi, a.sinks, none, PIECES);
+            if constexpr (CT == DT_F8) {  // a scale byte past the keys may stand for anything
 #pragma unroll
-            for (int u = 0; u < 2 * SUB; u++) {
-                const uint32_t key = k0 + 16 * u + 4 * g;
-                const uint32_t top = PAGED && (none >> (u * PIECES / (2 * SUB)) & 1) ? 0 : hi;
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[u][e] = (key + e >= lo || key + e < a.sinks) && key + e < top ? s[u][e] : -INFINITY;
-                if constexpr (CT == DT_F8) {  // a scale byte past the keys may stand for anything
-                    const uint32_t k = tl.hi > key ? min(tl.hi - key, 4u) : 0;
+                for (int u = 0; u < NK; u++) {
+                    const uint32_t key = k0 + 16 * u + 4 * g, k = tl.hi > key ? min(tl.hi - key, 4u) : 0;
                     raw.vs[u] &= k == 4 ? ~0u : (1u << (8 * k)) - 1;
                 }
             }
         }
-        float mx = -INFINITY;
+        if (qu.scaled) {
 #pragma unroll
-        for (int u = 0; u < 2 * SUB; u++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[u][e]);
-        mx = rows_max(mx);
-        const float sn = fminf(sub, -(mx * c));
-        const float al = sn == sub ? 1.0f : __builtin_amdgcn_exp2f(sn - sub);  // brings older sums to the new maximum
-        sub = sn;
-        const float su = sn == INFINITY ? 0.0f : sn;
+            for (int u = 0; u < NK; u++) s[u] *= qu.c;
+        }
+        refer<CT, NK>(s, m, qu.unit);
         u32x4v pf[SUB][KD::NQ];
-        float sum = 0.0f;
 #pragma unroll
         for (int x = 0; x < SUB; x++) {
             float p[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                p[j] = __builtin_amdgcn_exp2f(fmaf(s[2 * x + (j >> 2)][j & 3], c, su));
-                sum += p[j];
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
+                p[j] = __builtin_amdgcn_exp2f(s[2 * x + (j >> 2)][j & 3]);
+                m.ls += p[j];
                 if constexpr (CT == DT_F8) p[j] *= f8_pow2((raw.vs[2 * x + (j >> 2)] >> (8 * (j & 3))) & 255u);
-                else p[j] *= KD::PS;
             }
-            split8<CT>(p, pf[x]);
+            weights8<CT>(p, pf[x]);
         }
-        ls = fmaf(ls, al, sum);
 
         // p . v: a tile's sum starts from zero and joins the running one in one rounding.
         f32x4v ot[4];
@@ -414,32 +495,29 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
             dots<CT, 4>(vf, pf[x], ot);
         }
 #pragma unroll
-        for (int d = 0; d < 4; d++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[d][e] = fmaf(o[d][e], al, ot[d][e]);
-        load_values<CT>(raw, a, pc, l16, g);
+        for (int d = 0; d < 4; d++) m.o[d] += ot[d];
+        load_values<CT, PIECES>(raw, a, sp, at * PIECES, l16, g);
     }
 
     // The waves' parts of each row meet in wave order: a thread joins four dims of a row.
     {
         float *p = part + (wave * 16 + l16) * AT_LD + 16 * g;
 #pragma unroll
-        for (int e = 0; e < 4; e++) *reinterpret_cast<float4 *>(p + 4 * e) = make_float4(o[0][e], o[1][e], o[2][e], o[3][e]);
-        const float l = ls + __shfl_xor(ls, 16, 64), all = l + __shfl_xor(l, 32, 64);
+        for (int e = 0; e < 4; e++) *reinterpret_cast<float4 *>(p + 4 * e) = make_float4(m.o[0][e], m.o[1][e], m.o[2][e], m.o[3][e]);
+        const float l = m.ls + __shfl_xor(m.ls, 16, 64), all = l + __shfl_xor(l, 32, 64);
         if (g == 0) {
-            ms[wave * 16 + l16] = sub;
+            ms[wave * 16 + l16] = m.mark();
             sums[wave * 16 + l16] = all;
         }
     }
-    if (tid < WAVES / 2) redo[tid] = 0;
     __syncthreads();
     for (uint32_t j = tid; j < span * 16; j += 64 * WAVES) {
         const uint32_t rr = j / 16, d4 = 4 * (j & 15), rj = r0 + rr;  // row rr of the workgroup
-        if (rj >= r1) continue;
+        if (r0 + (j & ~63u) / 16 >= r1) break;  // (whole waves)
         const uint32_t tj = by_group(a, rj), headj = kvh * G + rj - tj * G;
         const size_t row = static_cast<size_t>(b) * T + tj;
         const uint32_t w0 = rr / 16 * a.keys, in = rr & 15;  // the row's waves, its place in each
-        float m = INFINITY, l = 0.0f;
+        float mk = INFINITY, l = 0.0f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         auto join = [&](auto count) {  // a count known here: all parts are read at once
             constexpr uint32_t N = decltype(count)::value;
@@ -453,10 +531,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
                 v[w] = *reinterpret_cast<const float4 *>(part + at * AT_LD + d4);
             }
 #pragma unroll
-            for (uint32_t w = 0; w < N; w++) m = fminf(m, mw[w]);
+            for (uint32_t w = 0; w < N; w++) mk = fminf(mk, mw[w]);
 #pragma unroll
             for (uint32_t w = 0; w < N; w++) {
-                const float f = mw[w] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mw[w]);
+                // (sums without a reference are zeros, or NaN)
+                const float f = mw[w] == INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mk - mw[w]);
                 l = fmaf(sw[w], f, l);
                 acc.x = fmaf(v[w].x, f, acc.x);
                 acc.y = fmaf(v[w].y, f, acc.y);
@@ -470,110 +549,419 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
         if constexpr (APART) {
             const size_t at = (row * a.hq + headj) * a.parts + blockIdx.z;
             float2 *ml = reinterpret_cast<float2 *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * a.parts * 64);
-            *reinterpret_cast<float4 *>(a.part + at * 64 + d4) = acc;
-            if (d4 == 0) ml[at] = make_float2(m, l);
+            if (rj < r1) {
+                *reinterpret_cast<float4 *>(a.part + at * 64 + d4) = acc;
+                if (d4 == 0) ml[at] = make_float2(mk, l);
+            }
         } else {
-            const float f = 1.0f / (l * KD::PS);
+            const float f = 1.0f / l;
             acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-            if (fabsf(acc.x) < INFINITY && fabsf(acc.y) < INFINITY && fabsf(acc.z) < INFINITY && fabsf(acc.w) < INFINITY)
-                *reinterpret_cast<float4 *>(a.out + row * a.ldo + headj * 64 + d4) = acc;
-            else
-                atomicOr(&redo[rr / 32], 1u << (rr % 32));
-        }
-    }
-    if constexpr (!APART) {
-        // Rows with an output that is not finite (or without a weight) once more, each from its own keys alone.
-        __syncthreads();
-        for (uint32_t rr = wave; rr < span; rr += WAVES) {
-            if (!((redo[rr / 32] >> (rr % 32)) & 1)) continue;
-            const uint32_t rj = r0 + rr, tj = by_group(a, rj);
-            attend_wave<CT>(a, b, b * T + tj, kvh * G + rj - tj * G, pos + tj);
+            const bool good = fabsf(acc.x) < INFINITY && fabsf(acc.y) < INFINITY && fabsf(acc.z) < INFINITY && fabsf(acc.w) < INFINITY;
+            uint64_t bad = __ballot(rj < r1 && !good);
+            if (rj < r1 && !((bad >> (lane & 48)) & 0xFFFF)) *reinterpret_cast<float4 *>(a.out + row * a.ldo + headj * 64 + d4) = acc;
+            while (bad) {  // rows with an output that is not finite (or without a weight) once more, each from its own keys alone
+                const uint32_t x = (__ffsll(static_cast<unsigned long long>(bad)) - 1) / 16, rx = r0 + (j & ~63u) / 16 + x, tx = by_group(a, rx);
+                bad &= ~(0xFFFFull << (16 * x));
+                attend_wave<CT>(a, b, b * T + tx, kvh * G + rx - tx * G, pos + tx);
+            }
         }
     }
 }
 
-// The parts of a row and head joined: lane d is dim d, a wave takes every waves-th part, and the waves' sums meet in wave order.
-constexpr uint32_t AJ_WAVES = 16;  // at most
+// ------------------------------------------------------------- many rows --
+
+// Rows of prompts.  A workgroup is WR x WK waves: WR of them have 16 rows each, and WK groups of them take every WK-th tile of
+// keys, which the group's waves share in LDS, 16 bits a value (as NC pieces), converted once.
+typedef short s16x4v __attribute__((ext_vector_type(4)));
+constexpr uint32_t WR = 4;
 
 template <int CT>
-__global__ __launch_bounds__(64 * AJ_WAVES) void window_join_kernel(WindowArgs a) {
-    __shared__ float acc[AJ_WAVES][64], sums[AJ_WAVES], ms[AJ_WAVES];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / 64;
-    const uint32_t row = blockIdx.x, head = blockIdx.y;
-    uint32_t b;
-    uint64_t slot;
-    if (!a.rows.at(row, b, slot)) return;
-    // The parts that the row's tile has.
-    const uint32_t t = row - b * a.rows.T, kvh = head / a.group, r = t * a.group + head - kvh * a.group;
-    const uint32_t n = a.rows.counts ? min(a.rows.counts[b], a.rows.T) : a.rows.T, rw = r & ~15u;
-    const Tiles tl = tiles_of<Raw<CT>::TK>(a, b, by_group(a, rw), by_group(a, min(rw + 16, n * a.group) - 1));
-    const uint32_t S = min(a.parts, (tl.n + a.run - 1) / a.run);
-    const size_t at = (static_cast<size_t>(row) * a.hq + head) * a.parts;
-    const float2 *ml = reinterpret_cast<const float2 *>(a.part + static_cast<size_t>(a.rows.B) * a.rows.T * a.hq * a.parts * 64) + at;
-    const float *o = a.part + at * 64 + lane;
-    float m = INFINITY, l = 0.0f, v = 0.0f;
-    for (uint32_t s0 = wave; s0 < S; s0 += 4 * waves) {  // four parts' loads at once
-        float2 e[4];
-        float x[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            const uint32_t s = min(s0 + i * waves, S - 1);
-            e[i] = ml[s];
-            x[i] = o[static_cast<size_t>(s) * 64];
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            // A part without a key of the row, or with scores of -infinity alone, has no sums; one of NaN scores alone has no
-            // maximum either, but a sum that is NaN.
-            if (s0 + i * waves >= S || (e[i].x == INFINITY && e[i].y == 0.0f)) continue;
-            const float mn = fminf(m, e[i].x);
-            const float f = m == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mn - m), k = __builtin_amdgcn_exp2f(mn - e[i].x);
-            m = mn;
-            l = fmaf(l, f, e[i].y * k);
-            v = fmaf(v, f, x[i] * k);
-        }
+struct Staged {
+    static constexpr uint32_t TK = CT == DT_F32 ? 32 : 64;      // keys of a tile
+    static constexpr uint32_t PLANE = TK * 128;                  // bytes of a piece of its keys (or values)
+    static constexpr uint32_t TILE = PLANE * Kind<CT>::NC;       // and of all pieces
+    static constexpr uint32_t CHUNKS = Cached<CT>::ROW / 16;     // 16-byte chunks of a cached row
+    static constexpr uint32_t ROWS = 64 / CHUNKS;                // rows of a wave's load
+    static constexpr uint32_t HALF = TK / ROWS;                  // loads of a tile's keys, and of its values
+    static constexpr int RUNS = TK / 16;                         // runs of 16 slots, each within one page
+};
+// Byte of chunk c (eight 16-bit values) of a tile's row.  LDS has 64 banks, so two rows are apart by themselves; the swizzle keeps
+// the same chunk of 16 rows apart, and chunks 2 d and 2 d + 1 of eight rows.
+__device__ __forceinline__ uint32_t chunk_at(uint32_t row, uint32_t c) {
+    return row * 128 + ((c ^ (((row >> 1) & 3) << 1 | ((row >> 3) & 1))) << 4);
+}
+
+template <int CT, bool PAGED, bool APART, int WK>
+__global__ __launch_bounds__(64 * WR * WK, CT == DT_F32 && WK == 2 ? 2 : 3) void window_rows_kernel(WindowArgs a) {
+    typedef Kind<CT> KD;
+    typedef Staged<CT> SD;
+    constexpr uint32_t TK = SD::TK, ROW = Cached<CT>::ROW, SPAN = WR * 16;
+    constexpr int NK = TK / 16, LOADS = 2 * SD::HALF / WR;
+    static_assert(2 * SD::HALF % WR == 0, "whole loads a wave");
+    __shared__ __attribute__((aligned(16))) char lds[2][WK][2][SD::TILE];  // two steps' tiles, keys and values
+    const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave / WR, wr = wave % WR;
+    const uint32_t G = a.group, T = a.rows.T;
+
+    // Workgroups go to the XCDs in turn: those of one sequence and key head go to one, whose L2 then fetches their keys once.
+    const uint32_t xcds = a.by_xcd ? 8 : 1, xcd = blockIdx.x % xcds, item = blockIdx.x / xcds;
+    const uint32_t turn = item / a.parts, part = item - turn * a.parts, lap = turn / a.seq_tiles, group = lap * xcds + xcd;
+    const uint32_t b = group / a.hkv, kvh = group - b * a.hkv;
+    if (b >= a.rows.B) return;
+    const uint32_t n = a.rows.counts ? min(a.rows.counts[b], T) : T;
+    const uint32_t r0 = (a.seq_tiles - 1 - (turn - lap * a.seq_tiles)) * SPAN, r1 = min(n * G, r0 + SPAN);  // the longest first
+    if (r0 >= r1) return;
+    // The lane's row (all four g's the same one).
+    const uint32_t rw = r0 + wr * 16, r = rw + l16, t = by_group(a, r), head = kvh * G + r - t * G;
+    const size_t row = static_cast<size_t>(b) * T + t;
+    const bool have = r < r1;
+    const RawQuery rq = load_query<true>(a.q + row * a.ldq + head * 64, g, have);  // (waits for nothing else)
+    const uint64_t pos = a.rows.pos ? a.rows.pos[b] : 0u;
+    uint32_t lo = 0, hi = 0, first;
+    if (have) row_keys(a, pos + t, first, lo, hi);
+    // The workgroup's tiles, its part of them [t0, t1), and the wave's rows' keys.
+    const Tiles tl = tiles_of<TK>(a, b, by_group(a, r0), by_group(a, r1 - 1));
+    Tiles mine{};
+    if (rw < r1) mine = tiles_of<TK>(a, b, by_group(a, rw), by_group(a, min(rw + 16, r1) - 1));
+    uint32_t t0 = 0, t1 = tl.n;
+    if constexpr (APART) {
+        t0 = min(t1, part * a.run);
+        if (part + 1 < a.parts) t1 = min(t1, t0 + a.run);
+        if (t0 == t1) return;
     }
-    if (waves > 1) {
-        acc[wave][lane] = v;
-        if (lane == 0) {
-            sums[wave] = l;
-            ms[wave] = m;
+    const uint32_t steps = (t1 - t0 + WK - 1) / WK;
+
+    // A step's tile on its way: this wave's chunks of it.  The spans of EACH steps' tiles, and the entries of the next ones.
+    u32x4v raw[LOADS];
+    uint32_t scales[LOADS];
+    constexpr uint32_t EACH = 64 / SD::RUNS;
+    auto tile_of = [&](uint32_t step) { return tl.at(min(t0 + step * WK + wk, t1 - 1)); };
+    auto slot_of = [&](uint32_t step) { return tile_of(step + lane / SD::RUNS) * TK + lane % SD::RUNS * 16; };
+    auto spans = [&](uint32_t step, uint32_t entry) {
+        return span_run<CT, PAGED, 16>(a, tl, kvh, slot_of(step), t0 + (step + lane / SD::RUNS) * WK + wk < t1, entry);
+    };
+    auto request = [&](const Spans &sp, uint32_t step) {
+#pragma unroll
+        for (int j = 0; j < LOADS; j++) {
+            const bool is_v = j * WR + wr >= SD::HALF;
+            const uint32_t x = (j * WR + wr) % SD::HALF * SD::ROWS, i = step % EACH * SD::RUNS + x / 16, in = x % 16;  // the load's first row
+            const uint32_t n = sp.rows(i), rows = n > in ? min(n - in, SD::ROWS) : 0;
+            raw[j] = __builtin_amdgcn_raw_buffer_load_b128(
+                span_of(static_cast<const char *>(pick(is_v, a.kv.k, a.kv.v)) + sp.at(i) + in * ROW, rows * ROW), 16 * lane, 0, 0);
+            if constexpr (CT == DT_F8)
+                scales[j] = __builtin_amdgcn_raw_buffer_load_b8(span_of(pick(is_v, a.kv.ks, a.kv.vs) + sp.scale(i) + in, rows), lane / SD::CHUNKS, 0, 0);
+        }
+    };
+    auto store = [&](uint32_t buf) {
+#pragma unroll
+        for (int j = 0; j < LOADS; j++) {
+            const uint32_t id = j * WR + wr, x = id % SD::HALF * SD::ROWS + lane / SD::CHUNKS, c = lane % SD::CHUNKS;
+            char *tile = lds[buf][wk][id >= SD::HALF ? 1 : 0];
+            const u32x4v w = raw[j];
+            if constexpr (CT == DT_F16) {
+                *reinterpret_cast<u32x4v *>(tile + chunk_at(x, c)) = w;
+            } else if constexpr (CT == DT_F8) {
+                const float f = f8_pow2(scales[j]);
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    *reinterpret_cast<u32x4v *>(tile + chunk_at(x, 2 * c + h)) =
+                        u32x4v{f8_bf16x2<false>(w[2 * h], f), f8_bf16x2<true>(w[2 * h], f), f8_bf16x2<false>(w[2 * h + 1], f), f8_bf16x2<true>(w[2 * h + 1], f)};
+            } else {
+                uint32_t p[3], q[3];
+                split2<CT>(__uint_as_float(w[0]), __uint_as_float(w[1]), p);
+                split2<CT>(__uint_as_float(w[2]), __uint_as_float(w[3]), q);
+#pragma unroll
+                for (int i = 0; i < 3; i++) *reinterpret_cast<u32x2v *>(tile + i * SD::PLANE + chunk_at(x, c / 2) + 8 * (c & 1)) = u32x2v{p[i], q[i]};
+            }
+        }
+    };
+    auto holes = [&](const Spans &sp, uint32_t step) {  // runs of 16 slots without a page
+        return PAGED ? static_cast<uint32_t>(sp.holes >> (step % EACH * SD::RUNS)) & ((1u << SD::RUNS) - 1) : 0;
+    };
+    Spans sp = spans(0, entry_of<PAGED>(a, b, slot_of(0)));
+    uint32_t next_entry = steps > EACH ? entry_of<PAGED>(a, b, slot_of(EACH)) : 0;
+    request(sp, 0);
+    uint32_t none = holes(sp, 0), none_next = 0;
+    const Query<CT> qu = query_of<CT>(rq, a.scale);
+    store(0);
+    __syncthreads();
+
+    Sums m;
+    for (uint32_t step = 0; step < steps; step++) {
+        const uint32_t buf = step & 1;
+        if (step + 1 < steps) {
+            if ((step + 1) % EACH == 0) {
+                sp = spans(step + 1, next_entry);
+                if (step + 1 + EACH < steps) next_entry = entry_of<PAGED>(a, b, slot_of(step + 1 + EACH));
+            }
+            request(sp, step + 1);
+            none_next = holes(sp, step + 1);
+        }
+        const uint32_t k0 = tile_of(step) * TK;
+        if (t0 + step * WK + wk < t1 && rw < r1 && k0 < mine.hi && (k0 < a.sinks || k0 + TK > mine.lo)) {
+            const char *kt = lds[buf][wk][0], *vt = lds[buf][wk][1];
+            f32x4v s[NK];
+            {
+                u32x4v kf[NK][2][KD::NC];
+#pragma unroll
+                for (int u = 0; u < NK; u++)
+#pragma unroll
+                    for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                        for (int x = 0; x < KD::NC; x++)
+                            kf[u][kk][x] = *reinterpret_cast<const u32x4v *>(kt + x * SD::PLANE + chunk_at(16 * u + l16, 4 * kk + g));
+                __builtin_amdgcn_sched_barrier(0);  // all reads on their way: one latency, not one a group of keys
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+                    for (int x = 0; x < Products<CT>::N; x++)
+#pragma unroll
+                        for (int u = 0; u < NK; u++)
+                            s[u] = mma<KD::HALF>(kf[u][kk][Products<CT>::C[x]], qu.f[kk][Products<CT>::Q[x]], kk + x == 0 ? m.below : s[u]);
+            }
+            u32x4v vf[4][KD::NC];
+            auto values = [&](int x) {
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+#pragma unroll
+                    for (int y = 0; y < KD::NC; y++) {
+                        u32x2v w[2];
+#pragma unroll
+                        for (int z = 0; z < 2; z++) {  // lane l16 gets dim 16 d + l16 of four keys, of which it points at a quarter of one
+                            const char *p = vt + y * SD::PLANE + chunk_at(32 * x + 16 * z + 4 * g + (l16 >> 2), 2 * d + ((l16 & 3) >> 1)) + 8 * (l16 & 1);
+                            w[z] = __builtin_bit_cast(u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4v *)(p)));
+                        }
+                        vf[d][y] = u32x4v{w[0][0], w[0][1], w[1][0], w[1][1]};
+                    }
+            };
+            values(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!((k0 >= mine.in_lo || k0 + TK <= a.sinks) && k0 + TK <= mine.in_hi) || none) hide<NK>(s, k0, g, lo, hi, a.sinks, none, NK);
+            if (qu.scaled) {
+#pragma unroll
+                for (int u = 0; u < NK; u++) s[u] *= qu.c;
+            }
+            refer<CT, NK>(s, m, qu.unit);
+            // p . v: a tile's sum starts from zero and joins the running one in one rounding.
+            f32x4v ot[4];
+#pragma unroll
+            for (int d = 0; d < 4; d++) ot[d] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < NK / 2; x++) {
+                u32x4v pf[KD::NQ];
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    p[j] = __builtin_amdgcn_exp2f(s[2 * x + j / 4][j % 4]);
+                    m.ls += p[j];
+                }
+                weights8<CT>(p, pf);
+#pragma unroll
+                for (int y = 0; y < Products<CT>::N; y++)
+#pragma unroll
+                    for (int d = 0; d < 4; d++) ot[d] = mma<KD::HALF>(vf[d][Products<CT>::C[y]], pf[Products<CT>::Q[y]], ot[d]);
+                if (x + 1 < NK / 2) values(x + 1);
+            }
+#pragma unroll
+            for (int d = 0; d < 4; d++) m.o[d] += ot[d];
+        }
+        none = none_next;
+        if (step + 1 < steps) store(buf ^ 1);
+        __syncthreads();
+    }
+
+    m.ls += __shfl_xor(m.ls, 16, 64);
+    m.ls += __shfl_xor(m.ls, 32, 64);
+    float mark = m.mark();
+    if constexpr (WK > 1) {  // the waves of a row meet in wave order, in the first of them
+        constexpr uint32_t WORDS = 18 * 64;
+        float *hand = reinterpret_cast<float *>(&lds[0][0][0][0]);  // [wave - WR][18][64]
+        static_assert(sizeof(lds) >= WR * (WK - 1) * WORDS * 4, "the hand-over fits the tiles' memory");
+        if (wk > 0) {
+            float *p = hand + (wave - WR) * WORDS + lane;
+#pragma unroll
+            for (int e = 0; e < 16; e++) p[e * 64] = m.o[e / 4][e % 4];
+            p[16 * 64] = mark;
+            p[17 * 64] = m.ls;
         }
         __syncthreads();
-        if (wave > 0) return;
-        m = INFINITY;
-        for (uint32_t i = 0; i < waves; i++) m = fminf(m, ms[i]);
-        l = v = 0.0f;
-        for (uint32_t i = 0; i < waves; i++) {
-            const float f = ms[i] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - ms[i]);
-            l = fmaf(sums[i], f, l);
-            v = fmaf(acc[i][lane], f, v);
+        if (wk > 0) return;
+#pragma unroll
+        for (int w = 1; w < WK; w++) {
+            const float *p = hand + (wave + (w - 1) * WR) * WORDS + lane;
+            const float other = p[16 * 64], both = fminf(mark, other);
+            // (sums without a reference are zeros, or NaN)
+            const float f0 = mark == INFINITY ? 1.0f : __builtin_amdgcn_exp2f(both - mark), f1 = other == INFINITY ? 1.0f : __builtin_amdgcn_exp2f(both - other);
+            m.ls = fmaf(p[17 * 64], f1, m.ls * f0);
+#pragma unroll
+            for (int e = 0; e < 16; e++) m.o[e / 4][e % 4] = fmaf(p[e * 64], f1, m.o[e / 4][e % 4] * f0);
+            mark = both;
         }
     }
-    v *= 1.0f / (l * Kind<CT>::PS);
-    if (__all(fabsf(v) < INFINITY)) a.out[static_cast<size_t>(row) * a.ldo + head * 64 + lane] = v;
-    else attend_wave<CT>(a, b, row, head, slot);
+    if constexpr (APART) {
+        if (!have) return;
+        const size_t at = (row * a.hq + head) * a.parts + part;
+        float2 *ml = reinterpret_cast<float2 *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * a.parts * 64);
+#pragma unroll
+        for (int d = 0; d < 4; d++) *reinterpret_cast<f32x4v *>(a.part + at * 64 + 16 * d + 4 * g) = m.o[d];
+        if (g == 0) ml[at] = make_float2(mark, m.ls);
+        return;
+    }
+    const float f = 1.0f / m.ls;
+    bool good = true;
+#pragma unroll
+    for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            m.o[d][e] *= f;
+            good = good && fabsf(m.o[d][e]) < INFINITY;
+        }
+    const uint64_t bad64 = __ballot(have && !good), bad32 = bad64 | bad64 >> 32;
+    uint32_t bad = static_cast<uint32_t>(bad32 | bad32 >> 16) & 0xFFFFu;
+    if (have && !((bad >> l16) & 1)) {
+        float *p = a.out + row * a.ldo + head * 64 + 4 * g;
+#pragma unroll
+        for (int d = 0; d < 4; d++) *reinterpret_cast<f32x4v *>(p + 16 * d) = m.o[d];
+    }
+    // Rows with an output that is not finite (or without a weight) once more, each from its own keys alone.
+    for (; bad; bad &= bad - 1) {
+        const uint32_t rj = rw + __builtin_ctz(bad), tj = by_group(a, rj);
+        attend_wave<CT>(a, b, b * T + tj, kvh * G + rj - tj * G, pos + tj);
+    }
+}
+
+// The parts of a row and head joined, by 2^a.join_log groups of 16 lanes that take every such part each and meet in LDS in their
+// order; a lane has four dims.
+constexpr uint32_t AJ_THREADS = 256, AJ_GROUPS = AJ_THREADS / 16;
+
+template <int CT>
+__global__ __launch_bounds__(AJ_THREADS) void window_join_kernel(WindowArgs a) {
+    __shared__ __attribute__((aligned(16))) float4 acc[AJ_GROUPS][16];
+    __shared__ float sums[AJ_GROUPS], ms[AJ_GROUPS];
+    const uint32_t lane = threadIdx.x & 15, group = threadIdx.x / 16, W = 1u << a.join_log, items = AJ_GROUPS >> a.join_log;
+    const uint32_t all = a.rows.B * a.rows.T * a.hq;  // below 2^31
+    const float2 *marks = reinterpret_cast<const float2 *>(a.part + static_cast<size_t>(all) * a.parts * 64);
+    // Item `it` of the workgroup: a row and head, if the sequence has the row.
+    auto locate = [&](uint32_t it, uint32_t &b, uint32_t &row, uint32_t &head, uint64_t &slot) {
+        const uint32_t i = blockIdx.x * items + it;
+        row = i / a.hq;
+        head = i - row * a.hq;
+        return i < all && a.rows.at(row, b, slot);
+    };
+    uint32_t b, row, head;
+    uint64_t slot;
+    float m = INFINITY, l = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (locate(group % items, b, row, head, slot)) {
+        // The parts that the row's workgroup has.
+        const uint32_t t = row - b * a.rows.T, kvh = head / a.group, r = t * a.group + head - kvh * a.group;
+        const uint32_t n = a.rows.counts ? min(a.rows.counts[b], a.rows.T) : a.rows.T, rw = r & ~(a.span - 1);
+        const Tiles tl = tiles_of<Raw<CT>::TK>(a, b, by_group(a, rw), by_group(a, min(rw + a.span, n * a.group) - 1));
+        const uint32_t S = min(a.parts, (tl.n + a.run - 1) / a.run);
+        const size_t at = (static_cast<size_t>(row) * a.hq + head) * a.parts;
+        for (uint32_t s0 = group / items; s0 < S; s0 += 4 * W) {  // four parts' loads at once
+            float2 e[4];
+            float4 x[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const size_t s = at + min(s0 + i * W, S - 1);
+                e[i] = marks[s];
+                x[i] = reinterpret_cast<const float4 *>(a.part + s * 64)[lane];
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                // A part without a key of the row, or with scores of -infinity alone, has no sums; one of NaN scores alone has no
+                // reference either, but a sum that is NaN.
+                if (s0 + i * W >= S || (e[i].x == INFINITY && e[i].y == 0.0f)) continue;
+                const float mn = fminf(m, e[i].x);
+                const float f = m == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mn - m), k = __builtin_amdgcn_exp2f(mn - e[i].x);
+                m = mn;
+                l = fmaf(l, f, e[i].y * k);
+                v.x = fmaf(v.x, f, x[i].x * k);
+                v.y = fmaf(v.y, f, x[i].y * k);
+                v.z = fmaf(v.z, f, x[i].z * k);
+                v.w = fmaf(v.w, f, x[i].w * k);
+            }
+        }
+    }
+    if (W > 1) {
+        acc[group][lane] = v;
+        if (lane == 0) {
+            sums[group] = l;
+            ms[group] = m;
+        }
+        __syncthreads();
+        if (group < items) {
+            m = INFINITY;
+            for (uint32_t g = group; g < AJ_GROUPS; g += items) m = fminf(m, ms[g]);
+            l = 0.0f;
+            v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t g = group; g < AJ_GROUPS; g += items) {
+                const float f = ms[g] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - ms[g]);
+                const float4 x = acc[g][lane];
+                l = fmaf(sums[g], ms[g] == INFINITY ? 1.0f : f, l);  // (0, or NaN, without a reference)
+                v.x = fmaf(x.x, f, v.x);
+                v.y = fmaf(x.y, f, v.y);
+                v.z = fmaf(x.z, f, v.z);
+                v.w = fmaf(x.w, f, v.w);
+            }
+        }
+    }
+    const bool have = group < items && locate(group, b, row, head, slot);
+    const float f = 1.0f / l;
+    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+    const bool good = fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY;
+    uint64_t bad = __ballot(have && !good);
+    if (have && !((bad >> (threadIdx.x & 48)) & 0xFFFF)) reinterpret_cast<float4 *>(a.out + static_cast<size_t>(row) * a.ldo + head * 64)[lane] = v;
+    while (bad) {  // such rows once more, each from its own keys alone, by the whole wave
+        const uint32_t g = (__ffsll(static_cast<unsigned long long>(bad)) - 1) / 16;
+        bad &= ~(0xFFFFull << (16 * g));
+        locate(threadIdx.x / 64 * 4 + g, b, row, head, slot);
+        attend_wave<CT>(a, b, row, head, slot);
+    }
+}
+
+template <int CT>
+int launch_join(const WindowArgs &a, hipStream_t stream) {
+    const uint32_t items = AJ_GROUPS >> a.join_log, all = a.rows.B * a.rows.T * a.hq;
+    hipLaunchKernelGGL(window_join_kernel<CT>, dim3((all + items - 1) / items), dim3(AJ_THREADS), 0, stream, a);
+    return check_launch("attention window (join)");
 }
 
 template <int CT, bool PAGED, int PIECES>
-int launch_tiles(const WindowArgs &a, const WindowPlan &p, hipStream_t stream) {
+int launch_few(const WindowArgs &a, const WindowPlan &p, hipStream_t stream) {
     const dim3 grid(a.rows.B * a.seq_tiles, a.hkv, a.parts), block(64 * p.waves);
     if (a.parts > 1) hipLaunchKernelGGL((attention_window_kernel<CT, PAGED, PIECES, true, AW_FEW>), grid, block, 0, stream, a);
     else if (p.waves == AW_FEW) hipLaunchKernelGGL((attention_window_kernel<CT, PAGED, PIECES, false, AW_FEW>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((attention_window_kernel<CT, PAGED, PIECES, false, AW_WAVES>), grid, block, 0, stream, a);
     const int rc = check_launch("attention window");
-    if (rc || a.parts == 1) return rc;
-    hipLaunchKernelGGL(window_join_kernel<CT>, dim3(a.rows.B * a.rows.T, a.hq), dim3(64 * std::min(AJ_WAVES, (a.parts + 1) / 2)), 0, stream, a);
-    return check_launch("attention window (join)");
+    return rc || a.parts == 1 ? rc : launch_join<CT>(a, stream);
+}
+
+template <int CT, bool PAGED>
+int launch_rows(const WindowArgs &a, const WindowPlan &p, hipStream_t stream) {
+    const uint32_t groups = a.rows.B * a.hkv;
+    const dim3 grid((a.by_xcd ? (groups + 7) / 8 * 8 : groups) * a.seq_tiles * a.parts), block(64 * p.waves);
+    if (a.parts > 1) {
+        if (p.keys == 1) hipLaunchKernelGGL((window_rows_kernel<CT, PAGED, true, 1>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((window_rows_kernel<CT, PAGED, true, 2>), grid, block, 0, stream, a);
+    } else if (p.keys == 1) {
+        hipLaunchKernelGGL((window_rows_kernel<CT, PAGED, false, 1>), grid, block, 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((window_rows_kernel<CT, PAGED, false, 2>), grid, block, 0, stream, a);
+    }
+    const int rc = check_launch("attention window (rows)");
+    return rc || a.parts == 1 ? rc : launch_join<CT>(a, stream);
 }
 
 template <int CT>
 int launch_kind(const WindowArgs &a, const WindowPlan &p, hipStream_t stream) {
+    if (p.shared) return a.kv.table ? launch_rows<CT, true>(a, p, stream) : launch_rows<CT, false>(a, p, stream);
     constexpr int PIECES = Raw<CT>::TK / 16;
-    if (!a.kv.table) return launch_tiles<CT, false, 1>(a, p, stream);
+    if (!a.kv.table) return launch_few<CT, false, 1>(a, p, stream);
     // Pages that hold whole tiles: one page a tile.
-    if (a.kv.page_len % Raw<CT>::TK == 0) return launch_tiles<CT, true, 1>(a, p, stream);
-    return launch_tiles<CT, true, PIECES>(a, p, stream);
+    if (a.kv.page_len % Raw<CT>::TK == 0) return launch_few<CT, true, 1>(a, p, stream);
+    return launch_few<CT, true, PIECES>(a, p, stream);
 }
 
 }  // namespace
@@ -582,10 +970,18 @@ int launch_kind(const WindowArgs &a, const WindowPlan &p, hipStream_t stream) {
 // fits wherever the call runs.
 WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window, uint32_t sinks, int ct) {
     const uint64_t tk = ct == DT_F32 ? Raw<DT_F32>::TK : Raw<DT_F8>::TK, cus = 256;
-    WindowPlan p{AW_WAVES, AW_WAVES, 1, 0};
+    WindowPlan p{AW_WAVES, AW_WAVES, 1, 0, false, false};
+    len_max = std::min(len_max, 1u << 30);  // a sequence has no more slots
     const uint64_t seen = window ? static_cast<uint64_t>(window) + sinks + T - 1 : len_max;
     const uint64_t own = std::max<uint64_t>(1, std::min<uint64_t>(len_max, seen));  // keys a row tile attends at most
     const uint64_t rows = static_cast<uint64_t>(T) * (hq / hkv), heads = static_cast<uint64_t>(B) * hkv;
+#ifdef WINDOW_SWEEP
+    if (const char *e = getenv("MT_PLAN")) {  // shared, waves, keys, parts, run, xcd
+        unsigned v[6];
+        sscanf(e, "%u,%u,%u,%u,%u,%u", v, v + 1, v + 2, v + 3, v + 4, v + 5);
+        return WindowPlan{v[1], v[2], v[3], v[4], v[0] != 0, v[5] != 0};
+    }
+#endif
     auto groups = [&](uint64_t waves, uint64_t keys) { return heads * ((rows + waves / keys * 16 - 1) / (waves / keys * 16)); };
     if (rows > 16 && groups(AW_WAVES, AW_WAVES) > cus) {
         p.waves = p.keys = AW_FEW;
@@ -609,10 +1005,14 @@ int launch_attention_window(const WindowArgs &args, const WindowPlan &p, int ct,
     a.keys = p.keys;
     a.parts = p.parts;
     a.run = p.run;
-    const uint32_t span = p.waves / p.keys * 16;
-    a.seq_tiles = (a.rows.T * a.group + span - 1) / span;
-    int rc = check_grid("attention window", static_cast<uint64_t>(a.rows.B) * a.seq_tiles, 64 * p.waves);
-    if (!rc && p.parts > 1) rc = check_grid("attention window (join)", static_cast<uint64_t>(a.rows.B) * a.rows.T, 64 * AJ_WAVES);
+    a.span = p.waves / p.keys * 16;
+    a.by_xcd = p.by_xcd;
+    const uint64_t tiles = (static_cast<uint64_t>(a.rows.T) * a.group + a.span - 1) / a.span, groups = static_cast<uint64_t>(a.rows.B) * a.hkv;
+    a.seq_tiles = static_cast<uint32_t>(tiles);
+    int rc = p.shared ? check_grid("attention window (rows)", (groups + 7) / 8 * 8 * tiles * p.parts, 64 * p.waves)
+                      : check_grid("attention window", a.rows.B * tiles, 64 * p.waves);
+    while (a.join_log < 4 && (4u << a.join_log) < p.parts) a.join_log++;  // about four parts a group
+    if (!rc && p.parts > 1) rc = check_grid("attention window (join)", ((static_cast<uint64_t>(a.rows.B) * a.rows.T * a.hq) << a.join_log) / AJ_GROUPS + 1, AJ_THREADS);
     if (rc) return rc;
     if (ct == DT_F32) return launch_kind<DT_F32>(a, p, stream);
     if (ct == DT_F16) return launch_kind<DT_F16>(a, p, stream);

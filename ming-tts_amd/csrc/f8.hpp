@@ -121,7 +121,10 @@ struct WindowArgs {
     float *part;    // split keys: [B T, hq, parts] sums of 64 and behind them as many pairs (minus the maximum, the weights' sum)
     uint32_t parts, run;  // parts of a row tile's keys, and the key tiles of each (the last: all that is left)
     uint32_t keys;        // waves of a workgroup that share rows and split their keys (the rest: other rows)
-    uint32_t seq_tiles;   // row tiles of a sequence and key head
+    uint32_t span;        // rows of a workgroup
+    uint32_t seq_tiles;   // workgroups of a sequence and key head, times parts
+    bool by_xcd;          // rows of prompts: a sequence's and key head's workgroups on one XCD
+    uint32_t join_log;    // groups of lanes that join a row's parts: 2^join_log
     uint32_t group, group_magic;  // as in SharedArgs
 };
 
@@ -129,6 +132,8 @@ struct WindowArgs {
 struct WindowPlan {
     uint32_t waves, keys;  // waves of a workgroup, those that share rows and split their keys
     uint32_t parts, run;   // parts of 1: one pass; more: joined by a second kernel
+    bool shared;           // rows of prompts: the waves share their keys in LDS
+    bool by_xcd;
 };
 
 // How mt_attention_shared places its work (shared_plan).
