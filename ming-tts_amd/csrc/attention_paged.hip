@@ -281,24 +281,41 @@ __device__ __forceinline__ void weights8(const float *x, u32x4v *p) {
 // The keys (values) of a tile's pieces, whose spans lanes `first` and on hold; zeros, which the buffers' bounds give, for slots that
 // no row sees and without a page.
 template <int CT, int PIECES>
-__device__ __forceinline__ void load_keys(Raw<CT> &r, const WindowArgs &a, const Spans &p, uint32_t first, uint32_t l16, uint32_t g) {
+__device__ __forceinline__ void load_keys(Raw<CT> &r, const WindowArgs &a, const Spans &p, uint32_t first, uint32_t lane) {
     constexpr uint32_t ROW = Cached<CT>::ROW;
-    constexpr int GROUPS = 2 * Raw<CT>::SUB, EACH = GROUPS / PIECES;  // groups of 16 keys, those of a piece
+    constexpr int GROUPS = 2 * Raw<CT>::SUB, EACH = GROUPS / PIECES, LOADS = Kind<CT>::KW;  // groups of 16 keys, those of a piece; loads of a group
 #pragma unroll
     for (int i = 0; i < PIECES; i++) {
         const __amdgpu_buffer_rsrc_t b = span_of(static_cast<const char *>(a.kv.k) + p.at(first + i), p.rows(first + i) * ROW);
 #pragma unroll
-        for (int u = 0; u < EACH; u++)
-#pragma unroll
-            for (int w = 0; w < Kind<CT>::KW; w++)
-                r.k[(EACH * i + u) * Kind<CT>::KW + w] =
-                    __builtin_amdgcn_raw_buffer_load_b128(b, l16 * ROW + 16 * Cached<CT>::ES * g + 16 * ROW * u + 16 * w, 0, 0);
+        for (int u = 0; u < EACH * LOADS; u++) r.k[EACH * LOADS * i + u] = __builtin_amdgcn_raw_buffer_load_b128(b, 16 * lane + 1024 * u, 0, 0);
         if constexpr (CT == DT_F8) {
             const __amdgpu_buffer_rsrc_t s = span_of(a.kv.ks + p.scale(first + i), p.rows(first + i));
 #pragma unroll
-            for (int u = 0; u < EACH; u++) r.ks[EACH * i + u] = __builtin_amdgcn_raw_buffer_load_b8(s, l16 + 16 * u, 0, 0);
+            for (int u = 0; u < EACH; u++) r.ks[EACH * i + u] = __builtin_amdgcn_raw_buffer_load_b8(s, (lane & 15) + 16 * u, 0, 0);
         }
     }
+}
+// Loaded so, whole rows side by side (the loads of a wave whose neighbouring lanes are of different rows take the CU's address unit four
+// times as long), the keys change lanes in LDS: byte of chunk c (16 bytes) of a row, which keeps the same chunk of 16 rows in
+// different banks.
+template <int CT>
+__device__ __forceinline__ uint32_t key_at(uint32_t row, uint32_t c) {
+    const uint32_t f = CT == DT_F32 ? row & 15 : CT == DT_F16 ? (row >> 1) & 7 : (row >> 2) & 3;
+    return row * Cached<CT>::ROW + ((c ^ f) << 4);
+}
+template <int CT>
+__device__ __forceinline__ void turn_keys(Raw<CT> &r, char *lds, uint32_t lane) {
+    constexpr uint32_t CHUNKS = Cached<CT>::ROW / 16, ROWS = 64 / CHUNKS;
+    constexpr int N = 2 * Raw<CT>::SUB * Kind<CT>::KW;
+#pragma unroll
+    for (int j = 0; j < N; j++) *reinterpret_cast<u32x4v *>(lds + key_at<CT>(j * ROWS + lane / CHUNKS, lane % CHUNKS)) = r.k[j];
+    wave_sync();
+#pragma unroll
+    for (int u = 0; u < 2 * Raw<CT>::SUB; u++)
+#pragma unroll
+        for (int w = 0; w < Kind<CT>::KW; w++)
+            r.k[u * Kind<CT>::KW + w] = *reinterpret_cast<const u32x4v *>(lds + key_at<CT>(16 * u + (lane & 15), (lane >> 4) * Kind<CT>::KW + w));
 }
 template <int CT, int PIECES>
 __device__ __forceinline__ void load_values(Raw<CT> &r, const WindowArgs &a, const Spans &p, uint32_t first, uint32_t l16, uint32_t g) {
@@ -339,7 +356,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     typedef Kind<CT> KD;
     constexpr int SUB = Raw<CT>::SUB, NK = 2 * SUB;
     constexpr uint32_t TK = Raw<CT>::TK;
-    __shared__ __attribute__((aligned(16))) float part[WAVES * 16 * AT_LD];
+    constexpr uint32_t AREA = TK * Cached<CT>::ROW > 16 * AT_LD * 4 ? TK * Cached<CT>::ROW : 16 * AT_LD * 4;  // a tile's keys, or a wave's sums
+    __shared__ __attribute__((aligned(16))) char lds[WAVES * AREA];
     __shared__ float ms[WAVES * 16], sums[WAVES * 16];
     const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -393,7 +411,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     if (i < end) {
         sp = spans(0, PAGED && a.window == 0 ? early : entry_of<PAGED>(a, b, slot_of(0)));
         __builtin_amdgcn_sched_barrier(0);  // in this order, as in the loop, or its first wait is for all of them
-        load_keys<CT, PIECES>(raw, a, sp, 0, l16, g);
+        load_keys<CT, PIECES>(raw, a, sp, 0, lane);
         __builtin_amdgcn_sched_barrier(0);
         load_values<CT, PIECES>(raw, a, sp, 0, l16, g);
         __builtin_amdgcn_sched_barrier(0);
@@ -404,6 +422,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     Sums m;
     for (; i < end; i += a.keys, q++) {
         const uint32_t k0 = tl.at(i) * TK, none = PAGED ? static_cast<uint32_t>(sp.holes >> (q % EACH * PIECES)) & ((1u << PIECES) - 1) : 0;
+        turn_keys<CT>(raw, lds + wave * AREA, lane);
         f32x4v s[NK];
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
@@ -437,7 +456,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
         } else if (i + a.keys >= end) {
             sp.n = 0;
         }
-        load_keys<CT, PIECES>(raw, a, sp, at * PIECES, l16, g);
+        load_keys<CT, PIECES>(raw, a, sp, at * PIECES, lane);
 
         if (!((k0 >= tl.in_lo || k0 + TK <= a.sinks) && k0 + TK <= tl.in_hi) || none) {
             hide<NK>(s, k0, g, lo, hi, a.sinks, none, PIECES);
@@ -501,7 +520,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
 
     // The waves' parts of each row meet in wave order: a thread joins four dims of a row.
     {
-        float *p = part + (wave * 16 + l16) * AT_LD + 16 * g;
+        float *p = reinterpret_cast<float *>(lds + wave * AREA) + l16 * AT_LD + 16 * g;
 #pragma unroll
         for (int e = 0; e < 4; e++) *reinterpret_cast<float4 *>(p + 4 * e) = make_float4(m.o[0][e], m.o[1][e], m.o[2][e], m.o[3][e]);
         const float l = m.ls + __shfl_xor(m.ls, 16, 64), all = l + __shfl_xor(l, 32, 64);
@@ -528,7 +547,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
                 const uint32_t at = (w0 + w) * 16 + in;
                 mw[w] = ms[at];
                 sw[w] = sums[at];
-                v[w] = *reinterpret_cast<const float4 *>(part + at * AT_LD + d4);
+                v[w] = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(lds + (w0 + w) * AREA) + in * AT_LD + d4);
             }
 #pragma unroll
             for (uint32_t w = 0; w < N; w++) mk = fminf(mk, mw[w]);
