@@ -58,9 +58,11 @@ struct PagedRuns {
     }
 };
 
-// The workspace of a plan: its parts' sums of 64, maxima and weights' sums.
-uint64_t window_bytes(const WindowPlan &p, uint32_t B, uint32_t T, uint32_t hq) {
-    return p.parts > 1 ? static_cast<uint64_t>(B) * T * hq * p.parts * (64 + 2) * 4 : 0;
+// The workspace of a plan: its parts' sums, references and weights' sums, and their flags.
+uint64_t window_bytes(const WindowPlan &p, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv) {
+    if (p.parts <= 1) return 0;
+    const uint64_t rows = static_cast<uint64_t>(T) * (hq / hkv), tiles = static_cast<uint64_t>(B) * hkv * ((rows + 15) / 16);
+    return (static_cast<uint64_t>(B) * T * hq * 33 + tiles) * p.parts * 8;
 }
 
 // What mt_attention_paged and mt_attention_sinks check alike, behind their caches: `a` has those, `caches` their memory.
@@ -77,7 +79,7 @@ int attend(const char *who, WindowArgs &a, int ct, const Runs *caches, int n_cac
     for (int i = 0; i < n_caches; i++)
         if (meet(caches[i].p, caches[i].all(), out, ob)) return set_error(MT_EINVAL, "%s: out overlaps the caches", who);
     const WindowPlan plan = window_plan(B, T, hq, hkv, len_max ? len_max : a.kv.len, window, sinks, ct);
-    const uint64_t need = window_bytes(plan, B, T, hq);
+    const uint64_t need = window_bytes(plan, B, T, hq, hkv);
     if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return set_error(MT_EINVAL, "%s: needs %llu bytes of 16-byte aligned workspace, got %llu", who,
                          static_cast<unsigned long long>(need), static_cast<unsigned long long>(workspace ? workspace_bytes : 0));
@@ -140,7 +142,7 @@ int mt_rope_append_paged(const float *qkv, uint32_t ldq, uint32_t B, uint32_t T,
 uint64_t mt_attention_window_workspace(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window,
                                        uint32_t sinks, mt_dtype cache_t) {
     if (validate_heads("mt_attention_window_workspace", B, T, hq, hkv) || B == 0 || T == 0) return 0;
-    return window_bytes(window_plan(B, T, hq, hkv, len_max, window, sinks, cache_t), B, T, hq);
+    return window_bytes(window_plan(B, T, hq, hkv, len_max, window, sinks, cache_t), B, T, hq, hkv);
 }
 
 int mt_attention_paged(const float *q, uint32_t ldq, uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, const uint32_t *pos,

@@ -7,7 +7,8 @@
 //   - One wave a row and query head: 64 keys at a time, each lane a key's score, then each lane a dim's sum, an online softmax
 //     in fp32.
 #include <algorithm>
-#include <cstdlib>
+#include <atomic>
+#include <chrono>
 #include <type_traits>
 
 #include "attend_tiles.hpp"
@@ -350,6 +351,106 @@ __device__ __forceinline__ void load_values(Raw<CT> &r, const WindowArgs &a, con
 
 constexpr uint32_t AW_WAVES = 8, AW_FEW = 4;  // waves of a workgroup
 
+// Split keys: the parts of a row tile meet in the workgroup that ends last.  Their sums are written and read with device scope, past
+// the XCDs' L2s, which do not see each other's: a release and an acquire of all that an L2 holds (fences) made 64 sequences of up to
+// 4096 keys 56 us where this takes 20.
+__device__ __forceinline__ void put(uint64_t *p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t get(const uint64_t *p) { return __hip_atomic_load(const_cast<uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float low(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t two(float a, float b) { return __float_as_uint(a) | static_cast<uint64_t>(__float_as_uint(b)) << 32; }
+
+// Part `mine` of `n` of a unit is stored: are all?  A part's flag holds the call's tag once it is; the workgroups that see all (the
+// last one does, since each looks once its own flag stands) take the flags back, so that a replay of the call finds none set, and
+// join, to the same bits.  Whatever else the flags' memory holds is no tag: it is a random number of 64 bits.
+__device__ __forceinline__ bool all_there(uint64_t *flags, uint32_t mine, uint32_t n, uint64_t tag, uint32_t *said) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // each wave's stores stand
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        if (threadIdx.x == 0) put(flags + mine, tag);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        bool all = true;
+        for (uint32_t i = threadIdx.x; i < n; i += 64) all = all && get(flags + i) == tag;
+        all = __all(all);
+        if (threadIdx.x == 0) *said = all;
+    }
+    __syncthreads();
+    const bool last = *said != 0;
+    if (last)
+        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) put(flags + i, 0);
+    return last;
+}
+
+// The S parts of rows [r0, r1) of a tile joined.  A row's are taken by W groups of 16 lanes, every W-th part each, which meet in LDS
+// in their order; a lane has four dims.
+template <int CT, int WAVES>
+__device__ __forceinline__ void join_parts(const WindowArgs &a, uint32_t b, uint32_t kvh, uint32_t r0, uint32_t r1, uint32_t S, uint64_t pos, char *lds) {
+    constexpr uint32_t GROUPS = WAVES * 4, BATCH = 8;
+    const uint32_t lane = threadIdx.x & 15, group = threadIdx.x / 16, n = r1 - r0;
+    const uint32_t items = n > 8 ? 16 : n > 4 ? 8 : n > 2 ? 4 : n > 1 ? 2 : 1, W = GROUPS / items, it = group % items;
+    const uint32_t r = r0 + it, t = by_group(a, r), head = kvh * a.group + r - t * a.group;
+    const size_t row = static_cast<size_t>(b) * a.rows.T + t;
+    const bool have = it < n;
+    float m = INFINITY, l = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    // (the sums of parts before: brought to a smaller mark; a part without a key of the row, or with scores of -infinity alone, has no sums;
+    // one of NaN scores alone has no reference either, but a sum that is NaN)
+    auto add = [&](float pm, float pl, float4 x) {
+        if (pm == INFINITY && pl == 0.0f) return;
+        const float mn = fminf(m, pm), f = m == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mn - m), k = __builtin_amdgcn_exp2f(mn - pm);
+        m = mn;
+        l = fmaf(l, f, pl * k);
+        v.x = fmaf(v.x, f, x.x * k);
+        v.y = fmaf(v.y, f, x.y * k);
+        v.z = fmaf(v.z, f, x.z * k);
+        v.w = fmaf(v.w, f, x.w * k);
+    };
+    if (have) {
+        const size_t at = (row * a.hq + head) * a.parts;
+        const uint64_t *marks = reinterpret_cast<const uint64_t *>(a.part + static_cast<size_t>(a.rows.B) * a.rows.T * a.hq * a.parts * 64) + at;
+        const uint64_t *sums = reinterpret_cast<const uint64_t *>(a.part + at * 64) + 2 * lane;
+        for (uint32_t s0 = group / items; s0 < S; s0 += BATCH * W) {  // so many parts' loads at once
+            uint64_t e[BATCH], x[BATCH][2];
+#pragma unroll
+            for (uint32_t i = 0; i < BATCH; i++) {
+                const size_t p = s0 + i * W;
+                e[i] = two(INFINITY, 0.0f);
+                x[i][0] = x[i][1] = 0;
+                if (p < S) {
+                    e[i] = get(marks + p);
+                    x[i][0] = get(sums + p * 32);
+                    x[i][1] = get(sums + p * 32 + 1);
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < BATCH; i++) add(low(e[i]), high(e[i]), make_float4(low(x[i][0]), high(x[i][0]), low(x[i][1]), high(x[i][1])));
+        }
+    }
+    if (W > 1) {
+        float4 *acc = reinterpret_cast<float4 *>(lds);
+        float2 *mark = reinterpret_cast<float2 *>(lds + GROUPS * 256);
+        acc[group * 16 + lane] = v;
+        if (lane == 0) mark[group] = make_float2(m, l);
+        __syncthreads();
+        if (threadIdx.x / 64 * 4 >= items) return;  // (whole waves)
+        m = INFINITY;
+        l = 0.0f;
+        v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t g = group; g < GROUPS; g += items) add(mark[g].x, mark[g].y, acc[g * 16 + lane]);
+    }
+    const float f = 1.0f / l;
+    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+    const bool good = fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY;
+    const bool own = have && group < items;
+    uint64_t bad = __ballot(own && !good);
+    if (own && !((bad >> (threadIdx.x & 48)) & 0xFFFF)) reinterpret_cast<float4 *>(a.out + row * a.ldo + head * 64)[lane] = v;
+    while (bad) {  // rows with an output that is not finite (or without a weight) once more, each from its own keys alone
+        const uint32_t x = (__ffsll(static_cast<unsigned long long>(bad)) - 1) / 16, rx = r0 + threadIdx.x / 64 * 4 + x, tx = by_group(a, rx);
+        bad &= ~(0xFFFFull << (16 * x));
+        attend_wave<CT>(a, b, b * a.rows.T + tx, kvh * a.group + rx - tx * a.group, pos + tx);
+    }
+}
+
 // Few rows.  Grid: x the sequences' row tiles, y the key heads, z the parts.
 template <int CT, bool PAGED, int PIECES, bool APART, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) void attention_window_kernel(WindowArgs a) {
@@ -566,11 +667,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
         else if (a.keys == 2) join(std::integral_constant<uint32_t, 2>{});
         else join(std::integral_constant<uint32_t, 1>{});
         if constexpr (APART) {
-            const size_t at = (row * a.hq + headj) * a.parts + blockIdx.z;
-            float2 *ml = reinterpret_cast<float2 *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * a.parts * 64);
             if (rj < r1) {
-                *reinterpret_cast<float4 *>(a.part + at * 64 + d4) = acc;
-                if (d4 == 0) ml[at] = make_float2(mk, l);
+                const size_t at = (row * a.hq + headj) * a.parts + blockIdx.z;
+                uint64_t *to = reinterpret_cast<uint64_t *>(a.part + at * 64 + d4);
+                put(to, two(acc.x, acc.y));
+                put(to + 1, two(acc.z, acc.w));
+                if (d4 == 0) put(reinterpret_cast<uint64_t *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * a.parts * 64) + at, two(mk, l));
             }
         } else {
             const float f = 1.0f / l;
@@ -585,12 +687,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
             }
         }
     }
+    if constexpr (APART) {
+        __shared__ uint32_t said;
+        const uint32_t S = min(a.parts, (tl.n + a.run - 1) / a.run);  // the tile's parts
+        const size_t unit = static_cast<size_t>(blockIdx.x) * a.hkv + kvh;
+        uint64_t *flags = reinterpret_cast<uint64_t *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * a.parts * 66) + unit * a.parts;
+        if (!all_there(flags, blockIdx.z, S, a.tag, &said)) return;
+        join_parts<CT, WAVES>(a, b, kvh, r0, r1, S, pos, lds);
+    }
 }
 
 // ------------------------------------------------------------- many rows --
 
-// Rows of prompts.  A workgroup is WR x WK waves: WR of them have 16 rows each, and WK groups of them take every WK-th tile of
-// keys, which the group's waves share in LDS, 16 bits a value (as NC pieces), converted once.
+// Rows of prompts.  The WR waves of a workgroup have 16 rows each and share its tiles of keys in LDS, 16 bits a value (as NC pieces),
+// converted once.
 typedef short s16x4v __attribute__((ext_vector_type(4)));
 constexpr uint32_t WR = 4;
 
@@ -610,25 +720,25 @@ __device__ __forceinline__ uint32_t chunk_at(uint32_t row, uint32_t c) {
     return row * 128 + ((c ^ (((row >> 1) & 3) << 1 | ((row >> 3) & 1))) << 4);
 }
 
-template <int CT, bool PAGED, bool APART, int WK>
-__global__ __launch_bounds__(64 * WR * WK, CT == DT_F32 && WK == 2 ? 2 : 3) void window_rows_kernel(WindowArgs a) {
+template <int CT, bool PAGED>
+__global__ __launch_bounds__(64 * WR, 3) void window_rows_kernel(WindowArgs a) {
     typedef Kind<CT> KD;
     typedef Staged<CT> SD;
     constexpr uint32_t TK = SD::TK, ROW = Cached<CT>::ROW, SPAN = WR * 16;
     constexpr int NK = TK / 16, LOADS = 2 * SD::HALF / WR;
     static_assert(2 * SD::HALF % WR == 0, "whole loads a wave");
-    __shared__ __attribute__((aligned(16))) char lds[2][WK][2][SD::TILE];  // two steps' tiles, keys and values
+    __shared__ __attribute__((aligned(16))) char lds[2][2][SD::TILE];  // two tiles, keys and values of each
     const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave / WR, wr = wave % WR;
+    const uint32_t wr = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t G = a.group, T = a.rows.T;
 
     // Workgroups go to the XCDs in turn: those of one sequence and key head go to one, whose L2 then fetches their keys once.
     const uint32_t xcds = a.by_xcd ? 8 : 1, xcd = blockIdx.x % xcds, item = blockIdx.x / xcds;
-    const uint32_t turn = item / a.parts, part = item - turn * a.parts, lap = turn / a.seq_tiles, group = lap * xcds + xcd;
+    const uint32_t lap = item / a.seq_tiles, group = lap * xcds + xcd;
     const uint32_t b = group / a.hkv, kvh = group - b * a.hkv;
     if (b >= a.rows.B) return;
     const uint32_t n = a.rows.counts ? min(a.rows.counts[b], T) : T;
-    const uint32_t r0 = (a.seq_tiles - 1 - (turn - lap * a.seq_tiles)) * SPAN, r1 = min(n * G, r0 + SPAN);  // the longest first
+    const uint32_t r0 = (a.seq_tiles - 1 - (item - lap * a.seq_tiles)) * SPAN, r1 = min(n * G, r0 + SPAN);  // the longest first
     if (r0 >= r1) return;
     // The lane's row (all four g's the same one).
     const uint32_t rw = r0 + wr * 16, r = rw + l16, t = by_group(a, r), head = kvh * G + r - t * G;
@@ -638,26 +748,20 @@ __global__ __launch_bounds__(64 * WR * WK, CT == DT_F32 && WK == 2 ? 2 : 3) void
     const uint64_t pos = a.rows.pos ? a.rows.pos[b] : 0u;
     uint32_t lo = 0, hi = 0, first;
     if (have) row_keys(a, pos + t, first, lo, hi);
-    // The workgroup's tiles, its part of them [t0, t1), and the wave's rows' keys.
+    // The workgroup's tiles, one a step, and the wave's rows' keys.
     const Tiles tl = tiles_of<TK>(a, b, by_group(a, r0), by_group(a, r1 - 1));
     Tiles mine{};
     if (rw < r1) mine = tiles_of<TK>(a, b, by_group(a, rw), by_group(a, min(rw + 16, r1) - 1));
-    uint32_t t0 = 0, t1 = tl.n;
-    if constexpr (APART) {
-        t0 = min(t1, part * a.run);
-        if (part + 1 < a.parts) t1 = min(t1, t0 + a.run);
-        if (t0 == t1) return;
-    }
-    const uint32_t steps = (t1 - t0 + WK - 1) / WK;
+    const uint32_t steps = tl.n;
 
     // A step's tile on its way: this wave's chunks of it.  The spans of EACH steps' tiles, and the entries of the next ones.
     u32x4v raw[LOADS];
     uint32_t scales[LOADS];
     constexpr uint32_t EACH = 64 / SD::RUNS;
-    auto tile_of = [&](uint32_t step) { return tl.at(min(t0 + step * WK + wk, t1 - 1)); };
+    auto tile_of = [&](uint32_t step) { return tl.at(min(step, steps - 1)); };
     auto slot_of = [&](uint32_t step) { return tile_of(step + lane / SD::RUNS) * TK + lane % SD::RUNS * 16; };
     auto spans = [&](uint32_t step, uint32_t entry) {
-        return span_run<CT, PAGED, 16>(a, tl, kvh, slot_of(step), t0 + (step + lane / SD::RUNS) * WK + wk < t1, entry);
+        return span_run<CT, PAGED, 16>(a, tl, kvh, slot_of(step), step + lane / SD::RUNS < steps, entry);
     };
     auto request = [&](const Spans &sp, uint32_t step) {
 #pragma unroll
@@ -675,7 +779,7 @@ __global__ __launch_bounds__(64 * WR * WK, CT == DT_F32 && WK == 2 ? 2 : 3) void
 #pragma unroll
         for (int j = 0; j < LOADS; j++) {
             const uint32_t id = j * WR + wr, x = id % SD::HALF * SD::ROWS + lane / SD::CHUNKS, c = lane % SD::CHUNKS;
-            char *tile = lds[buf][wk][id >= SD::HALF ? 1 : 0];
+            char *tile = lds[buf][id >= SD::HALF ? 1 : 0];
             const u32x4v w = raw[j];
             if constexpr (CT == DT_F16) {
                 *reinterpret_cast<u32x4v *>(tile + chunk_at(x, c)) = w;
@@ -717,8 +821,8 @@ __global__ __launch_bounds__(64 * WR * WK, CT == DT_F32 && WK == 2 ? 2 : 3) void
             none_next = holes(sp, step + 1);
         }
         const uint32_t k0 = tile_of(step) * TK;
-        if (t0 + step * WK + wk < t1 && rw < r1 && k0 < mine.hi && (k0 < a.sinks || k0 + TK > mine.lo)) {
-            const char *kt = lds[buf][wk][0], *vt = lds[buf][wk][1];
+        if (rw < r1 && k0 < mine.hi && (k0 < a.sinks || k0 + TK > mine.lo)) {
+            const char *kt = lds[buf][0], *vt = lds[buf][1];
             f32x4v s[NK];
             {
                 u32x4v kf[NK][2][KD::NC];
@@ -791,41 +895,6 @@ __global__ __launch_bounds__(64 * WR * WK, CT == DT_F32 && WK == 2 ? 2 : 3) void
 
     m.ls += __shfl_xor(m.ls, 16, 64);
     m.ls += __shfl_xor(m.ls, 32, 64);
-    float mark = m.mark();
-    if constexpr (WK > 1) {  // the waves of a row meet in wave order, in the first of them
-        constexpr uint32_t WORDS = 18 * 64;
-        float *hand = reinterpret_cast<float *>(&lds[0][0][0][0]);  // [wave - WR][18][64]
-        static_assert(sizeof(lds) >= WR * (WK - 1) * WORDS * 4, "the hand-over fits the tiles' memory");
-        if (wk > 0) {
-            float *p = hand + (wave - WR) * WORDS + lane;
-#pragma unroll
-            for (int e = 0; e < 16; e++) p[e * 64] = m.o[e / 4][e % 4];
-            p[16 * 64] = mark;
-            p[17 * 64] = m.ls;
-        }
-        __syncthreads();
-        if (wk > 0) return;
-#pragma unroll
-        for (int w = 1; w < WK; w++) {
-            const float *p = hand + (wave + (w - 1) * WR) * WORDS + lane;
-            const float other = p[16 * 64], both = fminf(mark, other);
-            // (sums without a reference are zeros, or NaN)
-            const float f0 = mark == INFINITY ? 1.0f : __builtin_amdgcn_exp2f(both - mark), f1 = other == INFINITY ? 1.0f : __builtin_amdgcn_exp2f(both - other);
-            m.ls = fmaf(p[17 * 64], f1, m.ls * f0);
-#pragma unroll
-            for (int e = 0; e < 16; e++) m.o[e / 4][e % 4] = fmaf(p[e * 64], f1, m.o[e / 4][e % 4] * f0);
-            mark = both;
-        }
-    }
-    if constexpr (APART) {
-        if (!have) return;
-        const size_t at = (row * a.hq + head) * a.parts + part;
-        float2 *ml = reinterpret_cast<float2 *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * a.parts * 64);
-#pragma unroll
-        for (int d = 0; d < 4; d++) *reinterpret_cast<f32x4v *>(a.part + at * 64 + 16 * d + 4 * g) = m.o[d];
-        if (g == 0) ml[at] = make_float2(mark, m.ls);
-        return;
-    }
     const float f = 1.0f / m.ls;
     bool good = true;
 #pragma unroll
@@ -849,128 +918,22 @@ __global__ __launch_bounds__(64 * WR * WK, CT == DT_F32 && WK == 2 ? 2 : 3) void
     }
 }
 
-// The parts of a row and head joined, by 2^a.join_log groups of 16 lanes that take every such part each and meet in LDS in their
-// order; a lane has four dims.
-constexpr uint32_t AJ_THREADS = 256, AJ_GROUPS = AJ_THREADS / 16;
-
-template <int CT>
-__global__ __launch_bounds__(AJ_THREADS) void window_join_kernel(WindowArgs a) {
-    __shared__ __attribute__((aligned(16))) float4 acc[AJ_GROUPS][16];
-    __shared__ float sums[AJ_GROUPS], ms[AJ_GROUPS];
-    const uint32_t lane = threadIdx.x & 15, group = threadIdx.x / 16, W = 1u << a.join_log, items = AJ_GROUPS >> a.join_log;
-    const uint32_t all = a.rows.B * a.rows.T * a.hq;  // below 2^31
-    const float2 *marks = reinterpret_cast<const float2 *>(a.part + static_cast<size_t>(all) * a.parts * 64);
-    // Item `it` of the workgroup: a row and head, if the sequence has the row.
-    auto locate = [&](uint32_t it, uint32_t &b, uint32_t &row, uint32_t &head, uint64_t &slot) {
-        const uint32_t i = blockIdx.x * items + it;
-        row = i / a.hq;
-        head = i - row * a.hq;
-        return i < all && a.rows.at(row, b, slot);
-    };
-    uint32_t b, row, head;
-    uint64_t slot;
-    float m = INFINITY, l = 0.0f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (locate(group % items, b, row, head, slot)) {
-        // The parts that the row's workgroup has.
-        const uint32_t t = row - b * a.rows.T, kvh = head / a.group, r = t * a.group + head - kvh * a.group;
-        const uint32_t n = a.rows.counts ? min(a.rows.counts[b], a.rows.T) : a.rows.T, rw = r & ~(a.span - 1);
-        const Tiles tl = tiles_of<Raw<CT>::TK>(a, b, by_group(a, rw), by_group(a, min(rw + a.span, n * a.group) - 1));
-        const uint32_t S = min(a.parts, (tl.n + a.run - 1) / a.run);
-        const size_t at = (static_cast<size_t>(row) * a.hq + head) * a.parts;
-        for (uint32_t s0 = group / items; s0 < S; s0 += 4 * W) {  // four parts' loads at once
-            float2 e[4];
-            float4 x[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-                const size_t s = at + min(s0 + i * W, S - 1);
-                e[i] = marks[s];
-                x[i] = reinterpret_cast<const float4 *>(a.part + s * 64)[lane];
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-                // A part without a key of the row, or with scores of -infinity alone, has no sums; one of NaN scores alone has no
-                // reference either, but a sum that is NaN.
-                if (s0 + i * W >= S || (e[i].x == INFINITY && e[i].y == 0.0f)) continue;
-                const float mn = fminf(m, e[i].x);
-                const float f = m == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mn - m), k = __builtin_amdgcn_exp2f(mn - e[i].x);
-                m = mn;
-                l = fmaf(l, f, e[i].y * k);
-                v.x = fmaf(v.x, f, x[i].x * k);
-                v.y = fmaf(v.y, f, x[i].y * k);
-                v.z = fmaf(v.z, f, x[i].z * k);
-                v.w = fmaf(v.w, f, x[i].w * k);
-            }
-        }
-    }
-    if (W > 1) {
-        acc[group][lane] = v;
-        if (lane == 0) {
-            sums[group] = l;
-            ms[group] = m;
-        }
-        __syncthreads();
-        if (group < items) {
-            m = INFINITY;
-            for (uint32_t g = group; g < AJ_GROUPS; g += items) m = fminf(m, ms[g]);
-            l = 0.0f;
-            v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint32_t g = group; g < AJ_GROUPS; g += items) {
-                const float f = ms[g] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - ms[g]);
-                const float4 x = acc[g][lane];
-                l = fmaf(sums[g], ms[g] == INFINITY ? 1.0f : f, l);  // (0, or NaN, without a reference)
-                v.x = fmaf(x.x, f, v.x);
-                v.y = fmaf(x.y, f, v.y);
-                v.z = fmaf(x.z, f, v.z);
-                v.w = fmaf(x.w, f, v.w);
-            }
-        }
-    }
-    const bool have = group < items && locate(group, b, row, head, slot);
-    const float f = 1.0f / l;
-    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
-    const bool good = fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY;
-    uint64_t bad = __ballot(have && !good);
-    if (have && !((bad >> (threadIdx.x & 48)) & 0xFFFF)) reinterpret_cast<float4 *>(a.out + static_cast<size_t>(row) * a.ldo + head * 64)[lane] = v;
-    while (bad) {  // such rows once more, each from its own keys alone, by the whole wave
-        const uint32_t g = (__ffsll(static_cast<unsigned long long>(bad)) - 1) / 16;
-        bad &= ~(0xFFFFull << (16 * g));
-        locate(threadIdx.x / 64 * 4 + g, b, row, head, slot);
-        attend_wave<CT>(a, b, row, head, slot);
-    }
-}
-
-template <int CT>
-int launch_join(const WindowArgs &a, hipStream_t stream) {
-    const uint32_t items = AJ_GROUPS >> a.join_log, all = a.rows.B * a.rows.T * a.hq;
-    hipLaunchKernelGGL(window_join_kernel<CT>, dim3((all + items - 1) / items), dim3(AJ_THREADS), 0, stream, a);
-    return check_launch("attention window (join)");
-}
-
 template <int CT, bool PAGED, int PIECES>
 int launch_few(const WindowArgs &a, const WindowPlan &p, hipStream_t stream) {
     const dim3 grid(a.rows.B * a.seq_tiles, a.hkv, a.parts), block(64 * p.waves);
-    if (a.parts > 1) hipLaunchKernelGGL((attention_window_kernel<CT, PAGED, PIECES, true, AW_FEW>), grid, block, 0, stream, a);
+    if (a.parts > 1 && p.waves == AW_FEW) hipLaunchKernelGGL((attention_window_kernel<CT, PAGED, PIECES, true, AW_FEW>), grid, block, 0, stream, a);
+    else if (a.parts > 1) hipLaunchKernelGGL((attention_window_kernel<CT, PAGED, PIECES, true, AW_WAVES>), grid, block, 0, stream, a);
     else if (p.waves == AW_FEW) hipLaunchKernelGGL((attention_window_kernel<CT, PAGED, PIECES, false, AW_FEW>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((attention_window_kernel<CT, PAGED, PIECES, false, AW_WAVES>), grid, block, 0, stream, a);
-    const int rc = check_launch("attention window");
-    return rc || a.parts == 1 ? rc : launch_join<CT>(a, stream);
+    return check_launch("attention window");
 }
 
 template <int CT, bool PAGED>
 int launch_rows(const WindowArgs &a, const WindowPlan &p, hipStream_t stream) {
     const uint32_t groups = a.rows.B * a.hkv;
-    const dim3 grid((a.by_xcd ? (groups + 7) / 8 * 8 : groups) * a.seq_tiles * a.parts), block(64 * p.waves);
-    if (a.parts > 1) {
-        if (p.keys == 1) hipLaunchKernelGGL((window_rows_kernel<CT, PAGED, true, 1>), grid, block, 0, stream, a);
-        else hipLaunchKernelGGL((window_rows_kernel<CT, PAGED, true, 2>), grid, block, 0, stream, a);
-    } else if (p.keys == 1) {
-        hipLaunchKernelGGL((window_rows_kernel<CT, PAGED, false, 1>), grid, block, 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((window_rows_kernel<CT, PAGED, false, 2>), grid, block, 0, stream, a);
-    }
-    const int rc = check_launch("attention window (rows)");
-    return rc || a.parts == 1 ? rc : launch_join<CT>(a, stream);
+    const dim3 grid((a.by_xcd ? (groups + 7) / 8 * 8 : groups) * a.seq_tiles), block(64 * p.waves);
+    hipLaunchKernelGGL((window_rows_kernel<CT, PAGED>), grid, block, 0, stream, a);
+    return check_launch("attention window (rows)");
 }
 
 template <int CT>
@@ -984,6 +947,15 @@ int launch_kind(const WindowArgs &a, const WindowPlan &p, hipStream_t stream) {
 }
 
 }  // namespace
+
+// A number that no earlier call had and no memory holds but by a chance of 2^-63.
+static uint64_t new_tag() {
+    static std::atomic<uint64_t> state{static_cast<uint64_t>(std::chrono::system_clock::now().time_since_epoch().count()) ^ reinterpret_cast<uintptr_t>(&state)};
+    uint64_t x = state.fetch_add(0x9E3779B97F4A7C15ull, std::memory_order_relaxed);
+    x = (x ^ (x >> 30)) * 0xBF58476D1CE4E5B9ull;
+    x = (x ^ (x >> 27)) * 0x94D049BB133111EBull;
+    return (x ^ (x >> 31)) | 1;
+}
 
 // Where the work goes, from the sizes alone: 256 compute units are an MI355X's, not asked for, so that a workspace sized once
 // fits wherever the call runs.
@@ -1002,19 +974,26 @@ WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
     }
 #endif
     auto groups = [&](uint64_t waves, uint64_t keys) { return heads * ((rows + waves / keys * 16 - 1) / (waves / keys * 16)); };
-    if (rows > 16 && groups(AW_WAVES, AW_WAVES) > cus) {
+    const uint64_t wide = heads * ((rows + 16 * WR - 1) / (16 * WR)), units = groups(AW_WAVES, AW_WAVES);
+    if (rows > 16 && wide >= (ct == DT_F32 ? 2 * cus : 400)) {
+        p.shared = true;
+        p.waves = WR;
+        p.keys = 1;
+        p.by_xcd = heads % 8 == 0 || heads > 32;
+        return p;
+    }
+    if (rows > 16 && units > cus) {
         p.waves = p.keys = AW_FEW;
         while (p.keys > 1 && groups(AW_FEW, p.keys) > 4 * cus && own < 4 * tk * p.keys) p.keys /= 2;
         return p;
     }
-    const uint64_t all = groups(AW_WAVES, AW_WAVES);
-    const uint64_t share = all * own / (2 * cus), part = std::max<uint64_t>(share, 256);  // keys a workgroup, two a CU
-    const uint64_t so = std::min<uint64_t>(std::max<uint64_t>(1, own / part), 128);
-    const uint64_t longest = std::max<uint64_t>(share, own / so);
-    if (so > 1 && 2 * longest + 1200 < (all + cus - 1) / cus * own) {
-        p.waves = p.keys = AW_FEW;
-        p.parts = static_cast<uint32_t>(so);
-        p.run = static_cast<uint32_t>((own + so * tk - 1) / (so * tk));
+    if (units > cus) p.waves = p.keys = AW_FEW;
+    if (units <= 160 && own >= (ct == DT_F16 && units > 64 ? 2560 : 1536)) {
+        const uint64_t tiles = (own + tk - 1) / tk;
+        p.parts = static_cast<uint32_t>(
+            std::min<uint64_t>({64, own / 256, std::max<uint64_t>(cus / units, std::min<uint64_t>(8, (2 * cus + units - 1) / units))}));
+        p.run = static_cast<uint32_t>((tiles + p.parts - 1) / p.parts);
+        p.waves = p.keys = p.run * tk >= 2048 && units * p.parts <= cus / 2 ? AW_WAVES : AW_FEW;
     }
     return p;
 }
@@ -1028,10 +1007,9 @@ int launch_attention_window(const WindowArgs &args, const WindowPlan &p, int ct,
     a.by_xcd = p.by_xcd;
     const uint64_t tiles = (static_cast<uint64_t>(a.rows.T) * a.group + a.span - 1) / a.span, groups = static_cast<uint64_t>(a.rows.B) * a.hkv;
     a.seq_tiles = static_cast<uint32_t>(tiles);
-    int rc = p.shared ? check_grid("attention window (rows)", (groups + 7) / 8 * 8 * tiles * p.parts, 64 * p.waves)
+    int rc = p.shared ? check_grid("attention window (rows)", (groups + 7) / 8 * 8 * tiles, 64 * p.waves)
                       : check_grid("attention window", a.rows.B * tiles, 64 * p.waves);
-    while (a.join_log < 4 && (4u << a.join_log) < p.parts) a.join_log++;  // about four parts a group
-    if (!rc && p.parts > 1) rc = check_grid("attention window (join)", ((static_cast<uint64_t>(a.rows.B) * a.rows.T * a.hq) << a.join_log) / AJ_GROUPS + 1, AJ_THREADS);
+    if (p.parts > 1) a.tag = new_tag();
     if (rc) return rc;
     if (ct == DT_F32) return launch_kind<DT_F32>(a, p, stream);
     if (ct == DT_F16) return launch_kind<DT_F16>(a, p, stream);

@@ -118,13 +118,14 @@ struct WindowArgs {
     RowsArgs rows;
     PagedArgs kv;
     float scale;
-    float *part;    // split keys: [B T, hq, parts] sums of 64 and behind them as many pairs (minus the maximum, the weights' sum)
+    float *part;    // split keys: [B T, hq, parts] sums of 64, as many pairs (minus the reference, the weights' sum), and the flags
+                    // [row tiles, hkv, parts] that a part is there
+    uint64_t tag;    // the call's, which such flags hold
     uint32_t parts, run;  // parts of a row tile's keys, and the key tiles of each (the last: all that is left)
     uint32_t keys;        // waves of a workgroup that share rows and split their keys (the rest: other rows)
     uint32_t span;        // rows of a workgroup
     uint32_t seq_tiles;   // workgroups of a sequence and key head, times parts
     bool by_xcd;          // rows of prompts: a sequence's and key head's workgroups on one XCD
-    uint32_t join_log;    // groups of lanes that join a row's parts: 2^join_log
     uint32_t group, group_magic;  // as in SharedArgs
 };
 
