@@ -966,13 +966,6 @@ WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
     const uint64_t seen = window ? static_cast<uint64_t>(window) + sinks + T - 1 : len_max;
     const uint64_t own = std::max<uint64_t>(1, std::min<uint64_t>(len_max, seen));  // keys a row tile attends at most
     const uint64_t rows = static_cast<uint64_t>(T) * (hq / hkv), heads = static_cast<uint64_t>(B) * hkv;
-#ifdef WINDOW_SWEEP
-    if (const char *e = getenv("MT_PLAN")) {  // shared, waves, keys, parts, run, xcd
-        unsigned v[6];
-        sscanf(e, "%u,%u,%u,%u,%u,%u", v, v + 1, v + 2, v + 3, v + 4, v + 5);
-        return WindowPlan{v[1], v[2], v[3], v[4], v[0] != 0, v[5] != 0};
-    }
-#endif
     auto groups = [&](uint64_t waves, uint64_t keys) { return heads * ((rows + waves / keys * 16 - 1) / (waves / keys * 16)); };
     const uint64_t wide = heads * ((rows + 16 * WR - 1) / (16 * WR)), units = groups(AW_WAVES, AW_WAVES);
     if (rows > 16 && wide >= (ct == DT_F32 ? 2 * cus : 400)) {
