@@ -466,9 +466,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     const uint32_t G = a.group, T = a.rows.T, span = WAVES / a.keys * 16;  // rows of a workgroup
 
     // The workgroup's rows [r0, r1) of sequence b's rows (t, head of the group), the longest first.
-    const uint32_t kvh = blockIdx.y, b = a.seq_tiles == 1 ? blockIdx.x : blockIdx.x / a.seq_tiles;
+    // (A CU gets every 256th workgroup or so: each head and part begins at another sequence, or a CU would get all of a long one.)
+    uint32_t x = blockIdx.x + a.shift * (blockIdx.y + a.hkv * blockIdx.z);
+    if (x >= gridDim.x) x -= gridDim.x;
+    const uint32_t kvh = blockIdx.y, b = a.seq_tiles == 1 ? x : x / a.seq_tiles;
     const uint32_t n = a.rows.counts ? min(a.rows.counts[b], T) : T;
-    const uint32_t r0 = (a.seq_tiles - 1 - (blockIdx.x - b * a.seq_tiles)) * span, r1 = min(n * G, r0 + span);
+    const uint32_t r0 = (a.seq_tiles - 1 - (x - b * a.seq_tiles)) * span, r1 = min(n * G, r0 + span);
     if (r0 >= r1) return;
 
     // The lane's row (all four g's the same one) and its keys [lo, hi) and those before a.sinks.
@@ -690,7 +693,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     if constexpr (APART) {
         __shared__ uint32_t said;
         const uint32_t S = min(a.parts, (tl.n + a.run - 1) / a.run);  // the tile's parts
-        const size_t unit = static_cast<size_t>(blockIdx.x) * a.hkv + kvh;
+        const size_t unit = static_cast<size_t>(x) * a.hkv + kvh;
         uint64_t *flags = reinterpret_cast<uint64_t *>(a.part + static_cast<size_t>(a.rows.B) * T * a.hq * a.parts * 66) + unit * a.parts;
         if (!all_there(flags, blockIdx.z, S, a.tag, &said)) return;
         join_parts<CT, WAVES>(a, b, kvh, r0, r1, S, pos, lds);
@@ -983,8 +986,7 @@ WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
     if (units > cus) p.waves = p.keys = AW_FEW;
     if (units <= 160 && own >= (ct == DT_F16 && units > 64 ? 2560 : 1536)) {
         const uint64_t tiles = (own + tk - 1) / tk;
-        p.parts = static_cast<uint32_t>(
-            std::min<uint64_t>({64, own / 256, std::max<uint64_t>(cus / units, std::min<uint64_t>(8, (2 * cus + units - 1) / units))}));
+        p.parts = static_cast<uint32_t>(std::min<uint64_t>({64, own / 256, std::max<uint64_t>(cus / units, own >= 8192 ? 4 : 2)}));
         p.run = static_cast<uint32_t>((tiles + p.parts - 1) / p.parts);
         p.waves = p.keys = p.run * tk >= 2048 && units * p.parts <= cus / 2 ? AW_WAVES : AW_FEW;
     }
@@ -1000,6 +1002,7 @@ int launch_attention_window(const WindowArgs &args, const WindowPlan &p, int ct,
     a.by_xcd = p.by_xcd;
     const uint64_t tiles = (static_cast<uint64_t>(a.rows.T) * a.group + a.span - 1) / a.span, groups = static_cast<uint64_t>(a.rows.B) * a.hkv;
     a.seq_tiles = static_cast<uint32_t>(tiles);
+    a.shift = static_cast<uint32_t>(a.rows.B * tiles / (static_cast<uint64_t>(a.hkv) * p.parts));
     int rc = p.shared ? check_grid("attention window (rows)", (groups + 7) / 8 * 8 * tiles, 64 * p.waves)
                       : check_grid("attention window", a.rows.B * tiles, 64 * p.waves);
     if (p.parts > 1) a.tag = new_tag();

@@ -125,6 +125,7 @@ struct WindowArgs {
     uint32_t keys;        // waves of a workgroup that share rows and split their keys (the rest: other rows)
     uint32_t span;        // rows of a workgroup
     uint32_t seq_tiles;   // workgroups of a sequence and key head, times parts
+    uint32_t shift;       // row tiles that a key head's and part's first workgroup is ahead of the one before
     bool by_xcd;          // rows of prompts: a sequence's and key head's workgroups on one XCD
     uint32_t group, group_magic;  // as in SharedArgs
 };
