@@ -4,8 +4,24 @@
 // out = sum_j p_j v_j / sum_j p_j with p_j = exp(s_j - max s), s_j = scale q . k_j, over the slots j <= i of a row at slot i that have
 // j > i - window or j < sinks.
 //
-//   - One wave a row and query head: 64 keys at a time, each lane a key's score, then each lane a dim's sum, an online softmax
-//     in fp32.
+// Scores and weights on the matrix cores (16 x 16 x 32), to about fp32's accuracy: q and the weights p as two fp16 pieces against fp16
+// caches (K, V exact), as three bf16 pieces against 8-bit ones (K, V times a power of two exact in bf16) and against fp32 ones (three
+// pieces too, the six products that matter).  A tile's p . v starts from zero and joins the running sum in one rounding: the
+// matrix cores cut where they add.  The softmax is one pass over the keys with a running reference and sum in fp32.
+//
+//   - A tile is 16 rows (tokens times the heads that share a key head, so a decode step of 7 heads a key head fills 7 of them) by 64
+//     keys (fp32: 32).  S = K q^T, with keys as the matrix's rows: a lane then has 4 consecutive keys of one row, which are
+//     the weights' operand of p . v as they stand.
+//   - Few rows (attention_window_kernel): bytes bound.  A wave streams its own tiles, the next tile's keys and values on their way
+//     while one is worked on; the waves of a workgroup take tiles in turn and meet in LDS, and where there are few workgroups the keys
+//     are split over several, which meet in the one that ends last.  256 sequences of up to 4096 slots, fp16: 60 us, 4.5
+//     TB/s of keys and values (a large copy: 5.0); 64 of them 18.7 us; one of 131072 slots 20 us; two of 512 slots 6.9 us, of
+//     which 1.7 are an empty launch and the rest loads that wait for each other: position, table, keys, values.
+//   - Many rows (window_rows_kernel): bound by its products and the instructions around them.  A 16 x 64 tile of fp16 keys is 32
+//     matrix instructions of 16 cycles and about 400 cycles of others; they overlap by half.  One prompt of 8192 rows: 256 us, 470
+//     TFLOP/s counted as one product each of q k and p v (940 as computed, a large fp16 product: 1510).
+//   - Rows whose result is not finite, or without a weight, are computed once more by themselves, from their own keys alone
+//     (attend_wave): tiles hold slots that a row does not attend, whose NaN would reach it through a weight of zero.
 #include <algorithm>
 #include <atomic>
 #include <chrono>
@@ -451,7 +467,9 @@ __device__ __forceinline__ void join_parts(const WindowArgs &a, uint32_t b, uint
     }
 }
 
-// Few rows.  Grid: x the sequences' row tiles, y the key heads, z the parts.
+// Few rows.  Grid: x the sequences' row tiles, y the key heads, z the parts.  What a decode step spends beyond its bytes is loads that
+// wait for each other, so the table's entries and the query are requested before the position is known, and a wave holds the
+// places of its next 64 runs of slots, from loads made a round earlier.
 template <int CT, bool PAGED, int PIECES, bool APART, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) void attention_window_kernel(WindowArgs a) {
     typedef Kind<CT> KD;
@@ -703,7 +721,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
 // ------------------------------------------------------------- many rows --
 
 // Rows of prompts.  The WR waves of a workgroup have 16 rows each and share its tiles of keys in LDS, 16 bits a value (as NC pieces),
-// converted once.
+// converted once: a tile is worked on while the next is on its way, which needs one barrier a tile.  fp16 rows go from memory to LDS
+// by themselves, without passing registers: a prompt of 8192 rows took 310 us through registers (3 waves a SIMD), takes 274 us so, and
+// 256 us with the 4 waves a SIMD that the registers saved allow (4 through registers spill: slower than 3).  Tiles of 64 keys share
+// their two planes of 16 KB a stage; the values' operand is read transposed from LDS.
 typedef short s16x4v __attribute__((ext_vector_type(4)));
 constexpr uint32_t WR = 4;
 
@@ -724,11 +745,12 @@ __device__ __forceinline__ uint32_t chunk_at(uint32_t row, uint32_t c) {
 }
 
 template <int CT, bool PAGED>
-__global__ __launch_bounds__(64 * WR, 3) void window_rows_kernel(WindowArgs a) {
+__global__ __launch_bounds__(64 * WR, CT == DT_F16 ? 4 : 3) void window_rows_kernel(WindowArgs a) {
     typedef Kind<CT> KD;
     typedef Staged<CT> SD;
     constexpr uint32_t TK = SD::TK, ROW = Cached<CT>::ROW, SPAN = WR * 16;
     constexpr int NK = TK / 16, LOADS = 2 * SD::HALF / WR;
+    constexpr bool DIRECT = CT == DT_F16;
     static_assert(2 * SD::HALF % WR == 0, "whole loads a wave");
     __shared__ __attribute__((aligned(16))) char lds[2][2][SD::TILE];  // two tiles, keys and values of each
     const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
@@ -766,27 +788,35 @@ __global__ __launch_bounds__(64 * WR, 3) void window_rows_kernel(WindowArgs a) {
     auto spans = [&](uint32_t step, uint32_t entry) {
         return span_run<CT, PAGED, 16>(a, tl, kvh, slot_of(step), step + lane / SD::RUNS < steps, entry);
     };
+    // DIRECT: LDS takes a load's lanes side by side, so a lane fetches the chunk that belongs where it writes.  (What is past a span's
+    // bounds arrives as zeros there too.)
+    const uint32_t into = chunk_at(wr % 2 * SD::ROWS + lane / SD::CHUNKS, lane % SD::CHUNKS) % 128 + lane / SD::CHUNKS * 128;
     auto request = [&](const Spans &sp, uint32_t step) {
 #pragma unroll
         for (int j = 0; j < LOADS; j++) {
             const bool is_v = j * WR + wr >= SD::HALF;
             const uint32_t x = (j * WR + wr) % SD::HALF * SD::ROWS, i = step % EACH * SD::RUNS + x / 16, in = x % 16;  // the load's first row
             const uint32_t n = sp.rows(i), rows = n > in ? min(n - in, SD::ROWS) : 0;
-            raw[j] = __builtin_amdgcn_raw_buffer_load_b128(
-                span_of(static_cast<const char *>(pick(is_v, a.kv.k, a.kv.v)) + sp.at(i) + in * ROW, rows * ROW), 16 * lane, 0, 0);
+            const __amdgpu_buffer_rsrc_t from = span_of(static_cast<const char *>(pick(is_v, a.kv.k, a.kv.v)) + sp.at(i) + in * ROW, rows * ROW);
+            if constexpr (DIRECT)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)(lds[step & 1][is_v ? 1 : 0] + x * ROW), 16, into, 0, 0, 0);
+            else
+                raw[j] = __builtin_amdgcn_raw_buffer_load_b128(from, 16 * lane, 0, 0);
             if constexpr (CT == DT_F8)
                 scales[j] = __builtin_amdgcn_raw_buffer_load_b8(span_of(pick(is_v, a.kv.ks, a.kv.vs) + sp.scale(i) + in, rows), lane / SD::CHUNKS, 0, 0);
         }
     };
     auto store = [&](uint32_t buf) {
+        if constexpr (DIRECT) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < LOADS; j++) {
             const uint32_t id = j * WR + wr, x = id % SD::HALF * SD::ROWS + lane / SD::CHUNKS, c = lane % SD::CHUNKS;
             char *tile = lds[buf][id >= SD::HALF ? 1 : 0];
             const u32x4v w = raw[j];
-            if constexpr (CT == DT_F16) {
-                *reinterpret_cast<u32x4v *>(tile + chunk_at(x, c)) = w;
-            } else if constexpr (CT == DT_F8) {
+            if constexpr (CT == DT_F8) {
                 const float f = f8_pow2(scales[j]);
 #pragma unroll
                 for (int h = 0; h < 2; h++)
@@ -910,7 +940,10 @@ __global__ __launch_bounds__(64 * WR, 3) void window_rows_kernel(WindowArgs a) {
     const uint64_t bad64 = __ballot(have && !good), bad32 = bad64 | bad64 >> 32;
     uint32_t bad = static_cast<uint32_t>(bad32 | bad32 >> 16) & 0xFFFFu;
     if (have && !((bad >> l16) & 1)) {
-        float *p = a.out + row * a.ldo + head * 64 + 4 * g;
+        uint32_t own = r;
+        asm("" : "+v"(own));  // the address anew: held over the loop it would cost registers that the loop needs
+        const uint32_t to = by_group(a, own);
+        float *p = a.out + (static_cast<size_t>(b) * T + to) * a.ldo + (kvh * G + own - to * G) * 64 + 4 * g;
 #pragma unroll
         for (int d = 0; d < 4; d++) *reinterpret_cast<f32x4v *>(p + 16 * d) = m.o[d];
     }
@@ -961,7 +994,20 @@ static uint64_t new_tag() {
 }
 
 // Where the work goes, from the sizes alone: 256 compute units are an MI355X's, not asked for, so that a workspace sized once
-// fits wherever the call runs.
+// fits wherever the call runs.  Units are row tiles of 16, `own` the keys one attends at most.  Measured (fp16, 14 heads over 2 key
+// heads, us; the rule's side first):
+//   - Prompts' rows share LDS where there are workgroups of 64 rows for the chip: 64 prompts of 100 rows behind up to 1180 slots
+//     (960 workgroups) 46 against 63 with waves of their own; 8 of 130 (240) 19 against 26.  Between them, 16 of 130 (480), both take
+//     27 to 28; fp32 tiles are of 32 keys and cost their barriers more often: from 512 on.
+//   - A workgroup's waves share one row tile and split its keys: 8 of 130 rows 19, 2 waves a tile 22, one 32.  With more than four
+//     workgroups a compute unit and few keys to split, fewer waves a tile.
+//   - Eight waves where units leave compute units idle (96 sequences in a window of 1024: 10.9 against 12.3 with four), unless
+//     tiles are too few for them (20 rows at 128 slots: 5.9 against 6.4).
+//   - Keys split over workgroups: one sequence of 131072 slots in 64 parts 20, in 16 34, unsplit 369; two of 2048 in 8 parts 8.8
+//     against 11.5; 64 of 4096 in 2 parts 18.7 against 22.1.  Below about 1536 keys the meeting costs more than it gives: two of
+//     512 6.9 against 8.5 in two parts, 32 in a window of 512 8.0 against 10.2.
+//   - The workgroups of a sequence and key head go to one XCD where that spreads over all eight: four prompts of 701 rows in
+//     fp32 30.6 against 34.9.
 WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window, uint32_t sinks, int ct) {
     const uint64_t tk = ct == DT_F32 ? Raw<DT_F32>::TK : Raw<DT_F8>::TK, cus = 256;
     WindowPlan p{AW_WAVES, AW_WAVES, 1, 0, false, false};
@@ -983,7 +1029,7 @@ WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
         while (p.keys > 1 && groups(AW_FEW, p.keys) > 4 * cus && own < 4 * tk * p.keys) p.keys /= 2;
         return p;
     }
-    if (units > cus) p.waves = p.keys = AW_FEW;
+    if (units > cus || own <= AW_FEW * tk) p.waves = p.keys = AW_FEW;
     if (units <= 160 && own >= (ct == DT_F16 && units > 64 ? 2560 : 1536)) {
         const uint64_t tiles = (own + tk - 1) / tk;
         p.parts = static_cast<uint32_t>(std::min<uint64_t>({64, own / 256, std::max<uint64_t>(cus / units, own >= 8192 ? 4 : 2)}));

@@ -124,7 +124,7 @@ struct WindowArgs {
     uint32_t parts, run;  // parts of a row tile's keys, and the key tiles of each (the last: all that is left)
     uint32_t keys;        // waves of a workgroup that share rows and split their keys (the rest: other rows)
     uint32_t span;        // rows of a workgroup
-    uint32_t seq_tiles;   // workgroups of a sequence and key head, times parts
+    uint32_t seq_tiles;   // row tiles (workgroups of `span` rows) of a sequence and key head
     uint32_t shift;       // row tiles that a key head's and part's first workgroup is ahead of the one before
     bool by_xcd;          // rows of prompts: a sequence's and key head's workgroups on one XCD
     uint32_t group, group_magic;  // as in SharedArgs
@@ -133,9 +133,9 @@ struct WindowArgs {
 // How mt_attention_paged and mt_attention_sinks place their work (window_plan).
 struct WindowPlan {
     uint32_t waves, keys;  // waves of a workgroup, those that share rows and split their keys
-    uint32_t parts, run;   // parts of 1: one pass; more: joined by a second kernel
+    uint32_t parts, run;   // parts of 1: one pass; more: joined by the workgroup of a row tile that ends last; tiles of a part
     bool shared;           // rows of prompts: the waves share their keys in LDS
-    bool by_xcd;
+    bool by_xcd;           // and a sequence's and key head's workgroups go to one XCD
 };
 
 // How mt_attention_shared places its work (shared_plan).
