@@ -501,8 +501,8 @@ int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, ui
  * with MT_F8 also k_scale and v_scale [pages, hkv, page_len] bytes, 4-byte aligned, scale_stride bytes a page (a multiple of 4).
  * Slot s of sequence b is row s % page_len of page table[b table_stride + s / page_len] (device, uint32; table_len entries a
  * sequence, so it has table_len page_len slots, at most 2^30; table_stride is not read for one sequence).  page_len is a multiple
- * of 16 up to 32768.  An entry of `pages` or more (0xFFFFFFFF, say) is no page: nothing is read or written for its slots.  Entries
- * of slots that a call neither writes nor attends are not read for anything but that.  Several entries may name one page, such as
+ * of 16 up to 32768.  An entry of `pages` or more (0xFFFFFFFF, say) is no page: nothing is read or written for its slots.  What
+ * the entries of slots that a call neither writes nor attends hold does not matter.  Several entries may name one page, such as
  * a prompt that many sequences share; a page that one call appends to through two entries holds either's rows.  k, v and the
  * scales overlap neither each other nor the table; with one stride (in bytes) they may lie between each other, a page's keys and
  * values side by side.  B sequences of T rows, pos and counts are as at mt_kv.
@@ -534,15 +534,15 @@ int mt_rope_append_paged(const float *qkv, uint32_t ldq, uint32_t B, uint32_t T,
  * contiguous caches: row t of sequence b, at slot i = pos[b] + t (or the cache's last where that is past it), attends slots j <= i,
  * and where a window is given those of them with j > i - window or j < sinks (window 0 = all; then sinks has no effect).  So a
  * stream that runs past its window keeps its first positions, a voice prompt say, in sight, and the pages between them
- * and the window can be given back: their entries are not read.  q rows (stride ldq) hold hq heads of 64,
+ * and the window can be given back.  q rows (stride ldq) hold hq heads of 64,
  * already rotated; out rows stride ldo; scores scaled by `scale`, max-subtracted softmax; q and out 16-byte aligned with 16-byte
  * row strides, out apart from q and the caches.  Slots that a row does not attend do not reach its result, whatever they hold; nor do
  * slots without a page.  A NaN or +infinity among the scores that it does attend makes its head NaN; a score of -infinity is no
- * weight; a head without any weight is zeros.
+ * weight; a head without any weight is zeros.  Sums are fp32, of weights up to 1: values so large that they pass it give infinity.
  *
  * len_max (the caller's bound on max(pos[b] + counts[b]); 0: all slots) and the workspace are as at mt_attention_shared: len_max
- * only places the work, the workspace holds nothing between calls, and calls that may overlap need one each.  The workspace is
- * sized for the caches' type and the same B, T, hq, hkv, len_max (0: the number of slots), window and sinks.
+ * only places the work, the workspace holds nothing between calls, and calls that may overlap need one each.  It lies apart from q, out and the
+ * caches, and is sized for the caches' type and the same B, T, hq, hkv, len_max (0: the number of slots), window and sinks.
  */
 uint64_t mt_attention_window_workspace(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window,
                                        uint32_t sinks, mt_dtype cache_t);

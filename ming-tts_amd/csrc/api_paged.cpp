@@ -83,6 +83,11 @@ int attend(const char *who, WindowArgs &a, int ct, const Runs *caches, int n_cac
     if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return set_error(MT_EINVAL, "%s: needs %llu bytes of 16-byte aligned workspace, got %llu", who,
                          static_cast<unsigned long long>(need), static_cast<unsigned long long>(workspace ? workspace_bytes : 0));
+    if (need) {
+        bool met = meet(workspace, need, q, span(all, w, ldq, 4)) || meet(workspace, need, out, ob);
+        for (int i = 0; i < n_caches; i++) met = met || meet(workspace, need, caches[i].p, caches[i].all());
+        if (met) return set_error(MT_EINVAL, "%s: the workspace overlaps q, out or the caches", who);
+    }
     a.q = q;
     a.out = out;
     a.ldq = ldq;

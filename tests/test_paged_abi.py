@@ -139,6 +139,20 @@ def test_small_workspaces_are_refused(make):
         assert attend(kv, B=1, ws=ws, wsn=n) == mt.EINVAL and "workspace" in mt.last_error()
 
 
+@pytest.mark.parametrize("make", [paged, contiguous])
+@pytest.mark.parametrize("ws", [1024 * MB, 1536 * MB, A + 1 * MB, A + 65 * MB, A + 128 * MB, "table"])
+def test_workspaces_lie_apart(make, ws):
+    L = mt.load()
+    kv = make(table_len=8192, table_stride=8192, pages=8192) if make is paged else make(cache_len=1 << 17)
+    need = L.mt_attention_window_workspace(1, 1, 14, 2, 1 << 17, 0, 0, mt.F8)
+    assert need > 0
+    if ws == "table":
+        if make is contiguous:
+            return
+        ws = A + 130 * MB + 8192 * 4 - 16
+    assert attend(kv, B=1, ws=ws, wsn=need) == mt.EINVAL and "workspace overlaps" in mt.last_error()
+
+
 # ------------------------------------------------------------- Python --
 
 class Reached(Exception):
