@@ -220,8 +220,12 @@ int launch_append(const char *what, const float *qkv, uint32_t ldq, const RowsAr
     // One row a workgroup while that leaves CUs free; else two, which share the angles' set-up, where their heads fit 320 threads at
     // once (5280 rows of 16 ragged prompts, 14 + 2 x 2 heads: one row 10.7 us, two 10.5, four 10.9; 3200 rows of 16 + 2 x 16
     // heads: one 12.4, two 14.0).
-    const uint32_t per = all <= 512 || KV_ROWS * (hq + 2 * hkv) * 8 > 320 ? 1 : KV_ROWS;
-    const dim3 grid((all + per - 1) / per), block(append_threads(hq + 2 * hkv, per));
+    uint32_t per = all <= 512 || KV_ROWS * (hq + 2 * hkv) * 8 > 320 ? 1 : KV_ROWS, threads = append_threads(hq + 2 * hkv, per);
+    if (static_cast<uint64_t>(all / per + 1) * threads > 0xFFFFFFFFull) {  // more rows than such a launch holds: fewer threads for more of them
+        per = KV_ROWS;
+        threads = std::min<uint32_t>(threads, KV_THREADS);
+    }
+    const dim3 grid((all + per - 1) / per), block(threads);
     const int rc = check_grid(what, grid.x, block.x);
     if (rc) return rc;
     if (ct == DT_F32)

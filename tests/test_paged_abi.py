@@ -1,6 +1,9 @@
 """The paged and windowed entry points without a GPU: refusals before any HIP call, calls without work, and what the
 Python classes and calls check."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -137,6 +140,33 @@ def test_small_workspaces_are_refused(make):
         pytest.skip("this size is not split")
     for ws, n in ((None, need), (A, need - 1), (A + 8, need)):
         assert attend(kv, B=1, ws=ws, wsn=n) == mt.EINVAL and "workspace" in mt.last_error()
+
+
+APPEND = """
+import ctypes, sys
+sys.path[:0] = %r
+import mingtts as mt
+import test_paged_abi as t
+L, rows, heads = mt.load(), int(sys.argv[1]), int(sys.argv[2])
+kv = t.paged() if sys.argv[3] == "paged" else t.contiguous()
+call = L.mt_rope_append_paged if sys.argv[3] == "paged" else L.mt_rope_append
+a = (1 << 50, heads * 64, 1, rows, heads - 4, 2, None, None, 0, ctypes.byref(kv), t.A, None, 0, None)
+rc = call(*a)
+print(rc, mt.last_error())
+"""
+
+
+@pytest.mark.parametrize("which", ["paged", "contiguous"])
+@pytest.mark.parametrize("rows,heads", [(30_000_000, 64), (33_000_000, 18), (33_000_000, 20), (8_400_000, 255)])
+def test_many_rows_are_no_refusal(which, rows, heads):
+    """Appends of as many rows as 256 threads for two rows hold, by a process that sees no device: the launch fails, not the sizes."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = APPEND % [here, os.path.join(os.path.dirname(here), "ming-tts_amd")]
+    env = {**os.environ, "HIP_VISIBLE_DEVICES": "-1", "ROCR_VISIBLE_DEVICES": "-1"}
+    out = subprocess.run([sys.executable, "-c", code, str(rows), str(heads), which], env=env, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr
+    rc = int(out.stdout.split()[0])
+    assert rc < 0 and rc != mt.EINVAL, out.stdout
 
 
 @pytest.mark.parametrize("make", [paged, contiguous])
