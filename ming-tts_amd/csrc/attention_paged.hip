@@ -1008,7 +1008,7 @@ static uint64_t new_tag() {
 //     against 11.5; 64 of 4096 in 2 parts 18.7 against 22.1.  Below about 1536 keys the meeting costs more than it gives: two of
 //     512 6.9 against 8.5 in two parts, 32 in a window of 512 8.0 against 10.2.  A part costs the join its loads, a longer one its
 //     waves their rounds, so both grow with the root of the keys: one sequence of 16384 in 32 parts 12.2, in 64 14.3, of 65536 in 64
-//     of eight waves 16.7, of four 18.4.  Parts are whole rounds of their waves: 1600 slots in 7 parts of 4 tiles 9.0, in 5 of 5 9.8.
+//     of eight waves 16.7, of four 18.4.  fp32 tiles cost twice as much: from 512 keys on (1024: 9.1 against 14.1).  Parts are whole rounds of their waves: 1600 slots in 7 parts of 4 tiles 9.0, in 5 of 5 9.8.
 //   - The workgroups of a sequence and key head go to one XCD where that spreads over all eight: four prompts of 701 rows in
 //     fp32 30.6 against 34.9.
 WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window, uint32_t sinks, int ct) {
@@ -1033,11 +1033,12 @@ WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
         return p;
     }
     if (units > cus || own <= AW_FEW * tk) p.waves = p.keys = AW_FEW;
-    if (units <= 160 && own >= (ct == DT_F16 && units > 64 ? 2560 : 1536)) {
+    const uint64_t split = ct == DT_F32 ? (units > 32 ? 896 : 512) : units <= 64 ? 1536 : ct == DT_F16 ? 2560 : 2048;
+    if (units <= 160 && own >= split) {
         const uint64_t tiles = (own + tk - 1) / tk;
         const uint64_t even = static_cast<uint64_t>(std::sqrt(static_cast<double>(own / (ct == DT_F32 ? 8 : 16))));
         const uint64_t places = ct == DT_F16 && units <= 8 && own >= 16384 ? cus / 2 : cus;
-        const uint64_t parts = std::min<uint64_t>({64, own / 256, even, std::max<uint64_t>(places / units, own >= 8192 ? 4 : 2)});
+        const uint64_t parts = std::min<uint64_t>({64, own / (ct == DT_F32 ? 128 : 256), even, std::max<uint64_t>(places / units, own >= 8192 ? 4 : 2)});
         const uint64_t run = (tiles + parts - 1) / parts;
         const bool half = units * parts <= cus / 2;  // of the compute units have a part
         p.waves = p.keys = run * tk >= (half ? 512 : 1024) && (half || (ct != DT_F16 && units * parts <= cus)) ? AW_WAVES : AW_FEW;
