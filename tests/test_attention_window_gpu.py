@@ -92,6 +92,19 @@ def test_long_split_and_hints(gpu, kind, page):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B,T,hq,hkv,cap", [
+    (1, 1, 4, 1, 512), (3, 1, 4, 1, 700), (1, 1, 14, 2, 1600), (2, 3, 4, 2, 3000), (8, 1, 2, 1, 8192), (1, 1, 7, 1, 33000),
+    (33, 1, 2, 1, 2100), (40, 1, 4, 2, 1000), (70, 1, 2, 2, 2600), (150, 1, 1, 1, 2052), (5, 20, 2, 1, 1700),
+])
+def test_parts_of_many_sizes(gpu, kind, B, T, hq, hkv, cap):
+    """Keys split into few and many parts, of four waves and of eight, the last part shorter, sequences that end in the first."""
+    say(f"parts {kind} {B} {T} {cap}")
+    pos = [(cap - T, 5, cap // 2, 130)[b % 4] for b in range(B)]
+    c = Case(gpu, kind, B, T, hq, hkv, cap, page=64, pos=pos)
+    c.check(c.run(), rows={(b, t) for b in range(min(B, 12)) for t in range(T)})
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("page", [None, 32])
 @pytest.mark.parametrize("T", [1, 30])
 @pytest.mark.parametrize("scale,q_scale", [(0.125, 30.0), (-0.2, 3.0), (1.0, 1e-3), (1e-6, 1.0), (0.0, 1.0)])
