@@ -12,7 +12,8 @@
 //   - Eight lanes a head: lane r holds dims 4 r .. + 3 and 32 + 4 r .. + 3, both halves of its four
 //     pairs.  The block's largest value is three DPP steps, the codes two words a lane.
 //   - Bound: launch latency for a decode step's rows (3.0 us a call for two in a graph, an empty launch 1.7), the bytes of qkv and q
-//     for prompts (16 sequences of up to 330 rows, 34 MB: 10.5 us into pages of 8 bits; their copy to fp16 2.2-4).
+//     for prompts (16 sequences of up to 330 rows, 34 MB: 10.7 us into pages of 8 bits, 33 MB: 9.4 into contiguous caches; their
+//     copy to fp16 2.2-4).  The heads' values requested before the angles, or one head ahead: 3 to 13 % slower.
 #include <algorithm>
 
 #include "f8.hpp"
@@ -97,62 +98,47 @@ __global__ __launch_bounds__(KV_MOST) void rope_append_kernel(const float *qkv, 
     __shared__ double2 cs[KV_ROWS][32];
     const uint32_t tid = threadIdx.x, r = tid & 7, octets = blockDim.x / 8, all = rows.B * rows.T;
     const uint32_t row0 = blockIdx.x * per_group, n = min(per_group, all - row0), heads = hq + 2 * hkv;
-    // The octet's row and head, and its values, on their way before the angles are known.
-    uint32_t m = 0, h = 0, b = 0;
-    uint64_t slot = 0;
-    float4 lo = {}, hi = {};
-    Place at{};
-    bool there = false;
-    auto request = [&](uint32_t i) {
-        m = i / heads;
-        h = i - m * heads;
-        if (i >= n * heads || !rows.at(row0 + m, b, slot) || (h < hq && q == nullptr)) return false;
-        const float *src = qkv + static_cast<size_t>(row0 + m) * ldq + h * 64 + 4 * r;
-        lo = *reinterpret_cast<const float4 *>(src);
-        hi = *reinterpret_cast<const float4 *>(src + 32);
-        there = h >= hq && place(kv, b, slot, at);
-        return true;
-    };
-    uint32_t i = tid / 8;
-    bool have = request(i);
     for (uint32_t a = tid; a < n * 32; a += blockDim.x) {
-        uint32_t bt;
-        uint64_t st;
-        rows.at(row0 + a / 32, bt, st);
-        cs[a / 32][a & 31] = turn(st + offset, inv_freq[a & 31]);
+        uint32_t b;
+        uint64_t slot;
+        rows.at(row0 + a / 32, b, slot);
+        cs[a / 32][a & 31] = turn(slot + offset, inv_freq[a & 31]);
     }
     __syncthreads();
-    while (true) {
-        if (have) {
-            const bool is_q = h < hq;
-            float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-            if (h < hq + hkv) {
+    for (uint32_t i = tid / 8; i < n * heads; i += octets) {
+        const uint32_t m = i / heads, h = i - m * heads, row = row0 + m;
+        uint32_t b;
+        uint64_t slot;
+        if (!rows.at(row, b, slot)) continue;
+        const bool is_q = h < hq;
+        Place at;
+        if (is_q ? q == nullptr : !place(kv, b, slot, at)) continue;
+        const float *src = qkv + static_cast<size_t>(row) * ldq + h * 64 + 4 * r;
+        const float4 lo = *reinterpret_cast<const float4 *>(src), hi = *reinterpret_cast<const float4 *>(src + 32);
+        float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (h < hq + hkv) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const double2 t = cs[m][4 * r + e];
-                    const double a = x[e], b2 = x[4 + e];
-                    const double lo2 = fma(-b2, t.y, a * t.x), hi2 = fma(a, t.y, b2 * t.x);
-                    // (a NaN among the odd ones stays one; infinities are exact)
-                    x[e] = CT != DT_F32 && !is_q ? to_odd(lo2) : static_cast<float>(lo2);
-                    x[4 + e] = CT != DT_F32 && !is_q ? to_odd(hi2) : static_cast<float>(hi2);
-                }
-            }
-            if (is_q) {
-                float *dst = q + static_cast<size_t>(row0 + m) * ldo + h * 64 + 4 * r;
-                *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4 *>(dst + 32) = make_float4(x[4], x[5], x[6], x[7]);
-            } else if (there) {
-                const bool is_k = h < hq + hkv;
-                const size_t kh = is_k ? h - hq : h - hq - hkv;
-                constexpr size_t ES = CT == DT_F32 ? 4 : CT == DT_F16 ? 2 : 1;
-                char *cache = static_cast<char *>(is_k ? kv.k : kv.v) + at.row * ES;
-                uint8_t *scales = CT == DT_F8 ? (is_k ? kv.ks : kv.vs) + at.scale : nullptr;
-                store_row<CT>(x, cache, scales, kh * at.step, 4 * r, 32 + 4 * r, r);
+            for (int e = 0; e < 4; e++) {
+                const double2 t = cs[m][4 * r + e];
+                const double a = x[e], b2 = x[4 + e];
+                const double lo2 = fma(-b2, t.y, a * t.x), hi2 = fma(a, t.y, b2 * t.x);
+                // (a NaN among the odd ones stays one; infinities are exact)
+                x[e] = CT != DT_F32 && !is_q ? to_odd(lo2) : static_cast<float>(lo2);
+                x[4 + e] = CT != DT_F32 && !is_q ? to_odd(hi2) : static_cast<float>(hi2);
             }
         }
-        i += octets;
-        if (i >= n * heads) break;
-        have = request(i);
+        if (is_q) {
+            float *dst = q + static_cast<size_t>(row) * ldo + h * 64 + 4 * r;
+            *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4 *>(dst + 32) = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+            const bool is_k = h < hq + hkv;
+            const size_t kh = is_k ? h - hq : h - hq - hkv;
+            constexpr size_t ES = CT == DT_F32 ? 4 : CT == DT_F16 ? 2 : 1;
+            char *cache = static_cast<char *>(is_k ? kv.k : kv.v) + at.row * ES;
+            uint8_t *scales = CT == DT_F8 ? (is_k ? kv.ks : kv.vs) + at.scale : nullptr;
+            store_row<CT>(x, cache, scales, kh * at.step, 4 * r, 32 + 4 * r, r);
+        }
     }
 }
 
@@ -217,14 +203,13 @@ template <class KV>
 int launch_append(const char *what, const float *qkv, uint32_t ldq, const RowsArgs &rows, uint32_t hq, uint32_t hkv, uint32_t offset,
                   const KV &kv, int ct, const float *inv_freq, float *q, uint32_t ldo, hipStream_t stream) {
     const uint32_t all = rows.B * rows.T;
-    // One row a workgroup while that leaves CUs free; else two, which share the angles' set-up, where their heads fit 320 threads at
-    // once (5280 rows of 16 ragged prompts, 14 + 2 x 2 heads: one row 10.7 us, two 10.5, four 10.9; 3200 rows of 16 + 2 x 16
-    // heads: one 12.4, two 14.0).
-    uint32_t per = all <= 512 || KV_ROWS * (hq + 2 * hkv) * 8 > 320 ? 1 : KV_ROWS, threads = append_threads(hq + 2 * hkv, per);
-    if (static_cast<uint64_t>(all / per + 1) * threads > 0xFFFFFFFFull) {  // more rows than such a launch holds: fewer threads for more of them
-        per = KV_ROWS;
-        threads = std::min<uint32_t>(threads, KV_THREADS);
-    }
+    // One row a workgroup while that leaves CUs free; else two, which share the angles' set-up (5280 rows of 16 ragged prompts, 14 + 2
+    // x 2 heads, into pages: one row 10.7 us, two 10.5, four 10.9).  Threads for all their heads at once (2048 rows, contiguous caches: 5.0
+    // against 5.6 with 256), but 256 where that takes more than 320 (3200 rows of 16 + 2 x 16 heads: 11.3, one row each 12.4, two at
+    // once 14.0).
+    const uint32_t per = all <= 512 ? 1 : KV_ROWS, most = append_threads(hq + 2 * hkv, per);
+    const bool launchable = static_cast<uint64_t>(all / per + 1) * most <= 0xFFFFFFFFull;
+    const uint32_t threads = per > 1 && (most > 320 || !launchable) ? KV_THREADS : most;
     const dim3 grid((all + per - 1) / per), block(threads);
     const int rc = check_grid(what, grid.x, block.x);
     if (rc) return rc;
