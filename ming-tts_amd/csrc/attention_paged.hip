@@ -481,8 +481,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     __shared__ float ms[WAVES * 16], sums[WAVES * 16];
     const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t wk = wave % a.keys, wr = wave / a.keys;
-    const uint32_t G = a.group, T = a.rows.T, span = WAVES / a.keys * 16;  // rows of a workgroup
+    constexpr bool TWO = !APART && WAVES == AW_FEW;  // four waves may have two row tiles
+    const uint32_t keys = TWO ? a.keys : WAVES, wk = wave % keys, wr = wave / keys;
+    const uint32_t G = a.group, T = a.rows.T, span = WAVES / keys * 16;  // rows of a workgroup
 
     // The workgroup's rows [r0, r1) of sequence b's rows (t, head of the group), the longest first.
     // (A CU gets every 256th workgroup or so: each head and part begins at another sequence, or a CU would get all of a long one.)
@@ -501,7 +502,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     constexpr uint32_t EACH = 64 / PIECES, LEN = TK / PIECES;  // tiles whose spans a wave holds, slots of a piece
     uint32_t early = 0;
     if (PAGED && a.window == 0) {
-        const uint32_t tile = (APART ? blockIdx.z * a.run : 0) + wk + lane / PIECES * a.keys;
+        const uint32_t tile = (APART ? blockIdx.z * a.run : 0) + wk + lane / PIECES * keys;
         early = entry_of<PAGED>(a, b, tile * TK + lane % PIECES * LEN);  // (window_plan keeps it within 32 bits)
     }
     const uint64_t pos = a.rows.pos ? a.rows.pos[b] : 0u;
@@ -523,9 +524,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
     Raw<CT> raw;
     // The spans of EACH tiles of this wave, and the entries of the next ones.
     const uint32_t i0 = i;
-    auto slot_of = [&](uint32_t q) { return tl.at(min(i0 + (q + lane / PIECES) * a.keys, end - 1)) * TK + lane % PIECES * LEN; };
+    auto slot_of = [&](uint32_t q) { return tl.at(min(i0 + (q + lane / PIECES) * keys, end - 1)) * TK + lane % PIECES * LEN; };
     auto spans = [&](uint32_t q, uint32_t entry) {
-        return span_run<CT, PAGED, LEN>(a, tl, kvh, slot_of(q), i0 + (q + lane / PIECES) * a.keys < end, entry);
+        return span_run<CT, PAGED, LEN>(a, tl, kvh, slot_of(q), i0 + (q + lane / PIECES) * keys < end, entry);
     };
     Spans sp{};
     uint32_t q = 0, next_entry = 0;  // this wave's tiles so far
@@ -538,12 +539,12 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
         __builtin_amdgcn_sched_barrier(0);
         load_values<CT, PIECES>(raw, a, sp, 0, l16, g);
         __builtin_amdgcn_sched_barrier(0);
-        if (i + EACH * a.keys < end) next_entry = entry_of<PAGED>(a, b, slot_of(EACH));
+        if (i + EACH * keys < end) next_entry = entry_of<PAGED>(a, b, slot_of(EACH));
     }
     const Query<CT> qu = query_of<CT>(rq, a.scale);
 
     Sums m;
-    for (; i < end; i += a.keys, q++) {
+    for (; i < end; i += keys, q++) {
         const uint32_t k0 = tl.at(i) * TK, none = PAGED ? static_cast<uint32_t>(sp.holes >> (q % EACH * PIECES)) & ((1u << PIECES) - 1) : 0;
         turn_keys<CT>(raw, lds + wave * AREA, lane);
         f32x4v s[NK];
@@ -573,10 +574,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
             dots<CT, NK>(kf, qu.f[kk], s);
         }
         const uint32_t at = (q + 1) % EACH;
-        if (at == 0 && i + a.keys < end) {
+        if (at == 0 && i + keys < end) {
             sp = spans(q + 1, next_entry);
-            if (i + (1 + EACH) * a.keys < end) next_entry = entry_of<PAGED>(a, b, slot_of(q + 1 + EACH));
-        } else if (i + a.keys >= end) {
+            if (i + (1 + EACH) * keys < end) next_entry = entry_of<PAGED>(a, b, slot_of(q + 1 + EACH));
+        } else if (i + keys >= end) {
             sp.n = 0;
         }
         load_keys<CT, PIECES>(raw, a, sp, at * PIECES, lane);
@@ -658,7 +659,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
         if (r0 + (j & ~63u) / 16 >= r1) break;  // (whole waves)
         const uint32_t tj = by_group(a, rj), headj = kvh * G + rj - tj * G;
         const size_t row = static_cast<size_t>(b) * T + tj;
-        const uint32_t w0 = rr / 16 * a.keys, in = rr & 15;  // the row's waves, its place in each
+        const uint32_t w0 = rr / 16 * keys, in = rr & 15;  // the row's waves, its place in each
         float mk = INFINITY, l = 0.0f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         auto join = [&](auto count) {  // a count known here: all parts are read at once
@@ -685,9 +686,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 && CT != DT_F32 ? 3 : 2) voi
                 acc.w = fmaf(v[w].w, f, acc.w);
             }
         };
-        if (a.keys == WAVES) join(std::integral_constant<uint32_t, WAVES>{});
-        else if (a.keys == 2) join(std::integral_constant<uint32_t, 2>{});
-        else join(std::integral_constant<uint32_t, 1>{});
+        if (keys == WAVES) join(std::integral_constant<uint32_t, WAVES>{});
+        else if constexpr (TWO) join(std::integral_constant<uint32_t, WAVES / 2>{});
         if constexpr (APART) {
             if (rj < r1) {
                 const size_t at = (row * a.hq + headj) * a.parts + blockIdx.z;
@@ -1001,7 +1001,7 @@ static uint64_t new_tag() {
 //     (960 workgroups) 46 against 63 with waves of their own; 8 of 130 (240) 19 against 26.  Between them, 16 of 130 (480), both take
 //     27 to 28; fp32 tiles are of 32 keys and cost their barriers more often: from 512 on.
 //   - A workgroup's waves share one row tile and split its keys: 8 of 130 rows 19, 2 waves a tile 22, one 32.  With more than four
-//     workgroups a compute unit and few keys to split, fewer waves a tile.
+//     workgroups a compute unit and few keys to split, two waves a tile.
 //   - Eight waves where units leave compute units idle (96 sequences in a window of 1024: 10.9 against 12.3 with four), unless
 //     tiles are too few for them (20 rows at 128 slots: 5.9 against 6.4).
 //   - Keys split over workgroups: one sequence of 131072 slots in 64 parts 20, in 16 34, unsplit 369; two of 2048 in 8 parts 8.8
@@ -1029,7 +1029,8 @@ WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
     }
     if (rows > 16 && units > cus) {
         p.waves = p.keys = AW_FEW;
-        while (p.keys > 1 && groups(AW_FEW, p.keys) > 4 * cus && own < 4 * tk * p.keys) p.keys /= 2;
+        // (Two, not one: even with two there are no more than four workgroups a compute unit, where the rows would share LDS.)
+        if (units > 4 * cus && own < 4 * tk * AW_FEW) p.keys = 2;
         return p;
     }
     if (units > cus || own <= AW_FEW * tk) p.waves = p.keys = AW_FEW;
