@@ -542,7 +542,9 @@ int mt_rope_append_paged(const float *qkv, uint32_t ldq, uint32_t B, uint32_t T,
  *
  * len_max (the caller's bound on max(pos[b] + counts[b]); 0: all slots) and the workspace are as at mt_attention_shared: len_max
  * only places the work, the workspace holds nothing between calls, and calls that may overlap need one each.  It lies apart from q, out and the
- * caches, and is sized for the caches' type and the same B, T, hq, hkv, len_max (0: the number of slots), window and sinks.
+ * caches.  Its size is mt_attention_window_workspace of the caches' type and the call's B, T, hq, hkv, len_max, window and sinks, with the
+ * caches' number of slots (cache_len, or table_len page_len) in len_max's place where the call has 0 there: the query sees
+ * no caches, and 0 asks it for one key, which needs none.
  */
 uint64_t mt_attention_window_workspace(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window,
                                        uint32_t sinks, mt_dtype cache_t);

@@ -1,10 +1,13 @@
-"""The placement of attention over pages and windows without a GPU: which shapes of workgroups the rule can choose."""
+"""The placement of attention over pages and windows without a GPU: which shapes of workgroups the rule can choose, and the
+workspace that a call without a bound of its length needs."""
 import random
+import re
 
 import pytest
 
 import mingtts as mt
 from _window_plan import window_plan
+from test_paged_abi import attend, contiguous, paged
 
 TYPES = [mt.F32, mt.F16, mt.F8]
 
@@ -28,3 +31,22 @@ def test_shapes_of_workgroups(t):
         else:
             assert p.parts == 1
     assert seen == {(True, 4, 1, False), (False, 4, 2, False), (False, 4, 4, False), (False, 8, 8, False), (False, 4, 4, True), (False, 8, 8, True)}
+
+
+@pytest.mark.parametrize("make", [paged, contiguous])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50000, 100)])
+def test_workspace_without_a_bound(make, t, window, sinks):
+    """A call with len_max 0 needs the workspace that is asked for with the number of slots."""
+    kv = make(t=t, table_len=8192, table_stride=8192, pages=8192) if make is paged else make(t=t, cache_len=1 << 17)
+    need = mt.load().mt_attention_window_workspace(1, 1, 14, 2, 1 << 17, window, sinks, t)
+    assert need > 0
+    assert attend(kv, B=1, window=window, sinks=sinks) == mt.EINVAL
+    assert int(re.search(r"needs (\d+) bytes", mt.last_error()).group(1)) == need
+    assert attend(kv, B=1, window=window, sinks=sinks, ws=1 << 50, wsn=need - 1) == mt.EINVAL
+    assert "needs" in mt.last_error()
+
+
+def test_workspace_of_no_key_is_none():
+    """0 is no way to ask for all slots: the query does not know the caches."""
+    assert mt.load().mt_attention_window_workspace(1, 1, 14, 2, 0, 0, 0, mt.F16) == 0
