@@ -995,22 +995,41 @@ static uint64_t new_tag() {
 }
 
 // Where the work goes, from the sizes alone: 256 compute units are an MI355X's, not asked for, so that a workspace sized once
-// fits wherever the call runs.  Units are row tiles of 16, `own` the keys one attends at most.  Measured (fp16, 14 heads over 2 key
-// heads, us; the rule's side first):
+// fits wherever the call runs.  Units are row tiles of 16, `own` the keys one attends at most.  Measured in graphs, us, the rule's side
+// first: 14 heads over 2 key heads, so two units a sequence of a decode step, fp16 unless it is said; one sequence fills the cache, the
+// others are of any length up to that, or, in a skewed batch, up to 1000 slots.
 //   - Prompts' rows share LDS where there are workgroups of 64 rows for the chip: 64 prompts of 100 rows behind up to 1180 slots
-//     (960 workgroups) 46 against 63 with waves of their own; 8 of 130 (240) 19 against 26.  Between them, 16 of 130 (480), both take
-//     27 to 28; fp32 tiles are of 32 keys and cost their barriers more often: from 512 on.
+//     (1408 workgroups) 46 against 69 with waves of their own; 10 of 130 (300) 22 against 28.  In between, from 400 on, either side wins, by the
+//     prompts: 14 of 130 (420) 28.1 against 26.4, 16 (480) 26.5 against 27.5, two of 1000 behind 8000 (440) 152 against 147;
+//     8 bits, 18 of 130 (540) 37.5 against 35.0.  fp32 tiles are of 32 keys and cost their barriers more often, so from 512 on: four of
+//     701 in a window (528) 30 against 40, two of 1000 of 16 heads (512) 50 against 54, but 18 of 130 (540) 73 against 60; one of 2000
+//     of 16 heads (500) 96 against 115 shared.
 //   - A workgroup's waves share one row tile and split its keys: 8 of 130 rows 19, 2 waves a tile 22, one 32.  With more than four
 //     workgroups a compute unit and few keys to split, two waves a tile.
-//   - Eight waves where units leave compute units idle (96 sequences in a window of 1024: 10.9 against 12.3 with four), unless
-//     tiles are too few for them (20 rows at 128 slots: 5.9 against 6.4).
-//   - Keys split over workgroups: one sequence of 131072 slots in 64 parts 20, in 16 34, unsplit 369; two of 2048 in 8 parts 8.8
-//     against 11.5; 64 of 4096 in 2 parts 18.7 against 22.1.  Below about 1536 keys the meeting costs more than it gives: two of
-//     512 6.9 against 8.5 in two parts, 32 in a window of 512 8.0 against 10.2.  A part costs the join its loads, a longer one its
-//     waves their rounds, so both grow with the root of the keys: one sequence of 16384 in 32 parts 12.2, in 64 14.3, of 65536 in 64
-//     of eight waves 16.7, of four 18.4.  fp32 tiles cost twice as much: from 512 keys on (1024: 9.1 against 14.1).  Parts are whole rounds of their waves: 1600 slots in 7 parts of 4 tiles 9.0, in 5 of 5 9.8.
+//   - Eight waves where units leave compute units idle: 64 sequences of 1024 9.4 against 10.1 with four, 8 bits 8.9 against 10.0.  Four
+//     where they do not: 130 of 1024 12.6 against 14.0 (fp32 21.5 against 20.2); or where tiles are too few for eight: 20 rows
+//     at 128 slots 5.9 against 6.4, though a decode step's rows at 256 5.6 against 5.4.
+//   - Keys split over workgroups: one sequence of 131072 slots in 64 parts 20, in 32 23, unsplit 369.  Below some length the meeting costs
+//     more than it gives.  Up to 64 units 1536: one of 1536 8.6 against 9.1, of 1280 unsplit 8.3 against 8.5; 32 of 2048 10.9 against
+//     11.8, of 1536 10.5 against 10.3.  Above that 2560: 34 of 2560 12.5 against 13.1, 64 of 2560 14.2 against 14.0, of 2048
+//     unsplit 12.4 against 13.2; 8 bits 2048: 64 of 2048 12.3 against 12.8, of 1536 unsplit 10.9 against 11.8.  fp32 tiles cost
+//     twice as much: up to 32 units 512 (one of 512 8.5 against 9.1, of 384 unsplit 7.7 against 8.3), above that 896 (36 of 896 12.1 against
+//     12.9, 64 of 896 14.1 against 13.3, of 768 unsplit 12.5 against 12.8; 32 would gain from 512 on: 9.7 unsplit against 8.7).
+//   - As many parts as there are compute units for, but two at least, and four from 8192 keys on, for a batch with one long
+//     sequence: skewed, 64 sequences of 16384 take 26 in four parts and 40 in two, of 65536 73 and 136, where lengths spread evenly
+//     lose (64 of 16384 65 against 60, 40 54 against 42 in three).  At 129 to 160 units two parts cost such evenly spread lengths as
+//     well (80 of 4096 25 against 20 unsplit; skewed of 7168 24 against 26) and four gain in both (80 of 16384 86 against 92, skewed 27 against
+//     52).  Past 160 units none: evenly spread, 96 of 8192 51.2 against 52.5 in four, 128 60.1 against 62.5; but 8 bits (34.5 against
+//     30.9 for 96), fp32 (97 against 85) and skewed batches (96 of 16384 52 against 27, of 65536 187 against 74) would gain.
+//   - A part costs the join its loads, a longer one its waves their rounds, so both grow with the root of the keys, up to 64 parts before
+//     the rounding to whole rounds of their waves, which can make them more (76): one sequence of 131072 in 8 bits in 64 19.1, in 86 19.7;
+//     1600 slots in 7 parts of 4 tiles 9.0, in 5 of 5 9.8.  At least 256 keys a part, fp32 128 (1024 in 8 parts 8.6, in 4 10.0).
+//   - Eight waves a part where parts leave half the compute units idle and have 512 keys or more (one of 65536 16.3 against 18.0),
+//     or, not in fp16, leave none without one and have 1024 (8 bits, 32 of 8192 16.4 against 18.0; fp16 18.2 against 18.4 with eight).
+//     For up to 8 units of 16384 keys or more fp16 has half as many parts, of eight waves: two of 32768 14.0 against 15.3, of
+//     98304 21.0 against 23.8, though four of 131072, more than the caches on the chip keep, 52 against 38.
 //   - The workgroups of a sequence and key head go to one XCD where that spreads over all eight: four prompts of 701 rows in
-//     fp32 30.6 against 34.9.
+//     fp32 30.2 against 34.9 (32 of 130 in fp16 40 against 38.5); one prompt over two key heads stays spread, 44 against 121.
 WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32_t len_max, uint32_t window, uint32_t sinks, int ct) {
     const uint64_t tk = ct == DT_F32 ? Raw<DT_F32>::TK : Raw<DT_F8>::TK, cus = 256;
     WindowPlan p{AW_WAVES, AW_WAVES, 1, 0, false, false};
