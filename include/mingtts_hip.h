@@ -432,7 +432,8 @@ int mt_attention_decode(const float *q, uint32_t ldq, uint32_t B, uint32_t hq, u
  * (device, B uint32; NULL: zeros) gives each sequence's first row's slot in its own caches, so row t
  * stands at slot pos[b] + t; counts (device, B uint32; NULL: T each) how many of its T rows a
  * sequence brings.  Rows past that are padding: nothing is read, written or computed for them.
- * B T (hq + 2 hkv) must stay below 2^31, and in mt_attention_shared B T (hq / hkv)^2 below 2^32.
+ * B T (hq + 2 hkv) must stay below 2^31, and in mt_attention_shared, mt_attention_paged and mt_attention_sinks
+ * hq / hkv be at most 4096 and B T (hq / hkv)^2 below 2^32.
  * These and the matrices' sizes are bounded too by the 2^32 threads of a launch (else MT_EINVAL).
  */
 typedef struct mt_kv {
@@ -503,7 +504,8 @@ int mt_attention_shared(const float *q, uint32_t ldq, uint32_t B, uint32_t T, ui
  * sequence, so it has table_len page_len slots, at most 2^30; table_stride is not read for one sequence).  page_len is a multiple
  * of 16 up to 32768.  An entry of `pages` or more (0xFFFFFFFF, say) is no page: nothing is read or written for its slots.  What
  * the entries of slots that a call neither writes nor attends hold does not matter.  Several entries may name one page, such as
- * a prompt that many sequences share; a page that one call appends to through two entries holds either's rows.  k, v and the
+ * a prompt that many sequences share, but one call appends to a slot of a page through one entry only, unless the
+ * rows are equal: else the slot holds parts of either's row, and in 8 bits codes of one beside the scale of the other.  k, v and the
  * scales overlap neither each other nor the table; with one stride (in bytes) they may lie between each other, a page's keys and
  * values side by side.  B sequences of T rows, pos and counts are as at mt_kv.
  *

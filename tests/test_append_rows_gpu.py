@@ -1,5 +1,5 @@
 """Appends of more than 512 rows, two a workgroup, whose last workgroup has one: contiguous caches against 64 bits, pages against
-them, with the threads of few heads and of many."""
+them, with the threads of few heads and of many; and equal rows that go to one page through many tables."""
 import numpy as np
 import pytest
 import torch
@@ -44,3 +44,18 @@ def test_odd_numbers_of_rows(gpu, kind, case):
         for name in ("k", "v") + (("k_scale", "v_scale") if kind == "f8" else ()):
             flat = getattr(paged, name)[table[b].long()].transpose(0, 1).flatten(1, 2)  # [hkv, cap, ...]
             assert torch.equal(flat[:, slots], getattr(kv, name)[b][:, slots]), (name, b)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "f8"])
+def test_equal_rows_through_two_entries(gpu, kind):
+    """A prompt that every sequence appends for itself into the pages that all their tables name."""
+    B, T, hq, hkv = 40, 30, 2, 2
+    g = torch.Generator(device=gpu)
+    g.manual_seed(1)
+    one, inv = torch.randn(T, (hq + 2 * hkv) * 64, generator=g, device=gpu), torch.from_numpy(INV).to(gpu)
+    kvs = [mt.PagedKV.empty(4, hkv, 16, torch.tensor([[2, 0]] * n, dtype=torch.int32, device=gpu), TORCH[kind]) for n in (1, B)]
+    mt.rope_append_paged(one, 1, T, hq, hkv, None, kvs[0], inv)
+    mt.rope_append_paged(one.repeat(B, 1), B, T, hq, hkv, None, kvs[1], inv)
+    torch.cuda.synchronize()
+    for name in ("k", "v") + (("k_scale", "v_scale") if kind == "f8" else ()):
+        assert torch.equal(getattr(kvs[0], name), getattr(kvs[1], name)), name
