@@ -14,8 +14,8 @@
 //     the weights' operand of p . v as they stand.
 //   - Few rows (attention_window_kernel): bytes bound.  A wave streams its own tiles, the next tile's keys and values on their way
 //     while one is worked on; the waves of a workgroup take tiles in turn and meet in LDS, and where there are few workgroups the keys
-//     are split over several, which meet in the one that ends last.  256 sequences of up to 4096 slots, fp16: 60 us, 4.5
-//     TB/s of keys and values (a large copy: 5.0); 64 of them 18.7 us; one of 131072 slots 20 us; two of 512 slots 6.9 us, of
+//     are split over several, which meet in the one that ends last.  In a graph 256 sequences of up to 4096 slots take 61 us in
+//     fp16, 4.4 TB/s of keys and values (a large copy: 5.0); 64 of them 18.8; one of 131072 slots 20; two of 512 6.6, of
 //     which 1.7 are an empty launch and the rest loads that wait for each other: position, table, keys, values.
 //   - Many rows (window_rows_kernel): bound by its products and the instructions around them.  A 16 x 64 tile of fp16 keys is 32
 //     matrix instructions of 16 cycles and about 400 cycles of others; they overlap by half.  One prompt of 8192 rows: 256 us, 470
