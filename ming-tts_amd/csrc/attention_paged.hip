@@ -1025,7 +1025,7 @@ static uint64_t new_tag() {
 //     the rounding to whole rounds of their waves, which can make them more (76): one sequence of 131072 in 8 bits in 64 19.1, in 86 19.7;
 //     1600 slots in 7 parts of 4 tiles 9.0, in 5 of 5 9.8.  At least 256 keys a part, fp32 128 (1024 in 8 parts 8.6, in 4 10.0).
 //   - Eight waves a part where parts leave half the compute units idle and have 512 keys or more (one of 65536 16.3 against 18.0),
-//     or, not in fp16, leave none without one and have 1024 (8 bits, 32 of 8192 16.4 against 18.0; fp16 18.2 against 18.4 with eight).
+//     or, not in fp16, have a compute unit each and 1024 (8 bits, 32 of 8192 16.4 against 18.0; fp16 18.2 against 18.4 with eight).
 //     For up to 8 units of 16384 keys or more fp16 has half as many parts, of eight waves: two of 32768 14.0 against 15.3, of
 //     98304 21.0 against 23.8, though four of 131072, more than the caches on the chip keep, 52 against 38.
 //   - The workgroups of a sequence and key head go to one XCD where that spreads over all eight: four prompts of 701 rows in
@@ -1048,7 +1048,7 @@ WindowPlan window_plan(uint32_t B, uint32_t T, uint32_t hq, uint32_t hkv, uint32
     }
     if (rows > 16 && units > cus) {
         p.waves = p.keys = AW_FEW;
-        // (Two, not one: even with two there are no more than four workgroups a compute unit, where the rows would share LDS.)
+        // (Two are enough: rows that would be more than four workgroups a compute unit with two share LDS.)
         if (units > 4 * cus && own < 4 * tk * AW_FEW) p.keys = 2;
         return p;
     }

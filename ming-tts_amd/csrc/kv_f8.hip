@@ -11,9 +11,9 @@
 //     fp16 keys would be the wrong neighbour of a tie if it were rounded to fp32 first.
 //   - Eight lanes a head: lane r holds dims 4 r .. + 3 and 32 + 4 r .. + 3, both halves of its four
 //     pairs.  The block's largest value is three DPP steps, the codes two words a lane.
-//   - Bound: launch latency for a decode step's rows (3.0 us a call for two in a graph, an empty launch 1.7), the bytes of qkv and q
-//     for prompts (16 sequences of up to 330 rows, 34 MB: 10.7 us into pages of 8 bits, 33 MB: 9.4 into contiguous caches; their
-//     copy to fp16 2.2-4).  The heads' values requested before the angles, or one head ahead: 3 to 13 % slower.
+//   - Bound: launch latency for a decode step's rows (2.9 to 3.3 us a call for two in a graph, an empty launch 1.7), the bytes of
+//     qkv and q for prompts (16 sequences of up to 330 rows, 34 MB: 10.9 us into pages of 8 bits, 33 MB: 9.4 into contiguous caches;
+//     their copy to fp16 2.2-4).  The heads' values requested before the angles, or one head ahead: 3 to 13 % slower.
 #include <algorithm>
 
 #include "f8.hpp"
